@@ -16,12 +16,12 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DSQG_HIP_LIB", PKG_DIR / "libdsqg_hip.so"))
 
 MAX_OFFSETS = 64
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 DSQG_OK, DSQG_EINVAL, DSQG_EUNSUPPORTED, DSQG_EHIP, DSQG_EWORKSPACE = 0, 1, 2, 3, 4
 DSQG_ETOOLARGE = 5
 NOALLOC_SCRATCH_BYTES = 64 << 20  # DSQG_NOALLOC_SCRATCH_BYTES
-DSQG_F32, DSQG_BF16, DSQG_F16 = 0, 1, 2
+DSQG_F32, DSQG_BF16, DSQG_F16, DSQG_E4M3, DSQG_INT8 = 0, 1, 2, 3, 4
 
 _i64x4 = ctypes.c_int64 * 4
 _vp = ctypes.c_void_p
@@ -118,6 +118,36 @@ class LinearWgradArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+_i64x3 = ctypes.c_int64 * 3
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+                ("B", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("P", ctypes.c_int32), ("page", ctypes.c_int32), ("M", ctypes.c_int32),
+                ("k_pages", _vp), ("k_stride", _i64x3), ("v_pages", _vp), ("v_stride", _i64x3),
+                ("k_scale", _vp), ("k_scale_stride", _i64x3),
+                ("v_scale", _vp), ("v_scale_stride", _i64x3),
+                ("page_table", _vp), ("table_stride", ctypes.c_int64)]
+
+
+class PagedWriteArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCache), ("N", ctypes.c_int32),
+                ("k", _vp), ("k_stride", _i64x3), ("v", _vp), ("v_stride", _i64x3),
+                ("pos", _vp), ("counts", _vp)]
+
+
+class PagedReadArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCache), ("T", ctypes.c_int32), ("lengths", _vp), ("k", _vp), ("v", _vp)]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCache), ("H", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+                ("q", _vp), ("q_stride", _i64x2), ("k_new", _vp), ("k_new_stride", _i64x2),
+                ("v_new", _vp), ("v_new_stride", _i64x2), ("pos", _vp), ("out", _vp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 # Every symbol include/dsqg.h declares, with its ctypes signature.
 SIGNATURES = {
     "dsqg_abi_version": (ctypes.c_int, []),
@@ -144,6 +174,11 @@ SIGNATURES = {
     "dsqg_linear_wgrad_workspace_size": (ctypes.c_int, [ctypes.POINTER(LinearWgradArgs),
                                                         ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_linear_wgrad": (ctypes.c_int, [ctypes.POINTER(LinearWgradArgs), _vp]),
+    "dsqg_paged_write": (ctypes.c_int, [ctypes.POINTER(PagedWriteArgs), _vp]),
+    "dsqg_paged_read": (ctypes.c_int, [ctypes.POINTER(PagedReadArgs), _vp]),
+    "dsqg_paged_decode_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs),
+                                                        ctypes.POINTER(ctypes.c_size_t)]),
+    "dsqg_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs), _vp]),
 }
 
 _LIB = None

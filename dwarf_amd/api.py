@@ -13,6 +13,9 @@
   gradient comes back as one [B,N,3*H*HD] tensor.
 * ``causal_mean_pool_gate(x, gate_pre)`` -- the interference pool of a DWARF block,
   train/train_2048_condU.py:289-292: ``sigmoid(gate_pre) * x.cumsum(1) / counts``.
+* ``paged_kv_write`` / ``paged_decode_step`` / ``paged_kv_read`` and ``PagedKVCache`` -- full attention
+  over a paged key/value cache, of the rows' type or 8 bits wide (no counterpart in the reference,
+  whose full-attention layer, train/train_2048_condU.py:210-245, keeps no cache).
 
 The output [B,H,N,HD] is stored token-major ([B,N,H,HD] memory), so the callers'
 ``out.permute(0, 2, 1, 3).reshape(B, N, H * HD)`` (train/train_2048_condU.py:186) is a view.
@@ -194,6 +197,59 @@ def causal_mean_pool_gate(x: Tensor, gate_pre: Tensor) -> Tensor:
     return _lib.host().pool_gate(x, gate_pre)
 
 
+def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor, *,
+                   counts: Optional[Tensor] = None, k_scale: Optional[Tensor] = None,
+                   v_scale: Optional[Tensor] = None) -> None:
+    """Write row i of each sequence of k and v [B,Hkv,N,D] to position pos[b] + i of a paged cache, for
+    i < counts[b] (default: all N); every other row of the pages stays as it is.
+
+    k_pages, v_pages [P,Hkv,page,D] are pools of pages (page a power of two from 16) and page_table [B,M]
+    int32 names the page that holds positions page * j .. page * (j + 1) - 1 of each sequence.  Rows are
+    float32, bfloat16 or float16, and so are the pages, of the same type, or they are 8 bits wide
+    (float8_e4m3fn or int8) with k_scale, v_scale [P,Hkv,page] float8_e8m0fnu: a row's scale is the
+    smallest power of two that brings its largest magnitude to at most 448 or 127, and its values are
+    rounded once.  A row that holds an infinity or NaN reads as NaN from 8-bit pages.  Positions without
+    a page (a number that is none of the pool's, a position past the table) are not written.  No gradient
+    passes through the cache.
+    """
+    if ops.traced(k, v, k_pages, v_pages):
+        return ops.paged_kv_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
+    return _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
+
+
+def paged_kv_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor,
+                  max_len: Optional[int] = None, *, k_scale: Optional[Tensor] = None,
+                  v_scale: Optional[Tensor] = None, dtype: Optional[torch.dtype] = None):
+    """(k, v) [B,Hkv,max_len,D]: positions 0 .. lengths[b] - 1 of each sequence of a paged cache (see
+    ``paged_kv_write``), zeros behind them, NaN at a position without a page.  max_len defaults to the
+    table's positions, dtype to the pages' or, for 8-bit pages, bfloat16 (whose precision holds their values)."""
+    if max_len is None:
+        max_len = page_table.shape[1] * k_pages.shape[2]
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.element_size() == 1 else k_pages.dtype
+    if ops.traced(k_pages, v_pages, page_table):
+        return ops.paged_kv_read(k_pages, v_pages, page_table, lengths, max_len, dtype, k_scale, v_scale)
+    return _lib.host().paged_read(k_pages, v_pages, page_table, lengths, max_len, dtype, k_scale, v_scale)
+
+
+def paged_decode_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_pages: Tensor,
+                      v_pages: Tensor, page_table: Tensor, pos: Tensor, *, k_scale: Optional[Tensor] = None,
+                      v_scale: Optional[Tensor] = None, softmax_scale: Optional[float] = None) -> Tensor:
+    """One decode step over a paged cache (see ``paged_kv_write``): k_new, v_new [B,Hkv,D] go to position
+    pos[b], and the H = Hkv * G query heads q [B,H,D] attend positions 0 .. pos[b] (query head h the
+    key/value head h // G); returns out [B,H,D].
+
+    softmax_scale defaults to D ** -0.5.  With k_new = v_new = None nothing is written and position
+    pos[b] is attended as the pages hold it.  A sequence with pos[b] < 0 attends nothing and gets zeros;
+    one that attends a position without a page gets NaN.  Sums are fp32 and the result does not change
+    from call to call.  The step has no gradient.
+    """
+    if ops.traced(q, k_pages, v_pages):
+        return ops.paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale)
+    return _lib.host().paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale,
+                                    softmax_scale)
+
+
 class DSQGRingCache:
     """Per-layer O(1) decode cache: K/V rings of S = max(offset)+1 slots (README.md:175-179).
 
@@ -231,3 +287,69 @@ class DSQGRingCache:
                                if_gain=if_gain)
         self.pos += 1
         return out
+
+
+class PagedKVCache:
+    """Key/value cache of one full-attention layer for B sequences of up to ``max_len`` positions, in pages
+    (see ``paged_kv_write``), each sequence at a position of its own (``pos`` [B], on the device).
+
+    ``dtype`` is the type of the rows and, unless ``kv_dtype`` (torch.float8_e4m3fn or torch.int8) asks for
+    8 bits, of the pages.  ``prefill(k, v)`` loads a prompt, ``write(k, v)`` appends rows, ``step(q, k_t,
+    v_t)`` runs one decode step and advances, ``read()`` returns the rows.  Every sequence owns its pages,
+    sequence b those from b * M on; a caller that shares or moves pages sets ``page_table``.  The host
+    does not know the positions: rows past a sequence's last page are not kept, and its steps give NaN.
+    """
+
+    def __init__(self, B: int, H: int, D: int, max_len: int, dtype=torch.bfloat16, device="cuda",
+                 kv_dtype: Optional[torch.dtype] = None, page_size: int = 64):
+        assert max_len >= 1, f"max_len must be positive, got {max_len}"
+        assert D in _lib.supported_head_dims(), f"head dim {D} is none of {_lib.supported_head_dims()}"
+        assert kv_dtype in (None, dtype, torch.float8_e4m3fn, torch.int8), \
+            f"kv_dtype must be float8_e4m3fn, int8 or the rows' {dtype}, got {kv_dtype}"
+        self.dtype = dtype
+        self.max_len = int(max_len)
+        M = -(-self.max_len // page_size)
+        shape = (B * M, H, page_size, D)
+        kv = kv_dtype or dtype
+        self.k_pages = torch.zeros(shape, dtype=kv, device=device)
+        self.v_pages = torch.zeros_like(self.k_pages)
+        self.k_scale = self.v_scale = None
+        if self.k_pages.element_size() == 1:
+            self.k_scale = torch.zeros(shape[:3], dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+            self.v_scale = torch.zeros_like(self.k_scale)
+        self.page_table = torch.arange(B * M, dtype=torch.int32, device=device).view(B, M)
+        self.pos = torch.zeros((B,), dtype=torch.int64, device=device)
+
+    def _state(self):
+        return dict(k_scale=self.k_scale, v_scale=self.v_scale)
+
+    def prefill(self, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
+        """Write prompts k, v [B,H,N,D] from position 0 on, counts[b] rows of each (default: N); pos becomes
+        that."""
+        assert k.shape[2] <= self.max_len, f"prompt of {k.shape[2]} rows exceeds the cache ({self.max_len})"
+        self.pos.zero_()
+        self.write(k, v, counts)
+
+    def write(self, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
+        """Append rows k, v [B,H,N,D], counts[b] of each (default: N), and advance."""
+        k, v = k.detach().to(self.dtype), v.detach().to(self.dtype)
+        if counts is not None:
+            counts = counts.clamp(0, k.shape[2])
+        paged_kv_write(k, v, self.k_pages, self.v_pages, self.page_table, self.pos, counts=counts, **self._state())
+        self.pos += k.shape[2] if counts is None else counts
+
+    def step(self, q: Tensor, k_new: Tensor, v_new: Tensor, softmax_scale: Optional[float] = None) -> Tensor:
+        """Output [B,H*G,D] of one new token per sequence at its position, which advances."""
+        dt = self.dtype
+        out = paged_decode_step(q.detach().to(dt), k_new.detach().to(dt), v_new.detach().to(dt), self.k_pages,
+                                self.v_pages, self.page_table, self.pos, softmax_scale=softmax_scale,
+                                **self._state())
+        self.pos += 1
+        return out.to(q.dtype)
+
+    def read(self, max_len: Optional[int] = None, dtype: Optional[torch.dtype] = None):
+        """(k, v) [B,H,max_len,D] (default: the cache's max_len) of the positions written so far, zeros
+        behind them, in the rows' dtype or another."""
+        return paged_kv_read(self.k_pages, self.v_pages, self.page_table, self.pos,
+                             self.max_len if max_len is None else max_len, dtype=dtype or self.dtype,
+                             **self._state())

@@ -40,6 +40,10 @@ struct Api {
   decltype(&dsqg_pool_gate_bwd) pool_bwd = nullptr;
   decltype(&dsqg_linear_wgrad_workspace_size) linear_workspace_size = nullptr;
   decltype(&dsqg_linear_wgrad) linear_wgrad = nullptr;
+  decltype(&dsqg_paged_write) paged_write = nullptr;
+  decltype(&dsqg_paged_read) paged_read = nullptr;
+  decltype(&dsqg_paged_decode_workspace_size) paged_decode_workspace_size = nullptr;
+  decltype(&dsqg_paged_decode) paged_decode = nullptr;
   PyObject* library_error = nullptr;  // dwarf_amd._lib.DSQGLibraryError
 } api;
 
@@ -774,6 +778,195 @@ Tensor linear(const Tensor& x0, const Tensor& w0, const OptTensor& b0) {
   return LinearFunction::apply(x, w0.to(dt), OptTensor(w0), b0);
 }
 
+// ---- Paged key/value cache. -------------------------------------------------------------------------------------
+
+// A cache's tensors, checked, and their argument block (for tensors of the type dt on the caller's side).
+// The pools are taken as they are (they are written in place); the small tensors are kept alive here.
+struct Paged {
+  dsqg_paged_cache a = {};
+  c10::Device dev{c10::kCPU};
+  Tensor table;
+
+  Paged(const Tensor& k, const Tensor& v, const Tensor& table0, const OptTensor& ks0, const OptTensor& vs0, at::ScalarType dt,
+        bool written) {
+    const auto ct = k.scalar_type();
+    const bool narrow = ct == at::kFloat8_e4m3fn || ct == at::kChar;
+    require(k.dim() == 4, "k_pages must be [P,H,page,D], got ", shape_str(k.sizes()));
+    require(v.sizes() == k.sizes() && v.scalar_type() == ct, "k_pages and v_pages must have the same shape and dtype");
+    require(narrow || ct == at::kFloat || ct == at::kBFloat16 || ct == at::kHalf,
+            "pages must be float32, bfloat16, float16, float8_e4m3fn or int8, got ", ct);
+    require(dt == at::kFloat || dt == at::kBFloat16 || dt == at::kHalf, "rows must be float32, bfloat16 or float16, got ", dt);
+    require(ks0.has_value() == narrow && vs0.has_value() == narrow,
+            narrow ? "8-bit pages need k_scale and v_scale" : "k_scale and v_scale are for 8-bit pages");
+    const int64_t P = k.size(0), H = k.size(1), page = k.size(2), D = k.size(3);
+    require(page >= 16 && page <= 65536 && (page & (page - 1)) == 0, "page size must be a power of two from 16 to 65536, got ", page);
+    require(table0.dim() == 2 && table0.scalar_type() == at::kInt, "page_table must be an int32 [B,M] tensor");
+    for (const Tensor* s : {narrow ? &*ks0 : nullptr, narrow ? &*vs0 : nullptr})
+      if (s)
+        require(s->sizes() == c10::IntArrayRef({P, H, page}) && s->scalar_type() == at::kFloat8_e8m0fnu,
+                "scales must be float8_e8m0fnu ", shape_str({P, H, page}), " tensors, got ", shape_str(s->sizes()));
+    dev = require_gpu({&k, &v, &table0});
+    if (narrow) dev = require_gpu({&k, &*ks0, &*vs0});
+    const bool inference = c10::InferenceMode::is_enabled();
+    for (const Tensor* t : {&k, &v, narrow ? &*ks0 : nullptr, narrow ? &*vs0 : nullptr}) {
+      if (!t) continue;
+      require(!t->is_neg(), "a cache tensor must not be a lazily negated view");
+      if (written && t->is_inference() && !inference)
+        raise(PyExc_RuntimeError, "Inplace update to inference tensor outside InferenceMode is not allowed");
+    }
+    require(P < (1ll << 31) && H <= 65535 && table0.size(0) <= 65535 && table0.size(1) * page < (1ll << 31),
+            "a cache has at most 65535 sequences, 65535 heads and 2^31 positions of a sequence");
+    const int64_t es = k.element_size();
+    for (const Tensor* t : {&k, &v}) {
+      bool ok = t->numel() == 0 || (t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0);
+      for (int i = 0; ok && t->numel() && i < 3; ++i) ok = t->stride(i) * es % 16 == 0;
+      require(ok, "pages must have unit inner stride and 16-byte aligned rows");
+    }
+    table = table0.stride(1) == 1 || table0.size(1) <= 1 ? table0 : table0.contiguous();
+    auto code = [](at::ScalarType t) {
+      return t == at::kFloat ? DSQG_F32 : t == at::kBFloat16 ? DSQG_BF16 : t == at::kHalf ? DSQG_F16 : t == at::kChar ? DSQG_INT8 : DSQG_E4M3;
+    };
+    a.dtype = code(dt);
+    a.cache_dtype = code(ct);
+    a.B = (int32_t)table.size(0); a.Hkv = (int32_t)H; a.D = (int32_t)D;
+    a.P = (int32_t)P; a.page = (int32_t)page; a.M = (int32_t)table.size(1);
+    a.k_pages = ptr(k); a.v_pages = ptr(v);
+    // (A dimension of one entry may have any stride.)
+    auto strides = [](int64_t (&dst)[3], const Tensor& t) {
+      for (int i = 0; i < 3; ++i) dst[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    };
+    strides(a.k_stride, k); strides(a.v_stride, v);
+    if (narrow) {
+      a.k_scale = static_cast<uint8_t*>(ptr(*ks0)); a.v_scale = static_cast<uint8_t*>(ptr(*vs0));
+      strides(a.k_scale_stride, *ks0); strides(a.v_scale_stride, *vs0);
+    }
+    a.page_table = static_cast<const int32_t*>(ptr(table));
+    a.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
+  }
+
+  // [B] positions or counts as the kernels read them.
+  Tensor index(const Tensor& t, const char* name) const {
+    require(at::isIntegralType(t.scalar_type(), false) && t.dim() == 1 && t.size(0) == a.B, name, " must be an integer [", a.B,
+            "] tensor, got ", shape_str(t.sizes()));
+    if (t.device() != dev)
+      raise(PyExc_RuntimeError, c10::str("tensors on different devices: ", dev, " and ", t.device()));
+    return t.to(at::kLong).contiguous();
+  }
+};
+
+// No gradient passes through a cache: a call that records one is refused.
+void refuse_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad())
+      raise(PyExc_RuntimeError, "the paged cache has no gradient: detach its operands, or call it under torch.no_grad()");
+}
+
+void cache_changed(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor plain_rows(const Tensor& t) { return rows_ready(t.is_neg() ? t.resolve_neg() : t); }
+
+void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& pos0,
+                 const OptTensor& counts0, const OptTensor& ks, const OptTensor& vs) {
+  py::gil_scoped_release nogil;
+  refuse_grad({&k0, &v0, &kp, &vp});
+  require(k0.dim() == 4 && v0.sizes() == k0.sizes(), "k and v must be [B,H,N,D] of the same shape, got ", shape_str(k0.sizes()),
+          " and ", shape_str(v0.sizes()));
+  const auto dt = k0.scalar_type();
+  require(v0.scalar_type() == dt, "k and v must share a dtype, got ", dt, " and ", v0.scalar_type());
+  Paged c(kp, vp, table, ks, vs, dt, true);
+  require(ks.has_value() || kp.scalar_type() == dt, "rows of ", dt, " do not go into pages of ", kp.scalar_type());
+  require(k0.size(0) == c.a.B && k0.size(1) == c.a.Hkv && k0.size(3) == c.a.D, "k and v must be [", c.a.B, ",", c.a.Hkv, ",N,", c.a.D,
+          "], got ", shape_str(k0.sizes()));
+  require_gpu({&kp, &k0, &v0});
+  const c10::OptionalDeviceGuard guard(c.dev);
+  const Tensor k = plain_rows(k0), v = plain_rows(v0), pos = c.index(pos0, "pos");
+  const Tensor counts = counts0 ? c.index(*counts0, "counts") : Tensor();
+  dsqg_paged_write_args a = {};
+  a.cache = c.a;
+  a.N = (int32_t)k.size(2);
+  require(k.size(2) < (1ll << 31), "k and v have too many rows: ", k.size(2));
+  a.k = ptr(k); a.v = ptr(v);
+  for (int i = 0; i < 3; ++i) { a.k_stride[i] = k.stride(i); a.v_stride[i] = v.stride(i); }
+  a.pos = static_cast<const int64_t*>(ptr(pos));
+  a.counts = static_cast<const int64_t*>(ptr(counts));
+  check(api.paged_write(&a, stream_of(c.dev)), "dsqg_paged_write");
+  cache_changed({&kp, &vp});
+  if (ks) cache_changed({&*ks, &*vs});
+}
+
+std::tuple<Tensor, Tensor> paged_read(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths0, int64_t T,
+                                      at::ScalarType dt, const OptTensor& ks, const OptTensor& vs) {
+  py::gil_scoped_release nogil;
+  refuse_grad({&kp, &vp});
+  Paged c(kp, vp, table, ks, vs, dt, false);
+  require(T >= 0 && T < (1ll << 31), "max_len must be from 0 to 2^31 - 1, got ", T);
+  const c10::OptionalDeviceGuard guard(c.dev);
+  const Tensor lengths = c.index(lengths0, "lengths");
+  const auto o = kp.options().dtype(dt);
+  const Tensor k = at::empty({c.a.B, c.a.Hkv, T, c.a.D}, o), v = at::empty({c.a.B, c.a.Hkv, T, c.a.D}, o);
+  dsqg_paged_read_args a = {};
+  a.cache = c.a;
+  a.T = (int32_t)T;
+  a.lengths = static_cast<const int64_t*>(ptr(lengths));
+  a.k = ptr(k); a.v = ptr(v);
+  check(api.paged_read(&a, stream_of(c.dev)), "dsqg_paged_read");
+  return {k, v};
+}
+
+Tensor paged_decode(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, const Tensor& kp, const Tensor& vp, const Tensor& table,
+                    const Tensor& pos0, const OptTensor& ks, const OptTensor& vs, std::optional<double> scale) {
+  py::gil_scoped_release nogil;
+  const Tensor kn = undef(k0), vn = undef(v0);
+  refuse_grad({&q0, &kn, &vn, &kp, &vp});
+  const auto dt = q0.scalar_type();
+  require(q0.dim() == 3, "q must be [B,H,D], got ", shape_str(q0.sizes()));
+  require(kn.defined() == vn.defined(), "k_new and v_new go together");
+  Paged c(kp, vp, table, ks, vs, dt, kn.defined());
+  require(ks.has_value() || kp.scalar_type() == dt, "queries of ", dt, " do not go with pages of ", kp.scalar_type());
+  const int64_t B = c.a.B, Hkv = c.a.Hkv, D = c.a.D, H = q0.size(1);
+  require(q0.size(0) == B && q0.size(2) == D && (Hkv > 0 ? H % Hkv == 0 : H == 0), "q must be [", B, ",H,", D,
+          "] with H a multiple of ", Hkv, ", got ", shape_str(q0.sizes()));
+  for (const Tensor* t : {&kn, &vn})
+    if (t->defined())
+      require(t->sizes() == c10::IntArrayRef({B, Hkv, D}) && t->scalar_type() == dt, "k_new and v_new must be ", dt, " ",
+              shape_str({B, Hkv, D}), " tensors, got ", t->scalar_type(), " ", shape_str(t->sizes()));
+  require_gpu({&kp, &q0, &kn, &vn});
+  const c10::OptionalDeviceGuard guard(c.dev);
+  const Tensor q = plain_rows(q0), pos = c.index(pos0, "pos");
+  const Tensor out = at::empty({B, H, D}, q0.options());
+  dsqg_paged_decode_args a = {};
+  a.cache = c.a;
+  a.H = (int32_t)H;
+  a.softmax_scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
+  a.q = ptr(q);
+  const Tensor k = kn.defined() ? plain_rows(kn) : kn, v = vn.defined() ? plain_rows(vn) : vn;
+  if (kn.defined()) { a.k_new = ptr(k); a.v_new = ptr(v); }
+  for (int i = 0; i < 2; ++i) {
+    a.q_stride[i] = q.stride(i);
+    if (kn.defined()) { a.k_new_stride[i] = k.stride(i); a.v_new_stride[i] = v.stride(i); }
+  }
+  a.pos = static_cast<const int64_t*>(ptr(pos));
+  a.out = ptr(out);
+  size_t nbytes = 0;
+  check(api.paged_decode_workspace_size(&a, &nbytes), "dsqg_paged_decode_workspace_size");
+  Tensor ws;
+  if (nbytes) {
+    ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = nbytes;
+  }
+  check(api.paged_decode(&a, stream_of(c.dev)), "dsqg_paged_decode");
+  if (kn.defined()) {
+    cache_changed({&kp, &vp});
+    if (ks) cache_changed({&*ks, &*vs});
+  }
+  return out;
+}
+
 void init(const py::dict& addresses, const py::object& library_error) {
   auto get = [&](auto& fn, const char* name) {
     fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addresses[name].cast<uintptr_t>());
@@ -790,6 +983,10 @@ void init(const py::dict& addresses, const py::object& library_error) {
   get(api.pool_bwd, "dsqg_pool_gate_bwd");
   get(api.linear_workspace_size, "dsqg_linear_wgrad_workspace_size");
   get(api.linear_wgrad, "dsqg_linear_wgrad");
+  get(api.paged_write, "dsqg_paged_write");
+  get(api.paged_read, "dsqg_paged_read");
+  get(api.paged_decode_workspace_size, "dsqg_paged_decode_workspace_size");
+  get(api.paged_decode, "dsqg_paged_decode");
   api.library_error = library_error.inc_ref().ptr();  // lives as long as the process
 }
 
@@ -805,4 +1002,7 @@ PYBIND11_MODULE(_dsqg_host, m) {
   m.def("ring_load", &ring_load);
   m.def("pool_gate", &pool_gate);
   m.def("linear", &linear);
+  m.def("paged_write", &paged_write);
+  m.def("paged_read", &paged_read);
+  m.def("paged_decode", &paged_decode);
 }

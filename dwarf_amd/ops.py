@@ -1,5 +1,6 @@
 """torch custom ops over the C ABI: ``dwarf::dsqg_fwd``, ``dwarf::dsqg_fwd_qkv``, ``dwarf::dsqg_bwd``,
-``dwarf::dsqg_decode``, and the interference pool ``dwarf::pool_gate_fwd`` / ``_bwd``.
+``dwarf::dsqg_decode``, the interference pool ``dwarf::pool_gate_fwd`` / ``_bwd``, and the paged cache's
+``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``.
 
 The ops take device tensors, pass raw pointers, element strides and the current HIP stream
 to libdsqg_hip.so through ctypes, and allocate their outputs (and the backward workspace) with
@@ -653,3 +654,48 @@ def _pool_backward(ctx, dout):
 torch.library.register_autograd("dwarf::pool_gate_fwd", _pool_backward,
                                 setup_context=_pool_setup_context)
 
+
+
+# ------------------------------------------------------------------------------------------
+# Paged key/value cache (no gradients; the calls and their checks are the native host layer's)
+# ------------------------------------------------------------------------------------------
+
+@torch.library.custom_op("dwarf::paged_kv_write", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor,
+                   counts: Optional[Tensor], k_scale: Optional[Tensor], v_scale: Optional[Tensor]) -> None:
+    """Rows of k and v [B,H,N,D] to positions pos .. pos + counts - 1 of the pages."""
+    _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
+
+
+@paged_kv_write.register_fake
+def _(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op("dwarf::paged_kv_read", mutates_args=())
+def paged_kv_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor, max_len: int,
+                  dtype: torch.dtype, k_scale: Optional[Tensor],
+                  v_scale: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    """k and v [B,H,max_len,D] of the pages, zeros behind each sequence's length."""
+    return _lib.host().paged_read(k_pages, v_pages, page_table, lengths, max_len, dtype, k_scale, v_scale)
+
+
+@paged_kv_read.register_fake
+def _(k_pages, v_pages, page_table, lengths, max_len, dtype, k_scale, v_scale):
+    _, H, _, D = k_pages.shape
+    shape = (page_table.shape[0], H, max_len, D)
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("dwarf::paged_decode", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def paged_decode(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_pages: Tensor, v_pages: Tensor,
+                 page_table: Tensor, pos: Tensor, k_scale: Optional[Tensor], v_scale: Optional[Tensor],
+                 softmax_scale: Optional[float]) -> Tensor:
+    """out [B,H,D] of one new token per sequence; its row goes to the pages."""
+    return _lib.host().paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale,
+                                    softmax_scale)
+
+
+@paged_decode.register_fake
+def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale):
+    return q.new_empty(q.shape)

@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DSQG_ABI_VERSION 4
+#define DSQG_ABI_VERSION 5
 #define DSQG_MAX_OFFSETS 64
 
 /* Same type as hipStream_t; NULL is the null stream. */
@@ -70,8 +70,9 @@ typedef enum {
  * D64 and the 44-offset table with dscale_embed, 10 MB without). */
 #define DSQG_NOALLOC_SCRATCH_BYTES (64u << 20)
 
-/* DSQG_F16 is accepted by the pool entry points only. */
-typedef enum { DSQG_F32 = 0, DSQG_BF16 = 1, DSQG_F16 = 2 } dsqg_dtype;
+/* The attention over fixed offsets takes the first two; the entry points that say so take DSQG_F16, and
+ * a paged cache also holds the 8-bit types (float8 e4m3 without infinities, and int8). */
+typedef enum { DSQG_F32 = 0, DSQG_BF16 = 1, DSQG_F16 = 2, DSQG_E4M3 = 3, DSQG_INT8 = 4 } dsqg_dtype;
 
 /* Shape and offset table shared by all entry points. */
 typedef struct {
@@ -317,6 +318,94 @@ typedef struct {
 
 int dsqg_linear_wgrad_workspace_size(const dsqg_linear_wgrad_args* args, size_t* bytes);
 int dsqg_linear_wgrad(const dsqg_linear_wgrad_args* args, dsqg_stream_t stream);
+
+/* A paged key/value cache of one layer (for full attention; train/train_2048_condU.py:210-245 keeps
+ * none and recomputes the prefix).  k_pages and v_pages are pools [P, Hkv, page, D]; page_table [B, M]
+ * says which page of the pools holds positions page * j .. page * (j + 1) - 1 of each sequence, so a
+ * sequence has M * page positions at most.  Several sequences may share a page that none of them
+ * writes.
+ *
+ * cache_dtype is dtype (that of the rows, queries and outputs) or an 8-bit type.  A row of an 8-bit
+ * pool has a byte in k_scale / v_scale [P, Hkv, page]: value = code * 2^(byte - 127), with the smallest
+ * power of two, 2^-127 at least, for which the row's largest magnitude is at most the type's largest
+ * value (448 or 127); codes are rounded to nearest, ties to even.  A row that holds an infinity or NaN
+ * gets byte 255 and reads as NaN.
+ *
+ * The kernels compare every page number with P and every position with M * page before they form an
+ * address.  A row whose position has no page (a number below 0 or at least P, or a position past the
+ * table) is not written; where it would be read, the result is NaN.
+ *
+ * page is a power of two from 16 to 65536, M * page < 2^31; D is one of dsqg_supported_head_dims
+ * (EUNSUPPORTED otherwise).  Pools have unit inner stride, other strides {page, head, row} in elements and
+ * bases that keep every row 16-byte aligned, and rows that do not overlap; the scales' strides are
+ * {page, head, row} as well.  B and Hkv are at most 65535. */
+typedef struct {
+    int32_t dtype;             /* DSQG_F32, DSQG_BF16 or DSQG_F16 */
+    int32_t cache_dtype;       /* that, DSQG_E4M3 or DSQG_INT8 */
+    int32_t B, Hkv, D;
+    int32_t P, page, M;
+    void* k_pages;     int64_t k_stride[3];
+    void* v_pages;     int64_t v_stride[3];
+    uint8_t* k_scale;  int64_t k_scale_stride[3];   /* NULL unless 8-bit */
+    uint8_t* v_scale;  int64_t v_scale_stride[3];
+    const int32_t* page_table;
+    int64_t table_stride;      /* elements from one sequence's row to the next */
+} dsqg_paged_cache;
+
+/* Row i of sequence b of k and v [B,Hkv,N,D] (unit inner stride, strides {b, h, n}, rows 16-byte
+ * aligned) goes to position pos[b] + i, for i < N and, where counts is given, i < counts[b]; every
+ * other row of the pools stays as it is. */
+typedef struct {
+    dsqg_paged_cache cache;
+    int32_t N;
+    const void* k;  int64_t k_stride[3];
+    const void* v;  int64_t v_stride[3];
+    const int64_t* pos;        /* [B] */
+    const int64_t* counts;     /* [B] or NULL */
+} dsqg_paged_write_args;
+
+int dsqg_paged_write(const dsqg_paged_write_args* args, dsqg_stream_t stream);
+
+/* Positions t < lengths[b] of each sequence as k and v [B,Hkv,T,D] (contiguous, 16-byte aligned, of the
+ * cache's dtype field, which here may differ from a 16- or 32-bit cache_dtype: values are rounded once);
+ * rows t >= lengths[b] are zeros. */
+typedef struct {
+    dsqg_paged_cache cache;
+    int32_t T;
+    const int64_t* lengths;    /* [B] */
+    void* k;
+    void* v;
+} dsqg_paged_read_args;
+
+int dsqg_paged_read(const dsqg_paged_read_args* args, dsqg_stream_t stream);
+
+/* Decode step: one new token per sequence.  q and out are [B,H,D], H a multiple of Hkv (query head h
+ * attends key/value head h / (H / Hkv)), k_new and v_new [B,Hkv,D]; each but out (contiguous) has unit
+ * inner stride, strides {b, h} and 16-byte aligned rows.  The step writes k_new and v_new to position
+ * pos[b] (as dsqg_paged_write does) and gives
+ *
+ *     out[b,h] = sum_t softmax_t(softmax_scale * q . k_t) v_t      over t = 0 .. pos[b],
+ *
+ * of the rows as the cache holds them.  With k_new = v_new = NULL nothing is written and position pos[b]
+ * is attended as it is.  A sequence with pos[b] < 0 attends nothing: its output is zeros and nothing is
+ * written.  Sums and softmax statistics are fp32, in an order that does not change between calls.
+ * No two sequences may have the same page at the position that a step writes.
+ * The workspace (256-byte aligned) holds the parts of sequences that are split over workgroups. */
+typedef struct {
+    dsqg_paged_cache cache;
+    int32_t H;
+    float softmax_scale;
+    const void* q;      int64_t q_stride[2];
+    const void* k_new;  int64_t k_new_stride[2];
+    const void* v_new;  int64_t v_new_stride[2];
+    const int64_t* pos;        /* [B] */
+    void* out;
+    void* workspace;
+    size_t workspace_bytes;
+} dsqg_paged_decode_args;
+
+int dsqg_paged_decode_workspace_size(const dsqg_paged_decode_args* args, size_t* bytes);
+int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
 
 #ifdef __cplusplus
 }
