@@ -16,16 +16,21 @@ the reference's computation; beyond it the reference slides its window, which sh
 position embedding, so each further token is recomputed on the window exactly as the
 reference does.  Sampling follows the reference: greedy below temperature 0.01, else
 temperature-scaled nucleus (top-p) sampling.
+
+The full-attention layer's cache is a flat tensor that every step attends whole, in torch, or, asked for
+with ``paged=True`` or an 8-bit ``kv_dtype``, a ``PagedKVCache``: the step then reads the rows in use only,
+in one HIP kernel, and the cache may be 8 bits wide.
 """
 
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
+from .api import PagedKVCache
 from .modules import FFN, DSQGBlock, Linear
 
 
@@ -53,10 +58,13 @@ class FullCausalAttention(nn.Module):
         gate = torch.sigmoid(self.gate_proj(x))
         return F.dropout(self.out_proj(out * gate), p=self.dropout_p, training=self.training)
 
-    def forward(self, x: Tensor, cache: Optional["_KVCache"] = None) -> Tensor:
+    def forward(self, x: Tensor, cache: Optional["KVCache"] = None) -> Tensor:
         B, N, E = x.shape
         q, k, v = self._heads(self.qkv_proj(x), B, N)
-        if cache is not None:
+        if isinstance(cache, PagedKVCache):
+            with torch.no_grad():
+                cache.prefill(k, v)
+        elif cache is not None:
             cache.k[:, :, :N] = k
             cache.v[:, :, :N] = v
             cache.pos.fill_(N)
@@ -69,12 +77,15 @@ class FullCausalAttention(nn.Module):
         return self._finish(out.permute(0, 2, 1, 3).reshape(B, N, E), x)
 
     @torch.no_grad()
-    def step(self, x_t: Tensor, cache: "_KVCache") -> Tensor:
+    def step(self, x_t: Tensor, cache: "KVCache") -> Tensor:
         """One token per sequence at the cache's position (a device tensor, so the step has
         fixed shapes and can be captured in a HIP graph): its K/V row goes to that slot and
         the query attends every slot up to it, in fp32."""
         B, E = x_t.shape
         q, k, v = self._heads(self.qkv_proj(x_t).unsqueeze(1), B, 1)
+        if isinstance(cache, PagedKVCache):
+            out = cache.step(q[:, :, 0], k[:, :, 0], v[:, :, 0])
+            return self._finish(out.reshape(B, E), x_t)
         slot = cache.pos[:1]
         cache.k.index_copy_(2, slot, k)
         cache.v.index_copy_(2, slot, v)
@@ -96,6 +107,9 @@ class _KVCache:
         self.pos = torch.zeros((B,), dtype=torch.int64, device=device)
 
 
+KVCache = Union[_KVCache, PagedKVCache]
+
+
 class FullAttentionBlock(nn.Module):
     """train/train_2048_condU.py:304-315: pre-norm block around FullCausalAttention + FFN."""
 
@@ -106,20 +120,25 @@ class FullAttentionBlock(nn.Module):
         self.attn = FullCausalAttention(embedding_dim, num_heads, dropout)
         self.ffn = FFN(embedding_dim, ffn_dim, dropout)
 
-    def forward(self, x: Tensor, cache: Optional[_KVCache] = None) -> Tensor:
+    def forward(self, x: Tensor, cache: Optional[KVCache] = None) -> Tensor:
         x = x + self.attn(self.norm1(x), cache)
         return x + self.ffn(self.norm2(x))
 
-    def new_cache(self, batch: int, max_len: int, device=None, dtype=None) -> _KVCache:
+    def new_cache(self, batch: int, max_len: int, device=None, dtype=None, paged: bool = False,
+                  kv_dtype: Optional[torch.dtype] = None) -> KVCache:
+        """A flat cache, or (``paged``, or any ``kv_dtype``) a PagedKVCache of that page type."""
         w = self.attn.qkv_proj.weight
+        if paged or kv_dtype is not None:
+            return PagedKVCache(batch, self.attn.num_heads, self.attn.head_dim, max_len, dtype or w.dtype,
+                                device or w.device, kv_dtype=kv_dtype)
         return _KVCache(batch, self.attn.num_heads, max_len, self.attn.head_dim,
                         dtype or w.dtype, device or w.device)
 
-    def prefill(self, x: Tensor, cache: _KVCache) -> Tensor:
+    def prefill(self, x: Tensor, cache: KVCache) -> Tensor:
         return self.forward(x, cache)
 
     @torch.no_grad()
-    def step(self, x_t: Tensor, cache: _KVCache) -> Tensor:
+    def step(self, x_t: Tensor, cache: KVCache) -> Tensor:
         x_t = x_t + self.attn.step(self.norm1(x_t), cache)
         return x_t + self.ffn(self.norm2(x_t))
 
@@ -180,11 +199,12 @@ class CondMTransformer(nn.Module):
 
     # ---- generation ------------------------------------------------------------------------
 
-    def new_cache(self, batch: int) -> "GenerationCache":
-        """Per-block caches (DSQG rings and pool sums, the full-attention K/V rows) and the
-        position of the next token."""
-        caches = [b.new_cache(batch, self.seq_len) if isinstance(b, FullAttentionBlock)
-                  else b.new_cache(batch) for b in self.blocks]
+    def new_cache(self, batch: int, paged: bool = False,
+                  kv_dtype: Optional[torch.dtype] = None) -> "GenerationCache":
+        """Per-block caches (DSQG rings and pool sums, the full-attention K/V rows; ``paged`` and
+        ``kv_dtype`` as FullAttentionBlock.new_cache takes them) and the position of the next token."""
+        caches = [b.new_cache(batch, self.seq_len, paged=paged, kv_dtype=kv_dtype)
+                  if isinstance(b, FullAttentionBlock) else b.new_cache(batch) for b in self.blocks]
         dev = self.embedding.weight.device
         return GenerationCache(caches, torch.zeros((batch,), dtype=torch.int64, device=dev))
 
@@ -219,11 +239,13 @@ class CondMTransformer(nn.Module):
 
     @torch.no_grad()
     def generate(self, idx: Tensor, max_new: int, temperature: float = 1.0, top_p: float = 0.9,
-                 generator: Optional[torch.Generator] = None, use_graph: bool = True) -> Tensor:
+                 generator: Optional[torch.Generator] = None, use_graph: bool = True,
+                 paged: bool = False, kv_dtype: Optional[torch.dtype] = None) -> Tensor:
         """Append ``max_new`` sampled tokens to idx [B, N]; returns [B, N + max_new].
 
         After the prefill, the first step runs eagerly and the next ones replay it from a HIP
-        graph (``use_graph``); sampling stays outside the graph.
+        graph (``use_graph``); sampling stays outside the graph.  ``paged`` and ``kv_dtype`` choose the
+        full-attention layer's cache (``new_cache``).
         """
         was_training = self.training
         self.eval()
@@ -236,7 +258,7 @@ class CondMTransformer(nn.Module):
             n = ids.shape[1]
             if n <= self.seq_len:
                 if cache is None:
-                    cache = self.new_cache(ids.shape[0])
+                    cache = self.new_cache(ids.shape[0], paged, kv_dtype)
                     logits = self.prefill(ids, cache)[:, -1]
                 # else: the last token's logits came from the previous step
             else:  # past the position table: the reference's sliding-window recomputation
