@@ -178,4 +178,54 @@ __device__ __forceinline__ float group_max_nan(float x) {
   return x;
 }
 
+// ---- The decode step. -----------------------------------------------------------------------------------
+
+struct PagedDecode {
+  PagedCache c;
+  int H, G;            // query heads; of one key/value head
+  float scale;         // softmax_scale * log2(e)
+  const char* q; long long qb, qh;  // strides in bytes
+  const char* kn; long long knb, knh;
+  const char* vn; long long vnb, vnh;
+  const long long* pos;
+  char* out;           // [B, H, D]
+  int chunk, splits;   // rows of a workgroup, a multiple of 64; chunks of the longest sequence
+  float* ml;           // workspace [B, H, splits, 2]
+  float* acc;          // ... [B, H, splits, D]
+};
+
+// Rows of sequence b that the step attends (0: none) or -1 where its position has no place in the table.
+__device__ __forceinline__ int rows_of(const PagedDecode& p, int b) {
+  const long long pos = p.pos[b];
+  if (pos < 0) return 0;
+  return pos >= ((long long)p.c.M << p.c.shift) ? -1 : (int)pos + 1;
+}
+
+// Rows that are read from the pool (the new one is not), and the workgroups they are split over.
+__device__ __forceinline__ int stored_of(const PagedDecode& p, int n) { return p.kn ? n - 1 : n; }
+__device__ __forceinline__ int chunks_of(const PagedDecode& p, int n) {
+  return n <= 0 ? 1 : max(1, (stored_of(p, n) + p.chunk - 1) / p.chunk);
+}
+
+template <int QT>
+__device__ __forceinline__ void store_out(char* out, long long e, float x) {
+  if constexpr (QT == DSQG_F32) reinterpret_cast<float*>(out)[e] = x;
+  else if constexpr (QT == DSQG_BF16) reinterpret_cast<bf16_t*>(out)[e] = (bf16_t)f32_to_bf16(x);
+  else reinterpret_cast<_Float16*>(out)[e] = (_Float16)x;
+}
+
+// 2^(a - b), where b is the larger: 0 for a = -inf also where b is, NaN for a NaN (which the maxima that
+// b comes from pass over, so that the sums carry it).
+__device__ __forceinline__ float weight(float a, float b) {
+  return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
+}
+
+// Largest group of query heads that one workgroup of the matrix-instruction kernel takes.
+constexpr int kMfmaHeads = 16;
+
+// The matrix-instruction kernel (dsqg_paged_mfma.hip): whether it takes these types and layouts, and its launch
+// over p.splits chunks (the join is the caller's).
+bool paged_mfma_takes(const PagedDecode& p, int dtype, int cache_dtype);
+void launch_paged_mfma(const PagedDecode& p, int dtype, int cache_dtype, int D, hipStream_t st);
+
 }  // namespace dsqg

@@ -29,40 +29,6 @@ namespace {
 
 constexpr int kWaves = kBlock / 64;
 
-struct DecodeArgs {
-  PagedCache c;
-  int H, G;            // query heads; of one key/value head
-  float scale;         // softmax_scale * log2(e)
-  const char* q; long long qb, qh;  // strides in bytes
-  const char* kn; long long knb, knh;
-  const char* vn; long long vnb, vnh;
-  const long long* pos;
-  char* out;           // [B, H, D]
-  int chunk, splits;   // rows of a workgroup, a multiple of 64; chunks of the longest sequence
-  float* ml;           // workspace [B, H, splits, 2]
-  float* acc;          // ... [B, H, splits, D]
-};
-
-// Rows of sequence b that the step attends (0: none) or -1 where its position has no place in the table.
-__device__ __forceinline__ int rows_of(const DecodeArgs& p, int b) {
-  const long long pos = p.pos[b];
-  if (pos < 0) return 0;
-  return pos >= ((long long)p.c.M << p.c.shift) ? -1 : (int)pos + 1;
-}
-
-// Rows that are read from the pool (the new one is not), and the workgroups they are split over.
-__device__ __forceinline__ int stored_of(const DecodeArgs& p, int n) { return p.kn ? n - 1 : n; }
-__device__ __forceinline__ int chunks_of(const DecodeArgs& p, int n) {
-  return n <= 0 ? 1 : max(1, (stored_of(p, n) + p.chunk - 1) / p.chunk);
-}
-
-template <int QT>
-__device__ __forceinline__ void store_out(char* out, long long e, float x) {
-  if constexpr (QT == DSQG_F32) reinterpret_cast<float*>(out)[e] = x;
-  else if constexpr (QT == DSQG_BF16) reinterpret_cast<bf16_t*>(out)[e] = (bf16_t)f32_to_bf16(x);
-  else reinterpret_cast<_Float16*>(out)[e] = (_Float16)x;
-}
-
 // a + sum of the products of eight queries and eight key elements.
 template <int QT, int CT>
 __device__ __forceinline__ float dot8(const Raw8<QT>& qr, const float (&q)[8], const Raw8<CT>& kr, float a) {
@@ -94,14 +60,8 @@ struct Running {
   }
 };
 
-// 2^(a - b), where b is the larger: 0 for a = -inf also where b is, NaN for a NaN (which the maxima that
-// b comes from pass over, so that the sums carry it).
-__device__ __forceinline__ float weight(float a, float b) {
-  return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
-}
-
 template <int QT, int CT, int D, int GT>
-__global__ __launch_bounds__(kBlock) void paged_decode_kernel(DecodeArgs p) {
+__global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   using R = RowMap<D>;
   constexpr int PC = R::pieces, ES = elem_size(CT);
   constexpr int U = CT == DSQG_F32 || PC > 1 ? 2 : 4;  // passes of a tile
@@ -362,82 +322,137 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(DecodeArgs p) {
   }
 }
 
-// Joins a head's chunks, in their order.  Grid: [B * H]; a lane per element.
+// Joins a head's chunks.  Grid: [B * H].  A chunk is JL lanes of four elements; the workgroup's rows of lanes
+// take chunks in turn, each with a running maximum of its own, and meet in LDS: the order is fixed by the
+// sequence's length alone.  Two memory round trips: the position, then every chunk's (m, l) and values.
 template <int QT, int D>
-__global__ __launch_bounds__(128) void paged_join_kernel(DecodeArgs p) {
-  const int b = blockIdx.x / p.H;
-  const int n = rows_of(p, b);
-  const int chunks = chunks_of(p, n);
-  if (chunks == 1 || threadIdx.x >= D) return;  // (written by its only workgroup)
-  const float* ml = p.ml + 2ll * blockIdx.x * p.splits;
-  const float* acc = p.acc + (long long)blockIdx.x * p.splits * D + threadIdx.x;
-  float m = -INFINITY, l = 0.f, x = 0.f;
-  for (int c = 0; c < chunks; ++c) m = fmaxf(m, ml[2 * c]);
-  for (int c = 0; c < chunks; ++c) {
-    const float a = weight(ml[2 * c], m);
-    l = fmaf(ml[2 * c + 1], a, l);
-    x = fmaf(acc[(long long)c * D], a, x);
+__global__ __launch_bounds__(1024) void paged_join_kernel(PagedDecode p) {
+  constexpr int JL = D <= 32 ? 8 : D <= 64 ? 16 : 32;
+  const int b = blockIdx.x / p.H, rows = blockDim.x / JL;
+  const int gl = threadIdx.x % JL, r = threadIdx.x / JL;
+  const int chunks = chunks_of(p, rows_of(p, b));
+  if (chunks == 1) return;  // (written by its only workgroup)
+  const float2* ml = reinterpret_cast<const float2*>(p.ml) + (long long)blockIdx.x * p.splits;
+  const float* acc = p.acc + (long long)blockIdx.x * p.splits * D + 4 * gl;
+  constexpr int U = 4;
+  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = r; c0 < chunks; c0 += U * rows) {
+    float2 s[U];
+    float4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * rows;
+      const bool live = c < chunks;
+      s[u] = live ? ml[c] : make_float2(-INFINITY, 0.f);
+      v[u] = live && 4 * gl < D ? *reinterpret_cast<const float4*>(acc + (long long)c * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, s[u].x);
+    const float a = weight(m, mn);
+    m = mn;
+    l *= a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] *= a;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = weight(s[u].x, m);
+      l = fmaf(s[u].y, w, l);
+      x[0] = fmaf(v[u].x, w, x[0]);
+      x[1] = fmaf(v[u].y, w, x[1]);
+      x[2] = fmaf(v[u].z, w, x[2]);
+      x[3] = fmaf(v[u].w, w, x[3]);
+    }
   }
-  store_out<QT>(p.out, (long long)blockIdx.x * D + threadIdx.x, x / l);
+  __shared__ float jm[1024 / JL], jl[1024 / JL], jx[1024 / JL][D];
+  if (4 * gl < D)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) jx[r][4 * gl + i] = x[i];
+  if (gl == 0) {
+    jm[r] = m;
+    jl[r] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int n = min(rows, chunks);
+  m = -INFINITY;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, jm[i]);
+  float o = 0.f;
+  l = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float w = weight(jm[i], m);
+    l = fmaf(jl[i], w, l);
+    o = fmaf(jx[i][threadIdx.x], w, o);
+  }
+  store_out<QT>(p.out, (long long)blockIdx.x * D + threadIdx.x, o / l);
 }
 
-// Rows of a chunk and the chunks of a sequence that fills its table.  Sixteen workgroups a CU in all, of 128
-// to 4096 rows each.
-void plan(DecodeArgs& p, int GT) {
+// The kernels of a call and its split.
+struct Plan {
+  bool mfma;
+  int heads;  // query heads of a workgroup
+};
+
+Plan plan(PagedDecode& p, int dtype, int cache_dtype, int D) {
+  Plan k;
+  k.mfma = p.G >= 2 && paged_mfma_takes(p, dtype, cache_dtype);
+  // Three groups of eight a lane leave registers for two heads of the vector kernel.
+  k.heads = k.mfma ? kMfmaHeads : p.G == 1 ? 1 : p.G == 2 || D == 80 || D == 96 ? 2 : 4;
   const long long T = std::max(1ll, (long long)p.c.M << p.c.shift);
-  const long long units = (long long)p.c.B * p.c.Hkv * ((p.G + GT - 1) / GT);
-  long long chunk = (T * units + 4095) / 4096;
-  chunk = std::min(4096ll, std::max(128ll, (chunk + 63) / 64 * 64));
+  const long long units = (long long)p.c.B * p.c.Hkv * ((p.G + k.heads - 1) / k.heads);
+  // Rows of a chunk: a few workgroups for each place on the chip, not so short that a workgroup's beginning
+  // and end outweigh its rows.
+  const long long most = k.mfma ? 1024 : 1536, least = k.mfma ? 256 : 128;
+  long long chunk = ((T * units + most - 1) / most + 63) / 64 * 64;
+  chunk = std::min(4096ll, std::max(least, chunk));
   chunk = std::max(chunk, (T / 65535 + 64) / 64 * 64);  // (the grid's limit)
   p.splits = (int)((T + chunk - 1) / chunk);
   p.chunk = (int)chunk;
+  return k;
 }
 
-// Query heads of a workgroup: three groups of eight a lane leave registers for two.
-int heads_per_block(int G, int D) { return G == 1 ? 1 : G == 2 || D == 80 || D == 96 ? 2 : 4; }
-
 template <int QT, int CT, int D, int GT>
-void launch(const DecodeArgs& p, hipStream_t st) {
+void launch(const PagedDecode& p, hipStream_t st) {
   const unsigned units = (unsigned)(p.c.B * p.c.Hkv * ((p.G + GT - 1) / GT));
   hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, GT>), dim3(units, (unsigned)p.splits), dim3(kBlock), 0, st, p);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((paged_join_kernel<QT, D>), dim3((unsigned)(p.c.B * p.H)), dim3(128), 0, st, p);
 }
 
 template <int QT, int CT, int D>
-void launch_heads(const DecodeArgs& p, hipStream_t st) {
-  const int gt = heads_per_block(p.G, D);
-  if (gt == 1) {
+void launch_heads(const PagedDecode& p, int heads, hipStream_t st) {
+  if (heads == 1) {
     launch<QT, CT, D, 1>(p, st);
-  } else if (gt == 2) {
+  } else if (heads == 2) {
     launch<QT, CT, D, 2>(p, st);
   } else if constexpr (RowMap<D>::pieces == 1) {
     launch<QT, CT, D, 4>(p, st);
   }
 }
 
-template <int QT, int CT>
-void launch_dim(const DecodeArgs& p, int D, hipStream_t st) {
-  switch (D) {
-    case 32: launch_heads<QT, CT, 32>(p, st); break;
-    case 64: launch_heads<QT, CT, 64>(p, st); break;
-    case 80: launch_heads<QT, CT, 80>(p, st); break;
-    case 96: launch_heads<QT, CT, 96>(p, st); break;
-    default: launch_heads<QT, CT, 128>(p, st); break;
-  }
+template <int QT, int D>
+void launch_types(const PagedDecode& p, const Plan& k, int ct, hipStream_t st) {
+  if (k.mfma) launch_paged_mfma(p, QT, ct, D, st);
+  else if (ct == DSQG_E4M3) launch_heads<QT, DSQG_E4M3, D>(p, k.heads, st);
+  else if (ct == DSQG_INT8) launch_heads<QT, DSQG_INT8, D>(p, k.heads, st);
+  else launch_heads<QT, QT, D>(p, k.heads, st);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((paged_join_kernel<QT, D>), dim3((unsigned)(p.c.B * p.H)), dim3(p.splits > 32 ? 1024 : 256), 0, st, p);
 }
 
 template <int QT>
-void launch_types(const DecodeArgs& p, int ct, int D, hipStream_t st) {
-  if (ct == DSQG_E4M3) launch_dim<QT, DSQG_E4M3>(p, D, st);
-  else if (ct == DSQG_INT8) launch_dim<QT, DSQG_INT8>(p, D, st);
-  else launch_dim<QT, QT>(p, D, st);
+void launch_dim(const PagedDecode& p, const Plan& k, int ct, int D, hipStream_t st) {
+  switch (D) {
+    case 32: launch_types<QT, 32>(p, k, ct, st); break;
+    case 64: launch_types<QT, 64>(p, k, ct, st); break;
+    case 80: launch_types<QT, 80>(p, k, ct, st); break;
+    case 96: launch_types<QT, 96>(p, k, ct, st); break;
+    default: launch_types<QT, 128>(p, k, ct, st); break;
+  }
 }
 
 // The checks that the size query and the launch share; workspace bytes of the parts.
-int check_decode(const dsqg_paged_decode_args* a, DecodeArgs* p, size_t* bytes) {
+int check_decode(const dsqg_paged_decode_args* a, PagedDecode* p, Plan* k, size_t* bytes) {
   if (!a || a->H < 0) return DSQG_EINVAL;
-  *p = DecodeArgs{};
+  *p = PagedDecode{};
   *bytes = 0;
   if (const int st = check_paged_cache(a->cache, &p->c)) return st;
   const dsqg_paged_cache& c = a->cache;
@@ -447,7 +462,7 @@ int check_decode(const dsqg_paged_decode_args* a, DecodeArgs* p, size_t* bytes) 
   if ((long long)c.B * a->H >= (1ll << 23)) return DSQG_EUNSUPPORTED;  // grid: a workgroup of 256 a head
   p->H = a->H;
   p->G = a->H / c.Hkv;
-  plan(*p, heads_per_block(p->G, c.D));
+  *k = plan(*p, c.dtype, c.cache_dtype, c.D);
   if (p->splits > 1) *bytes = (size_t)c.B * a->H * p->splits * (2 + c.D) * sizeof(float);
   return DSQG_OK;
 }
@@ -458,14 +473,16 @@ int check_decode(const dsqg_paged_decode_args* a, DecodeArgs* p, size_t* bytes) 
 using namespace dsqg;
 
 extern "C" int dsqg_paged_decode_workspace_size(const dsqg_paged_decode_args* a, size_t* bytes) {
-  DecodeArgs p;
-  return bytes ? check_decode(a, &p, bytes) : (int)DSQG_EINVAL;
+  PagedDecode p;
+  Plan k;
+  return bytes ? check_decode(a, &p, &k, bytes) : (int)DSQG_EINVAL;
 }
 
 extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t stream) {
-  DecodeArgs p;
+  PagedDecode p;
+  Plan k;
   size_t bytes = 0;
-  if (const int st = check_decode(a, &p, &bytes)) return st;
+  if (const int st = check_decode(a, &p, &k, &bytes)) return st;
   const dsqg_paged_cache& c = a->cache;
   if ((long long)c.B * a->H == 0) return DSQG_OK;
   const long long es = elem_size(c.dtype);
@@ -491,8 +508,8 @@ extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t 
   p.acc = static_cast<float*>(a->workspace);
   p.ml = p.acc + (long long)c.B * a->H * p.splits * c.D;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (c.dtype == DSQG_F32) launch_types<DSQG_F32>(p, c.cache_dtype, c.D, st);
-  else if (c.dtype == DSQG_BF16) launch_types<DSQG_BF16>(p, c.cache_dtype, c.D, st);
-  else launch_types<DSQG_F16>(p, c.cache_dtype, c.D, st);
+  if (c.dtype == DSQG_F32) launch_dim<DSQG_F32>(p, k, c.cache_dtype, c.D, st);
+  else if (c.dtype == DSQG_BF16) launch_dim<DSQG_BF16>(p, k, c.cache_dtype, c.D, st);
+  else launch_dim<DSQG_F16>(p, k, c.cache_dtype, c.D, st);
   return hipGetLastError() == hipSuccess ? DSQG_OK : DSQG_EHIP;
 }

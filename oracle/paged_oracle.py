@@ -87,11 +87,16 @@ def bound(out, mass, size, D, T, dtype):
     16 u.  All of these are relative to ``mass[:, 0]``.  A weight, or its product with the factor that a
     larger maximum brings, that lies below the normal numbers may come out as zero, which three such
     products in turn (tile, wave, chunk) add up to 4 * 2^-126 for each row, as the largest weight is 1:
-    that much of ``mass[:, 1]``.  Last, the result's rounding to its type, half a step of it: eps / 2
+    that much of ``mass[:, 1]``.  Weights that enter a product in two 16-bit terms are 2^-16 off in bfloat16
+    (a term of 8 bits rounded down and one of 8 bits rounded: 2^-7 * 2^-9) and, in float16, 2^-21 (2^-10 *
+    2^-11) or its subnormal step where the largest weight is 2^14: 2 * 2^-38 of ``mass[:, 1]`` (a float32
+    kernel has no such terms; its results' bound leaves them out).  Last, the result's rounding to its type, half a step of it: eps / 2
     relative, or half the smallest subnormal.
     """
     u = 2.0 ** -24
     w = 2 * ((D + 7) * u * size + 2 * u)
     tol = mass[:, 0] * (w + (2 * T + 16) * u) + mass[:, 1] * 4 * 2.0 ** -126
+    if dtype != torch.float32:
+        tol = tol + mass[:, 0] * 2.0 ** -16 + (mass[:, 1] * 2.0 ** -37 if dtype == torch.float16 else 0)
     fi = torch.finfo(dtype)
     return tol + (out.abs() + tol) * (fi.eps / 2) + fi.smallest_normal * fi.eps
