@@ -814,8 +814,8 @@ struct Paged {
       if (written && t->is_inference() && !inference)
         raise(PyExc_RuntimeError, "Inplace update to inference tensor outside InferenceMode is not allowed");
     }
-    require(P < (1ll << 31) && H <= 65535 && table0.size(0) <= 65535 && table0.size(1) * page < (1ll << 31),
-            "a cache has at most 65535 sequences, 65535 heads and 2^31 positions of a sequence");
+    require(P < (1ll << 31) && H <= 65535 && table0.size(0) <= 65535 && table0.size(1) * page <= (1ll << 30),
+            "a cache has at most 65535 sequences, 65535 heads and 2^30 positions of a sequence");
     const int64_t es = k.element_size();
     for (const Tensor* t : {&k, &v}) {
       bool ok = t->numel() == 0 || (t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0);

@@ -180,6 +180,16 @@ __device__ __forceinline__ float group_max_nan(float x) {
 
 // ---- The decode step. -----------------------------------------------------------------------------------
 
+// A step's work is split over workgroups in one of two ways.
+//  * Chunks (shares = 0): a workgroup for each unit (a sequence's key/value head and up to `heads` of its query
+//    heads) and chunk of `chunk` rows, as many chunks as the longest sequence that the table could hold would
+//    have; those behind a sequence's end leave at once.
+//  * Shares: the rows of all units in one line, in steps of kShareRows, cut into `shares` equal parts, one a
+//    workgroup: however the lengths differ, every workgroup has the same number of steps and no place on the chip
+//    waits for the longest sequence.  A share may cover parts of several units; part w of unit u is number w + u
+//    of the workspace, as one of the two grows from each part to the next.
+// A unit that is not split is finished by its workgroup; the others' parts are joined by a second launch, for
+// which the workgroup with a unit's first rows says how many there are, and where.
 struct PagedDecode {
   PagedCache c;
   int H, G;            // query heads; of one key/value head
@@ -189,10 +199,17 @@ struct PagedDecode {
   const char* vn; long long vnb, vnh;
   const long long* pos;
   char* out;           // [B, H, D]
-  int chunk, splits;   // rows of a workgroup, a multiple of 64; chunks of the longest sequence
-  float* ml;           // workspace [B, H, splits, 2]
-  float* acc;          // ... [B, H, splits, D]
+  int heads;           // query heads of a unit, at most
+  int chunk, splits;   // chunks: rows of one, a multiple of 64, and their number
+  int shares;          // shares: their number
+  int stream;          // rows are read past the caches' retention
+  float* ml;           // workspace [parts, 2]: chunks [units, splits, heads], shares [shares + units, heads]
+  float* acc;          // ... [parts, D]
+  int2* joins;         // ... [units]: the first part, in `heads`, and how many
 };
+
+constexpr int kShareRows = 128;
+constexpr int kShareSeqs = 512;  // sequences that a wave places its share among: eight a lane
 
 // Rows of sequence b that the step attends (0: none) or -1 where its position has no place in the table.
 __device__ __forceinline__ int rows_of(const PagedDecode& p, int b) {
@@ -201,11 +218,75 @@ __device__ __forceinline__ int rows_of(const PagedDecode& p, int b) {
   return pos >= ((long long)p.c.M << p.c.shift) ? -1 : (int)pos + 1;
 }
 
-// Rows that are read from the pool (the new one is not), and the workgroups they are split over.
+// Rows that are read from the pool (the new one is not), and the chunks or steps that they make.
 __device__ __forceinline__ int stored_of(const PagedDecode& p, int n) { return p.kn ? n - 1 : n; }
 __device__ __forceinline__ int chunks_of(const PagedDecode& p, int n) {
   return n <= 0 ? 1 : max(1, (stored_of(p, n) + p.chunk - 1) / p.chunk);
 }
+__device__ __forceinline__ int steps_of(const PagedDecode& p, int n) {
+  return n <= 0 ? 1 : max(1, (stored_of(p, n) + kShareRows - 1) / kShareRows);
+}
+
+// Where the units lie in the line of steps: a wave's view, for up to kShareSeqs sequences, whose rows it holds
+// eight a lane.
+struct ShareLine {
+  int n[kShareSeqs / 64], sum, incl, q;  // this lane's sequences' rows, their steps, and the steps up to them
+  int units, per;                        // units of a sequence; steps of a share
+  __device__ __forceinline__ ShareLine(const PagedDecode& p) {
+    const int l = threadIdx.x & 63;
+    q = (p.c.B + 63) / 64;
+    units = p.c.Hkv * ((p.G + p.heads - 1) / p.heads);
+#pragma unroll
+    for (int j = 0; j < kShareSeqs / 64; ++j) n[j] = j < q && l * q + j < p.c.B ? rows_of(p, l * q + j) : 0;
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < kShareSeqs / 64; ++j) sum += j < q && l * q + j < p.c.B ? steps_of(p, n[j]) : 0;
+    // Inclusive sums over the lanes: inside rows of 16, then rows 0 and 2 into 1 and 3, then the first half
+    // into the second.
+    incl = sum;
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xf, 0xf, true);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xf, 0xf, true);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xf, 0xf, true);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xf, 0xf, true);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x142, 0xa, 0xf, false);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x143, 0xc, 0xf, false);
+    const int total = steps();
+    per = (total + p.shares - 1) / p.shares;
+  }
+  __device__ __forceinline__ int steps() const { return __builtin_amdgcn_readlane(incl, 63) * units; }
+  // Rows of sequence b, and the line's steps before it.
+  __device__ __forceinline__ int rows(int b) const {
+    const int lane = b / q, j0 = b - lane * q;
+    int r = 0;
+#pragma unroll
+    for (int j = 0; j < kShareSeqs / 64; ++j)
+      if (j == j0) r = __builtin_amdgcn_readlane(n[j], lane);
+    return r;
+  }
+  __device__ __forceinline__ int before(const PagedDecode& p, int b) const {
+    const int lane = b / q, j0 = b - lane * q;
+    int r = __builtin_amdgcn_readlane(incl, lane) - __builtin_amdgcn_readlane(sum, lane);
+#pragma unroll
+    for (int j = 0; j < kShareSeqs / 64; ++j)
+      if (j < j0) r += steps_of(p, __builtin_amdgcn_readlane(n[j], lane));
+    return r * units;
+  }
+  // The sequence that step s belongs to (s < steps()).
+  __device__ __forceinline__ int sequence(const PagedDecode& p, int s) const {
+    const int lane = __builtin_ctzll(__ballot(s < incl * units));
+    int at = (__builtin_amdgcn_readlane(incl, lane) - __builtin_amdgcn_readlane(sum, lane)) * units, b = lane * q;
+#pragma unroll
+    for (int j = 0; j < kShareSeqs / 64 - 1; ++j)
+      if (j < q - 1) {
+        const int next = at + steps_of(p, __builtin_amdgcn_readlane(n[j], lane)) * units;
+        if (s >= next && b == lane * q + j) {
+          at = next;
+          ++b;
+        }
+      }
+    return b;
+  }
+};
 
 template <int QT>
 __device__ __forceinline__ void store_out(char* out, long long e, float x) {
@@ -227,5 +308,7 @@ constexpr int kMfmaHeads = 16;
 // over p.splits chunks (the join is the caller's).
 bool paged_mfma_takes(const PagedDecode& p, int dtype, int cache_dtype);
 void launch_paged_mfma(const PagedDecode& p, int dtype, int cache_dtype, int D, hipStream_t st);
+// Workgroups of it that the chip holds.
+int paged_mfma_places(int D);
 
 }  // namespace dsqg

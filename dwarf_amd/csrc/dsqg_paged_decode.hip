@@ -1,23 +1,22 @@
-// Attention of one new token per sequence over a paged key/value cache (gfx950).
+// Attention of one new token per sequence over a paged key/value cache (gfx950): the plan, the kernel of the
+// vector instructions and the join.
 //
 //   out[h] = sum_t w_t v_t,  w = softmax_t(scale q_h . k_t),  t = 0 .. pos
 //
 // One pass over the rows with a running maximum and sum: of the rows seen so far a group of lanes keeps
 // m = max s_t, l = sum 2^(s_t - m) and acc = sum 2^(s_t - m) v_t (scores in base 2), and the parts of
-// different rows join as  acc = sum_i 2^(m_i - m) acc_i.  Every key and value is read once and takes part
-// in one product per query head, so memory bounds the step.
+// different rows join as  acc = sum_i 2^(m_i - m) acc_i.  Every key and value is read once, so memory bounds
+// the step, and short ones the launches and the round trips from the position to the rows.
 //
-// A workgroup has one key/value head of one sequence, up to GT of the query heads that share it, and a
+// 16-bit queries take the matrix instructions (dsqg_paged_mfma.hip).  The kernel here takes float32 ones, whose
+// products those instructions would round, and 8-bit pools whose scales they cannot read four at a time.
+//
+// Its workgroup has one key/value head of one sequence, up to GT of the query heads that share it, and a
 // chunk of the sequence's rows; its four waves take tiles in turn.  In a tile a row is 4, 8 or 16
 // neighbouring lanes (RowMap), each wave load being whole rows of one page: a tile starts at a multiple of
-// the wave's rows and a page is a multiple of them too, so the page number is the same for all lanes and
-// comes from the table as a scalar.  Row groups keep statistics of their own until the chunk's end.
-//
-// Sequences longer than a chunk leave their chunks' (m, l, acc) in the workspace, and a second launch
-// joins them in the order of the chunks.
-//
-// The first chunk's workgroup takes the new row from the caller's k_new and v_new (as the cache will hold
-// it: through the 8-bit type's rounding), and stores it; no workgroup reads that row from the pool.
+// the wave's rows and a page is a multiple of them too.  Row groups keep statistics of their own until the
+// chunk's end.  The first chunk's workgroup takes the new row from the caller's k_new and v_new (as the cache
+// will hold it: through the 8-bit type's rounding), and stores it; no workgroup reads that row from the pool.
 #include <algorithm>
 
 #include "dsqg_launch.hpp"
@@ -30,17 +29,13 @@ namespace {
 constexpr int kWaves = kBlock / 64;
 
 // a + sum of the products of eight queries and eight key elements.
-template <int QT, int CT>
-__device__ __forceinline__ float dot8(const Raw8<QT>& qr, const float (&q)[8], const Raw8<CT>& kr, float a) {
-  if constexpr (QT == DSQG_BF16 && CT == DSQG_BF16) {
-    return dot8_bf16(qr.a, kr.a, a);
-  } else {
-    float k[8];
-    raw_floats<CT>(kr, k);
+template <int CT>
+__device__ __forceinline__ float dot8(const float (&q)[8], const Raw8<CT>& kr, float a) {
+  float k[8];
+  raw_floats<CT>(kr, k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaf(q[i], k[i], a);
-    return a;
-  }
+  for (int i = 0; i < 8; ++i) a = fmaf(q[i], k[i], a);
+  return a;
 }
 
 // Statistics and output sums of GT heads over the rows of one lane group.
@@ -65,40 +60,100 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   using R = RowMap<D>;
   constexpr int PC = R::pieces, ES = elem_size(CT);
   constexpr int U = CT == DSQG_F32 || PC > 1 ? 2 : 4;  // passes of a tile
-  constexpr int TR = U * R::rows;
+  constexpr int TR = U * R::rows, stride = kWaves * TR;
   const int hg = (p.G + GT - 1) / GT;
   const int b = blockIdx.x / (p.c.Hkv * hg), rest = blockIdx.x - b * p.c.Hkv * hg;
   const int hk = rest / hg, g0 = (rest - hk * hg) * GT;
   const int split = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gl = lane % R::lanes, r = lane / R::lanes;
-  const int n = rows_of(p, b);
-  const int chunks = chunks_of(p, n);
-  if (split >= chunks) return;
-  const long long h0 = (long long)b * p.H + hk * p.G + g0;  // first query head, in [B, H]
-  if (n <= 0) {  // no rows: zeros; a position outside the table: NaN
-    for (int e = threadIdx.x; e < GT * D; e += kBlock)
-      if (g0 + e / D < p.G) store_out<QT>(p.out, h0 * D + e, n == 0 ? 0.f : __uint_as_float(0x7fc00000u));
-    return;
-  }
 
+  // The page numbers of the wave's next 64 / U tiles, a pass each lane: no load stands between a tile and its
+  // rows.  Like the queries they need no position (entries behind the sequence's last page may be no pages:
+  // their rows are masked, whatever is said of them), so all of them are on their way together.
   const int* table = p.c.table + b * p.c.ts;
-  const bool fresh = p.kn != nullptr;
-  const int stored = stored_of(p, n);
-  const int t0 = split * p.chunk, t1 = min(t0 + p.chunk, stored);
+  const int last = (p.c.M << p.c.shift) - 1;
+  auto page_of = [&](int t) { return last < 0 ? -1 : table[min((unsigned)t, (unsigned)last) >> p.c.shift]; };
+  const int t0 = split * p.chunk, first = t0 + wave * TR;
+  auto pages_from = [&](int t) { return page_of(t + lane / U * stride + lane % U * R::rows); };
+  int pages = pages_from(first);
 
-  Raw8<QT> qr[GT][PC];
   float q[GT][PC][8];
 #pragma unroll
   for (int g = 0; g < GT; ++g)
 #pragma unroll
     for (int u = 0; u < PC; ++u) {
       const int piece = gl + R::lanes * u;
-      raw_zero<QT>(qr[g][u]);
+      Raw8<QT> x;
+      raw_zero<QT>(x);
       if (g0 + g < p.G && piece < R::CPR)
-        qr[g][u] = raw_load<QT>(p.q + b * p.qb + (hk * p.G + g0 + g) * p.qh + piece * 8 * elem_size(QT));
-      raw_floats<QT>(qr[g][u], q[g][u]);
+        x = raw_load<QT>(p.q + b * p.qb + (hk * p.G + g0 + g) * p.qh + piece * 8 * elem_size(QT));
+      raw_floats<QT>(x, q[g][u]);
     }
+
+  const int n = rows_of(p, b);
+  const int chunks = chunks_of(p, n);
+  if (split >= chunks) return;
+  if (split == 0 && p.joins && threadIdx.x == 0) p.joins[blockIdx.x] = make_int2(blockIdx.x * p.splits, chunks);
+  const long long h0 = (long long)b * p.H + hk * p.G + g0;  // first query head, in [B, H]
+  if (n <= 0) {  // no rows: zeros; a position outside the table: NaN
+    for (int e = threadIdx.x; e < GT * D; e += kBlock)
+      if (g0 + e / D < p.G) store_out<QT>(p.out, h0 * D + e, n == 0 ? 0.f : __uint_as_float(0x7fc00000u));
+    return;
+  }
+  const bool fresh = p.kn != nullptr;
+  const int t1 = min(t0 + p.chunk, stored_of(p, n));
+
+  // The wave's tile k.  Loads go through a buffer resource for each pass's rows, so that nothing outside them
+  // can be touched.  (A pass that lies behind the last row is masked.)
+  Raw8<CT> kr[U][PC], vr[U][PC];
+  int sk[U], sv[U];  // scale bytes
+  bool bad[U];
+  auto place = [&](int k, int u, unsigned& at, unsigned& slot) {
+    const int t = first + k * stride + u * R::rows, page = __builtin_amdgcn_readlane(pages, k % (64 / U) * U + u);
+    bad[u] = (unsigned)page >= (unsigned)p.c.P;
+    at = bad[u] ? 0u : (unsigned)page;
+    slot = (unsigned)t & ((1u << p.c.shift) - 1u);
+  };
+  auto load_rows = [&](Raw8<CT> (&x)[PC], const char* base, int row) {
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (R::rows - 1) * row + D * ES, 0x00020000);
+#pragma unroll
+    for (int w = 0; w < PC; ++w) {
+      // (A piece behind the row's end, at D = 80, is another row's or nobody's.)
+      const int off = r * row + (gl + R::lanes * w) * 8 * ES;
+      if constexpr (narrow(CT)) {
+        x[w].a = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0));
+      } else {
+        x[w].a = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+        if constexpr (CT == DSQG_F32) x[w].b = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 16, 0, 0));
+      }
+      if (gl + R::lanes * w >= R::CPR) raw_zero<CT>(x[w]);
+    }
+  };
+  auto load_k = [&](int k) {
+    if (k > 0 && k % (64 / U) == 0) pages = pages_from(first + k * stride);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unsigned at, slot;
+      place(k, u, at, slot);
+      load_rows(kr[u], p.c.k + at * p.c.kp + hk * p.c.kh + slot * p.c.kn, (int)p.c.kn);
+      if constexpr (narrow(CT)) sk[u] = p.c.ks[at * p.c.ksp + hk * p.c.ksh + (slot + r) * p.c.ksn];
+    }
+  };
+  auto load_v = [&](int k) {  // (after load_k of the same tile)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unsigned at, slot;
+      place(k, u, at, slot);
+      load_rows(vr[u], p.c.v + at * p.c.vp + hk * p.c.vh + slot * p.c.vn, (int)p.c.vn);
+      if constexpr (narrow(CT)) sv[u] = p.c.vs[at * p.c.vsp + hk * p.c.vsh + (slot + r) * p.c.vsn];
+    }
+  };
+  if (first < t1) {
+    load_k(0);
+    load_v(0);
+  }
 
   Running<GT, PC> s;
   s.clear();
@@ -145,14 +200,14 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
         vc[u] = y[u];
       }
     }
-    const int t = n - 1, page = table[t >> p.c.shift];
+    const int t = n - 1, page = page_of(t);
     const bool ok = (unsigned)page < (unsigned)p.c.P;
     const float sk = narrow(CT) ? scale_value(kb) : 1.f, sv = narrow(CT) ? scale_value(vb) : 1.f;
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
       float d = 0.f;
 #pragma unroll
-      for (int u = 0; u < PC; ++u) d = dot8<QT, CT>(qr[g][u], q[g][u], kc[u], d);
+      for (int u = 0; u < PC; ++u) d = dot8<CT>(q[g][u], kc[u], d);
       d = group_sum<R::lanes>(d) * (p.scale * sk);
       if (!ok) d = __uint_as_float(0x7fc00000u);  // nowhere to keep the row
       if (r == 0) {
@@ -188,55 +243,37 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
     }
   }
 
-  for (int tile = t0 + wave * TR; tile < t1; tile += kWaves * TR) {
-    Raw8<CT> k[U][PC], v[U][PC];
-    float sk[U], sv[U];
-    bool bad[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (A pass that lies behind the last row reads that row's page, which exists, and is masked.)
-      const int t = tile + u * R::rows;
-      int page = table[min(t, stored - 1) >> p.c.shift];
-      bad[u] = (unsigned)page >= (unsigned)p.c.P;
-      page = bad[u] ? 0 : page;
-      const long long slot = t & ((1 << p.c.shift) - 1);
-      const char* kr = p.c.k + page * p.c.kp + hk * p.c.kh + slot * p.c.kn + r * p.c.kn;
-      const char* vr = p.c.v + page * p.c.vp + hk * p.c.vh + slot * p.c.vn + r * p.c.vn;
-#pragma unroll
-      for (int w = 0; w < PC; ++w) {
-        const int piece = gl + R::lanes * w;
-        raw_zero<CT>(k[u][w]);
-        raw_zero<CT>(v[u][w]);
-        if (piece < R::CPR) {
-          k[u][w] = raw_load<CT>(kr + piece * 8 * ES);
-          v[u][w] = raw_load<CT>(vr + piece * 8 * ES);
-        }
-      }
-      sk[u] = sv[u] = 1.f;
-      if constexpr (narrow(CT)) {
-        sk[u] = scale_value(p.c.ks[page * p.c.ksp + hk * p.c.ksh + (slot + r) * p.c.ksn]);
-        sv[u] = scale_value(p.c.vs[page * p.c.vsp + hk * p.c.vsh + (slot + r) * p.c.vsn]);
-      }
-    }
+#pragma unroll 1
+  for (int k = 0, tile = first; tile < t1; ++k, tile += stride) {
+    const bool more = tile + stride < t1;
     float sc[GT][U];
+    bool no[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool live = tile + u * R::rows + r < t1;
+      no[u] = bad[u];
+      const float c = narrow(CT) ? p.scale * scale_value(sk[u]) : p.scale;
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
         float d = 0.f;
 #pragma unroll
-        for (int w = 0; w < PC; ++w) d = dot8<QT, CT>(qr[g][w], q[g][w], k[u][w], d);
-        d = group_sum<R::lanes>(d) * (p.scale * sk[u]);
-        if (bad[u]) d = __uint_as_float(0x7fc00000u);
-        sc[g][u] = live ? d : -INFINITY;
+        for (int w = 0; w < PC; ++w) d = dot8<CT>(q[g][w], kr[u][w], d);
+        sc[g][u] = group_sum<R::lanes>(d) * c;
+        if (no[u]) sc[g][u] = __uint_as_float(0x7fc00000u);
       }
+    }
+    // The next tile's keys are on their way during the softmax, its values during the next scores.
+    if (more) load_k(k + 1);
+    if (tile + TR > t1) {
       // What lies behind the last row is no number of this sequence: zeros, so that 0 * value is 0.
-      if (!live) {
-        sv[u] = 0.f;
 #pragma unroll
-        for (int w = 0; w < PC; ++w) raw_zero<CT>(v[u][w]);
-      }
+      for (int u = 0; u < U; ++u)
+        if (tile + u * R::rows + r >= t1) {
+          sv[u] = 127;
+#pragma unroll
+          for (int g = 0; g < GT; ++g) sc[g][u] = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < PC; ++w) raw_zero<CT>(vr[u][w]);
+        }
     }
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
@@ -254,7 +291,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
       for (int u = 0; u < U; ++u) {
         const float e = weight(sc[g][u], m);
         s.l[g] += e;
-        sc[g][u] = e * sv[u];
+        sc[g][u] = narrow(CT) ? e * scale_value(sv[u]) : e;
       }
     }
 #pragma unroll
@@ -262,12 +299,13 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
 #pragma unroll
       for (int w = 0; w < PC; ++w) {
         float x[8];
-        raw_floats<CT>(v[u][w], x);
+        raw_floats<CT>(vr[u][w], x);
 #pragma unroll
         for (int g = 0; g < GT; ++g)
 #pragma unroll
           for (int i = 0; i < 8; ++i) s.acc[g][w][i] = fmaf(sc[g][u], x[i], s.acc[g][w][i]);
       }
+    if (more) load_v(k + 1);
   }
 
   // The row groups of the wave, then the waves through LDS.
@@ -276,11 +314,13 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   for (int g = 0; g < GT; ++g) {
     float m = s.m[g];
 #pragma unroll
-    for (int x = R::lanes; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
+    for (int x = R::lanes; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
+    m = col_max(m);
     const float a = weight(s.m[g], m);
     float l = s.l[g] * a;
 #pragma unroll
-    for (int x = R::lanes; x < 64; x *= 2) l += __shfl_xor(l, x, 64);
+    for (int x = R::lanes; x < 16; x *= 2) l += __shfl_xor(l, x, 64);
+    l = col_sum(l);
     if (lane == 0) {
       wm[wave][g] = m;
       wl[wave][g] = l;
@@ -291,7 +331,8 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
       for (int i = 0; i < 8; ++i) {
         float x = s.acc[g][w][i] * a;
 #pragma unroll
-        for (int y = R::lanes; y < 64; y *= 2) x += __shfl_xor(x, y, 64);
+        for (int y = R::lanes; y < 16; y *= 2) x += __shfl_xor(x, y, 64);
+        x = col_sum(x);
         const int piece = gl + R::lanes * w;
         if (r == 0 && piece < R::CPR) wacc[wave][g][piece * 8 + i] = x;
       }
@@ -312,7 +353,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
     if (chunks == 1) {
       store_out<QT>(p.out, h0 * D + e, x / l);
     } else {
-      const long long at = (h0 + g) * p.splits + split;
+      const long long at = ((long long)blockIdx.x * p.splits + split) * p.heads + g;
       p.acc[at * D + d] = x;
       if (d == 0) {
         p.ml[2 * at] = m;
@@ -322,33 +363,52 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   }
 }
 
-// Joins a head's chunks.  Grid: [B * H].  A chunk is JL lanes of four elements; the workgroup's rows of lanes
-// take chunks in turn, each with a running maximum of its own, and meet in LDS: the order is fixed by the
-// sequence's length alone.  Two memory round trips: the position, then every chunk's (m, l) and values.
+// Joins a head's parts.  Grid: [units * heads].  A part is JL lanes of four elements; the workgroup's rows of
+// lanes take parts in turn, each with a running maximum of its own, and meet in LDS: the order is fixed by the
+// sequences' lengths.  Of chunks it is known beforehand where they are, so that one memory round trip brings how
+// many there are and the first of them; of shares, two.
 template <int QT, int D>
 __global__ __launch_bounds__(1024) void paged_join_kernel(PagedDecode p) {
-  constexpr int JL = D <= 32 ? 8 : D <= 64 ? 16 : 32;
-  const int b = blockIdx.x / p.H, rows = blockDim.x / JL;
+  constexpr int JL = D <= 32 ? 8 : D <= 64 ? 16 : 32, U = 4;
+  const int unit = blockIdx.x / p.heads, h = blockIdx.x - unit * p.heads, rows = blockDim.x / JL;
   const int gl = threadIdx.x % JL, r = threadIdx.x / JL;
-  const int chunks = chunks_of(p, rows_of(p, b));
-  if (chunks == 1) return;  // (written by its only workgroup)
-  const float2* ml = reinterpret_cast<const float2*>(p.ml) + (long long)blockIdx.x * p.splits;
-  const float* acc = p.acc + (long long)blockIdx.x * p.splits * D + 4 * gl;
-  constexpr int U = 4;
-  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = r; c0 < chunks; c0 += U * rows) {
-    float2 s[U];
-    float4 v[U];
+  const int units = (p.G + p.heads - 1) / p.heads;  // of a key/value head
+  const int bk = unit / units, hq = (unit - bk * units) * p.heads + h;
+  if (hq >= p.G) return;
+  const long long head = (long long)bk * p.G + hq;
+  float2 s[U];
+  float4 v[U];
+  const float2* ml = reinterpret_cast<const float2*>(p.ml) + h;
+  const float* acc = p.acc + (long long)h * D + 4 * gl;
+  auto load = [&](long long first, int c0, int parts) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = c0 + u * rows;
-      const bool live = c < chunks;
-      s[u] = live ? ml[c] : make_float2(-INFINITY, 0.f);
-      v[u] = live && 4 * gl < D ? *reinterpret_cast<const float4*>(acc + (long long)c * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[u] = make_float2(-INFINITY, 0.f);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < parts) {
+        s[u] = ml[(first + c) * p.heads];
+        if (4 * gl < D) v[u] = *reinterpret_cast<const float4*>(acc + (first + c) * p.heads * D);
+      }
     }
+  };
+  const bool chunked = p.shares == 0;
+  if (chunked) load((long long)unit * p.splits, r, p.splits);
+  const int2 join = p.joins[unit];
+  const int parts = join.y;
+  if (parts == 1) return;  // (written by its only workgroup)
+  if (!chunked) load(join.x, r, parts);
+  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = r;;) {
     float mn = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, s[u].x);
+    for (int u = 0; u < U; ++u) {
+      if (c0 + u * rows >= parts) {  // (what lies behind the last part was never written)
+        s[u] = make_float2(-INFINITY, 0.f);
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      mn = fmaxf(mn, s[u].x);
+    }
     const float a = weight(m, mn);
     m = mn;
     l *= a;
@@ -363,6 +423,9 @@ __global__ __launch_bounds__(1024) void paged_join_kernel(PagedDecode p) {
       x[2] = fmaf(v[u].z, w, x[2]);
       x[3] = fmaf(v[u].w, w, x[3]);
     }
+    c0 += U * rows;
+    if (c0 >= parts) break;
+    load(join.x, c0, parts);
   }
   __shared__ float jm[1024 / JL], jl[1024 / JL], jx[1024 / JL][D];
   if (4 * gl < D)
@@ -373,42 +436,45 @@ __global__ __launch_bounds__(1024) void paged_join_kernel(PagedDecode p) {
     jl[r] = l;
   }
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  const int n = min(rows, chunks);
+  const int n = min(rows, parts);
   m = -INFINITY;
   for (int i = 0; i < n; ++i) m = fmaxf(m, jm[i]);
-  float o = 0.f;
-  l = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const float w = weight(jm[i], m);
-    l = fmaf(jl[i], w, l);
-    o = fmaf(jx[i][threadIdx.x], w, o);
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float o = 0.f;
+    l = 0.f;
+    for (int i = 0; i < n; ++i) {
+      const float w = weight(jm[i], m);
+      l = fmaf(jl[i], w, l);
+      o = fmaf(jx[i][d], w, o);
+    }
+    store_out<QT>(p.out, head * D + d, o / l);
   }
-  store_out<QT>(p.out, (long long)blockIdx.x * D + threadIdx.x, o / l);
 }
 
-// The kernels of a call and its split.
-struct Plan {
-  bool mfma;
-  int heads;  // query heads of a workgroup
-};
+long long units_of(const PagedDecode& p) { return (long long)p.c.B * p.c.Hkv * ((p.G + p.heads - 1) / p.heads); }
 
-Plan plan(PagedDecode& p, int dtype, int cache_dtype, int D) {
-  Plan k;
-  k.mfma = p.G >= 2 && paged_mfma_takes(p, dtype, cache_dtype);
+// Chooses the kernel (true: matrix instructions) and the split; returns the parts (of `heads` each) that may have
+// to be joined.
+long long plan(PagedDecode& p, int dtype, int cache_dtype, int D, bool* mfma) {
+  *mfma = dtype != DSQG_F32 && paged_mfma_takes(p, dtype, cache_dtype);
   // Three groups of eight a lane leave registers for two heads of the vector kernel.
-  k.heads = k.mfma ? kMfmaHeads : p.G == 1 ? 1 : p.G == 2 || D == 80 || D == 96 ? 2 : 4;
+  p.heads = *mfma ? std::min(p.G, kMfmaHeads) : p.G == 1 ? 1 : p.G == 2 || D == 80 || D == 96 ? 2 : 4;
   const long long T = std::max(1ll, (long long)p.c.M << p.c.shift);
-  const long long units = (long long)p.c.B * p.c.Hkv * ((p.G + k.heads - 1) / k.heads);
-  // Rows of a chunk: a few workgroups for each place on the chip, not so short that a workgroup's beginning
-  // and end outweigh its rows.
-  const long long most = k.mfma ? 1024 : 1536, least = k.mfma ? 256 : 128;
-  long long chunk = ((T * units + most - 1) / most + 63) / 64 * 64;
-  chunk = std::min(4096ll, std::max(least, chunk));
-  chunk = std::max(chunk, (T / 65535 + 64) / 64 * 64);  // (the grid's limit)
+  const long long units = units_of(p), steps = units * ((T + kShareRows - 1) / kShareRows);
+  const long long places = *mfma ? paged_mfma_places(D) : 1536;
+  p.shares = p.splits = 0;
+  if (*mfma && p.c.B > 1 && p.c.B <= kShareSeqs && steps >= 16 * places && steps < (1ll << 30)) {
+    p.shares = (int)places;
+    return places + units;
+  }
+  // Rows of a chunk, a power of two: about as many workgroups as places on the chip, not so short that a
+  // workgroup's beginning and end outweigh its rows.
+  long long chunk = *mfma ? 256 : 128;
+  while (chunk < 4096 && chunk * 3 * places < T * units * 2) chunk *= 2;
+  while ((T + chunk - 1) / chunk > 65535) chunk *= 2;  // (the grid's limit)
   p.splits = (int)((T + chunk - 1) / chunk);
   p.chunk = (int)chunk;
-  return k;
+  return p.splits > 1 ? units * p.splits : 0;
 }
 
 template <int QT, int CT, int D, int GT>
@@ -418,10 +484,10 @@ void launch(const PagedDecode& p, hipStream_t st) {
 }
 
 template <int QT, int CT, int D>
-void launch_heads(const PagedDecode& p, int heads, hipStream_t st) {
-  if (heads == 1) {
+void launch_heads(const PagedDecode& p, hipStream_t st) {
+  if (p.heads == 1) {
     launch<QT, CT, D, 1>(p, st);
-  } else if (heads == 2) {
+  } else if (p.heads == 2) {
     launch<QT, CT, D, 2>(p, st);
   } else if constexpr (RowMap<D>::pieces == 1) {
     launch<QT, CT, D, 4>(p, st);
@@ -429,42 +495,52 @@ void launch_heads(const PagedDecode& p, int heads, hipStream_t st) {
 }
 
 template <int QT, int D>
-void launch_types(const PagedDecode& p, const Plan& k, int ct, hipStream_t st) {
-  if (k.mfma) launch_paged_mfma(p, QT, ct, D, st);
-  else if (ct == DSQG_E4M3) launch_heads<QT, DSQG_E4M3, D>(p, k.heads, st);
-  else if (ct == DSQG_INT8) launch_heads<QT, DSQG_INT8, D>(p, k.heads, st);
-  else launch_heads<QT, QT, D>(p, k.heads, st);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((paged_join_kernel<QT, D>), dim3((unsigned)(p.c.B * p.H)), dim3(p.splits > 32 ? 1024 : 256), 0, st, p);
+void launch_types(const PagedDecode& p, bool mfma, int ct, hipStream_t st) {
+  if (mfma) launch_paged_mfma(p, QT, ct, D, st);
+  else if (ct == DSQG_E4M3) launch_heads<QT, DSQG_E4M3, D>(p, st);
+  else if (ct == DSQG_INT8) launch_heads<QT, DSQG_INT8, D>(p, st);
+  else if constexpr (QT == DSQG_F32) launch_heads<QT, QT, D>(p, st);
+  if (!p.joins) return;
+  // The join's rows of lanes: about as many as a unit has parts; it takes any number.
+  const long long blocks = units_of(p) * p.heads, parts = p.shares ? 2 + p.shares / units_of(p) : p.splits;
+  hipLaunchKernelGGL((paged_join_kernel<QT, D>), dim3((unsigned)blocks), dim3(parts > 32 ? 1024 : parts > 4 ? 256 : 64), 0, st, p);
 }
 
 template <int QT>
-void launch_dim(const PagedDecode& p, const Plan& k, int ct, int D, hipStream_t st) {
+void launch_dim(const PagedDecode& p, bool mfma, int ct, int D, hipStream_t st) {
   switch (D) {
-    case 32: launch_types<QT, 32>(p, k, ct, st); break;
-    case 64: launch_types<QT, 64>(p, k, ct, st); break;
-    case 80: launch_types<QT, 80>(p, k, ct, st); break;
-    case 96: launch_types<QT, 96>(p, k, ct, st); break;
-    default: launch_types<QT, 128>(p, k, ct, st); break;
+    case 32: launch_types<QT, 32>(p, mfma, ct, st); break;
+    case 64: launch_types<QT, 64>(p, mfma, ct, st); break;
+    case 80: launch_types<QT, 80>(p, mfma, ct, st); break;
+    case 96: launch_types<QT, 96>(p, mfma, ct, st); break;
+    default: launch_types<QT, 128>(p, mfma, ct, st); break;
   }
 }
 
 // The checks that the size query and the launch share; workspace bytes of the parts.
-int check_decode(const dsqg_paged_decode_args* a, PagedDecode* p, Plan* k, size_t* bytes) {
+int check_decode(const dsqg_paged_decode_args* a, PagedDecode* p, bool* mfma, long long* parts) {
   if (!a || a->H < 0) return DSQG_EINVAL;
   *p = PagedDecode{};
-  *bytes = 0;
+  *mfma = false;
+  *parts = 0;
   if (const int st = check_paged_cache(a->cache, &p->c)) return st;
   const dsqg_paged_cache& c = a->cache;
   if (c.cache_dtype <= DSQG_F16 && c.cache_dtype != c.dtype) return DSQG_EINVAL;
   if (c.Hkv > 0 ? a->H % c.Hkv != 0 : a->H != 0) return DSQG_EINVAL;
   if ((long long)c.B * a->H == 0) return DSQG_OK;
-  if ((long long)c.B * a->H >= (1ll << 23)) return DSQG_EUNSUPPORTED;  // grid: a workgroup of 256 a head
+  if ((long long)c.B * a->H >= (1ll << 21)) return DSQG_EUNSUPPORTED;  // grid: a join of 1024 for each, rounded up to units
+  // Offsets inside a page, and from page to page, are 32 bits.
+  if (p->c.kn * c.page >= (1ll << 31) || p->c.vn * c.page >= (1ll << 31) || p->c.kp >= (1ll << 31) || p->c.vp >= (1ll << 31))
+    return DSQG_EUNSUPPORTED;
   p->H = a->H;
   p->G = a->H / c.Hkv;
-  *k = plan(*p, c.dtype, c.cache_dtype, c.D);
-  if (p->splits > 1) *bytes = (size_t)c.B * a->H * p->splits * (2 + c.D) * sizeof(float);
-  return DSQG_OK;
+  *parts = plan(*p, c.dtype, c.cache_dtype, c.D, mfma);
+  return *parts < (1ll << 31) ? DSQG_OK : DSQG_EUNSUPPORTED;
+}
+
+// Bytes of the parts, D sums, a maximum and a sum for each head, and of the joins.
+size_t part_bytes(const PagedDecode& p, long long parts, int D) {
+  return parts ? (size_t)parts * p.heads * (D + 2) * sizeof(float) + (size_t)units_of(p) * sizeof(int2) : 0;
 }
 
 }  // namespace
@@ -474,15 +550,19 @@ using namespace dsqg;
 
 extern "C" int dsqg_paged_decode_workspace_size(const dsqg_paged_decode_args* a, size_t* bytes) {
   PagedDecode p;
-  Plan k;
-  return bytes ? check_decode(a, &p, &k, bytes) : (int)DSQG_EINVAL;
+  bool mfma;
+  long long parts;
+  if (!bytes) return DSQG_EINVAL;
+  if (const int st = check_decode(a, &p, &mfma, &parts)) return st;
+  *bytes = part_bytes(p, parts, a->cache.D);
+  return DSQG_OK;
 }
 
 extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t stream) {
   PagedDecode p;
-  Plan k;
-  size_t bytes = 0;
-  if (const int st = check_decode(a, &p, &k, &bytes)) return st;
+  bool mfma;
+  long long parts;
+  if (const int st = check_decode(a, &p, &mfma, &parts)) return st;
   const dsqg_paged_cache& c = a->cache;
   if ((long long)c.B * a->H == 0) return DSQG_OK;
   const long long es = elem_size(c.dtype);
@@ -495,8 +575,8 @@ extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t 
   if (!row(a->q, a->q_stride) || !a->pos || !a->out || (reinterpret_cast<uintptr_t>(a->out) & 15u) != 0) return DSQG_EINVAL;
   if (!a->k_new != !a->v_new) return DSQG_EINVAL;
   if (a->k_new && (!row(a->k_new, a->k_new_stride) || !row(a->v_new, a->v_new_stride))) return DSQG_EINVAL;
-  if (bytes > 0) {
-    if (!a->workspace || a->workspace_bytes < bytes) return DSQG_EWORKSPACE;
+  if (parts > 0) {
+    if (!a->workspace || a->workspace_bytes < part_bytes(p, parts, c.D)) return DSQG_EWORKSPACE;
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return DSQG_EINVAL;
   }
   p.scale = a->softmax_scale * 1.4426950408889634f;
@@ -505,11 +585,17 @@ extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t 
   p.vn = static_cast<const char*>(a->v_new); p.vnb = a->v_new_stride[0] * es; p.vnh = a->v_new_stride[1] * es;
   p.pos = reinterpret_cast<const long long*>(a->pos);
   p.out = static_cast<char*>(a->out);
-  p.acc = static_cast<float*>(a->workspace);
-  p.ml = p.acc + (long long)c.B * a->H * p.splits * c.D;
+  if (parts > 0) {
+    p.acc = static_cast<float*>(a->workspace);
+    p.ml = p.acc + parts * p.heads * c.D;
+    p.joins = reinterpret_cast<int2*>(p.ml + parts * p.heads * 2);
+  }
+  // Pools of more than a third of the 256 MB Infinity Cache are not found there by the next step, or only at
+  // the cost of what else it holds.
+  p.stream = 2ll * c.P * c.Hkv * c.page * c.D * elem_size(c.cache_dtype) > (85ll << 20);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (c.dtype == DSQG_F32) launch_dim<DSQG_F32>(p, k, c.cache_dtype, c.D, st);
-  else if (c.dtype == DSQG_BF16) launch_dim<DSQG_BF16>(p, k, c.cache_dtype, c.D, st);
-  else launch_dim<DSQG_F16>(p, k, c.cache_dtype, c.D, st);
+  if (c.dtype == DSQG_F32) launch_dim<DSQG_F32>(p, mfma, c.cache_dtype, c.D, st);
+  else if (c.dtype == DSQG_BF16) launch_dim<DSQG_BF16>(p, mfma, c.cache_dtype, c.D, st);
+  else launch_dim<DSQG_F16>(p, mfma, c.cache_dtype, c.D, st);
   return hipGetLastError() == hipSuccess ? DSQG_OK : DSQG_EHIP;
 }

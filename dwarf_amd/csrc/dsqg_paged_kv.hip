@@ -18,7 +18,7 @@ int check_paged_cache(const dsqg_paged_cache& a, PagedCache* c) {
   if (a.B < 0 || a.Hkv < 0 || a.D <= 0 || a.P < 0 || a.M < 0 || a.page <= 0) return DSQG_EINVAL;
   if ((a.page & (a.page - 1)) != 0) return DSQG_EINVAL;
   if (!head_dim_supported(a.D) || a.page < 16 || a.page > 65536) return DSQG_EUNSUPPORTED;
-  if ((long long)a.M * a.page >= (1ll << 31) || a.B > 65535 || a.Hkv > 65535) return DSQG_EUNSUPPORTED;
+  if ((long long)a.M * a.page > (1ll << 30) || a.B > 65535 || a.Hkv > 65535) return DSQG_EUNSUPPORTED;
   *c = PagedCache{};
   c->B = a.B; c->Hkv = a.Hkv; c->P = a.P; c->M = a.M;
   while ((1 << c->shift) < a.page) ++c->shift;

@@ -115,8 +115,16 @@ struct ValueMap {
   static constexpr int passes = kTile / rows;
 };
 
-template <int QT, int CT, int D>
-__global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
+// A workgroup's part: a unit, its rows from t0 on (at most `rows` of them), how many parts the unit has, and the
+// number of this one.
+struct Part {
+  int b, hk, g0, t0, rows, n;
+  int unit, count, at;
+};
+
+template <int QT, int CT, int D, bool SHARES>
+__device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf16_t (&sV)[kWaves][kTile * Geo<D>::RV],
+                                            float (&wm)[kWaves][kMfmaHeads], float (&wl)[kWaves][kMfmaHeads]) {
   using S = Steps<CT, D>;
   using V = ValueMap<CT, D>;
   constexpr bool F16 = CT == DSQG_F16;                       // operands in float16 (else bf16)
@@ -124,58 +132,40 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
   constexpr int ES = elem_size(CT), KS = S::count, DB = D / 16, RV = Geo<D>::RV;
   constexpr float kLift = F16 ? 14.f : 0.f;                  // weights are 2^kLift of the largest's
 
-  __shared__ __align__(16) bf16_t sV[kWaves][kTile * RV];
-  __shared__ float wm[kWaves][kMfmaHeads], wl[kWaves][kMfmaHeads];
-
-  const int ht = (p.G + kMfmaHeads - 1) / kMfmaHeads;
-  const int b = blockIdx.x / (p.c.Hkv * ht), rest = blockIdx.x - b * p.c.Hkv * ht;
-  const int hk = rest / ht, g0 = (rest - hk * ht) * kMfmaHeads;
-  const int split = blockIdx.y;
-  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = part.b, hk = part.hk, g0 = part.g0;
+  // (Opaque, so that what follows from it is worked out for each part and not held in registers across them.)
+  const int l = opaque(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = l & 15, g = l >> 4;
   const int heads = min(kMfmaHeads, p.G - g0);
 
   // The page numbers of the wave's next 32 tiles, one half each lane: no load stands between a tile and its
   // rows.  They need no position (entries behind the sequence's last page may be no pages: their rows are
-  // masked, whatever is said of them), so they are on their way together with it.
+  // masked, whatever is said of them), so with chunks they are on their way together with it.
   const int* table = p.c.table + b * p.c.ts;
   const int last = (p.c.M << p.c.shift) - 1;
-  auto page_of = [&](int t) { return last < 0 ? -1 : table[min(t, last) >> p.c.shift]; };
-  const int first = split * p.chunk + wave * kTile;
+  auto page_of = [&](int t) { return last < 0 ? -1 : table[min((unsigned)t, (unsigned)last) >> p.c.shift]; };
+  const int first = part.t0 + wave * kTile;
   auto pages_from = [&](int t) { return page_of(t + (l >> 1) * (kWaves * kTile) + 16 * (l & 1)); };
   int pages = pages_from(first);
+  Raw8<QT> qraw[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    raw_zero<QT>(qraw[s]);
+    const int d = S::at(s, g);
+    if (i < heads && d < D) qraw[s] = raw_load<QT>(p.q + b * p.qb + (hk * p.G + g0 + i) * p.qh + d * elem_size(QT));
+  }
 
-  const int n = rows_of(p, b);
-  const int chunks = chunks_of(p, n);
-  if (split >= chunks) return;
+  const int n = SHARES ? part.n : rows_of(p, b);
+  const int count = SHARES ? part.count : chunks_of(p, n);
+  if (!SHARES && (int)blockIdx.y >= count) return;
+  if (part.t0 == 0 && p.joins && threadIdx.x == 0) p.joins[part.unit] = make_int2(part.at, count);
   const long long h0 = (long long)b * p.H + hk * p.G + g0;  // first query head, in [B, H]
   if (n <= 0) {  // no rows: zeros; a position outside the table: NaN
     for (int e = threadIdx.x; e < heads * D; e += kBlock)
       store_out<QT>(p.out, h0 * D + e, n == 0 ? 0.f : __uint_as_float(0x7fc00000u));
     return;
   }
-  const int t1 = min(split * p.chunk + p.chunk, stored_of(p, n));
-
-  // Scores are taken times |scale|, so that their maximum may be found before it: a negative scale's sign
-  // goes to the queries.
-  const float scale = fabsf(p.scale);
-  const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
-  uint4 qh[KS], ql[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    Raw8<QT> r;
-    raw_zero<QT>(r);
-    const int d = S::at(s, g);
-    if (i < heads && d < D) r = raw_load<QT>(p.q + b * p.qb + (hk * p.G + g0 + i) * p.qh + d * elem_size(QT));
-    r.a = make_uint4(r.a.x ^ sign, r.a.y ^ sign, r.a.z ^ sign, r.a.w ^ sign);
-    if constexpr (QLO) {
-      float x[8];
-      raw_floats<QT>(r, x);
-      split8(x, qh[s], ql[s]);
-    } else {
-      qh[s] = r.a;
-    }
-  }
+  const int t1 = min(part.t0 + part.rows, stored_of(p, n));
 
   // The wave's tile: key operands' bytes, value rows' pieces, scale bytes of rows 4 g + r of each half.  Loads
   // go through a buffer resource for each half's sixteen rows, so that a lane has one offset for all keys and
@@ -192,7 +182,8 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
   const bf16_t* const vtr = sVw + (4 * g + (i >> 2)) * RV + 4 * (i & 3);
   const long long kh = hk * p.c.kh, vh = hk * p.c.vh, ksh = hk * p.c.ksh, vsh = hk * p.c.vsh;
 
-  auto load = [&](int k) {  // the wave's tile k
+  auto load_as = [&](int k, auto aux) {  // the wave's tile k; aux: the loads' cache policy
+    constexpr int AUX = decltype(aux)::value;
     const int tile = first + k * (kWaves * kTile);
     if ((k & 31) == 0 && k > 0) pages = pages_from(tile);
     __amdgpu_buffer_rsrc_t rk[2], rv[2];
@@ -224,7 +215,7 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
 #pragma unroll
       for (int q = 0; q < S::pairs; ++q) {
         if constexpr (narrow(CT)) {
-          const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk[h], klane + 64 * q, 0, 0));
+          const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk[h], klane + 64 * q, 0, AUX));
           kr[h][2 * q].a = make_uint2(x.x, x.y);
           kr[h][2 * q + 1].a = make_uint2(x.z, x.w);
         }
@@ -235,8 +226,8 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
         constexpr bool cut = D % 32 != 0;
         const bool out = cut && s == KS - 1 && g >= D % 32 / 8;
         const int off = krest + (S::at(s, 0) * ES);
-        if constexpr (narrow(CT)) kr[h][s].a = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rk[h], off, 0, 0));
-        else kr[h][s].a = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk[h], off, 0, 0));
+        if constexpr (narrow(CT)) kr[h][s].a = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rk[h], off, 0, AUX));
+        else kr[h][s].a = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk[h], off, 0, AUX));
         if (out) raw_zero<CT>(kr[h][s]);
       }
     }
@@ -247,14 +238,19 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
         // (A piece behind the row's end is not used.)
         const __amdgpu_buffer_rsrc_t r = rv[u * V::rows / 16];
         const int off = vlane + 16 * V::lanes * w, row = u * V::rows % 16 * vn;
-        uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, row, 0));
+        uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, row, AUX));
         if constexpr (V::rows > 16) {  // both halves in one pass
-          const uint4 y = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv[1], off, row, 0));
+          const uint4 y = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv[1], off, row, AUX));
           if (l / V::lanes >= 16) x = y;
         }
         vr[u][w] = x;
       }
     }
+  };
+
+  auto load = [&](int k) {
+    if (p.stream) load_as(k, std::integral_constant<int, 2>{});  // (non-temporal)
+    else load_as(k, std::integral_constant<int, 0>{});
   };
 
   // The tile's value rows below `live` to LDS as operand values, zeros in the others' place.
@@ -288,6 +284,27 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
     }
   };
 
+
+  if (first < t1) load(0);
+  __builtin_amdgcn_sched_barrier(0);
+
+  // Scores are taken times |scale|, so that their maximum may be found before it: a negative scale's sign
+  // goes to the queries.
+  const float scale = fabsf(p.scale);
+  const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
+  uint4 qh[KS], ql[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const Raw8<QT> r = {make_uint4(qraw[s].a.x ^ sign, qraw[s].a.y ^ sign, qraw[s].a.z ^ sign, qraw[s].a.w ^ sign)};
+    if constexpr (QLO) {
+      float x[8];
+      raw_floats<QT>(r, x);
+      split8(x, qh[s], ql[s]);
+    } else {
+      qh[s] = r.a;
+    }
+  }
+
   // Scores of 16 rows (A operands in a), before any scale.
   auto scores = [&](const Raw8<CT> (&a)[KS]) {
     f32x4_t s = zero4();
@@ -309,7 +326,7 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = zero4();
 
-  if (p.kn && split == 0 && wave == 0) {
+  if (p.kn && part.t0 == 0 && wave == 0) {
     // The new row begins the statistics: its score is row 0 of a product whose other rows are zeros, its
     // weight is the reference's.
     const int t = n - 1, at = __builtin_amdgcn_readfirstlane(page_of(t));
@@ -402,7 +419,6 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
     for (int d = 0; d < DB; ++d) o[d] *= e;
   }
 
-  if (first < t1) load(0);
 #pragma unroll 1
   for (int k = 0, tile = first; tile < t1; ++k, tile += kWaves * kTile) {
     const int live = t1 - tile;
@@ -493,10 +509,10 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
   lsum = col_sum(lsum);
   __builtin_amdgcn_s_waitcnt(0xc07f);
   __builtin_amdgcn_wave_barrier();
-  float* const part = reinterpret_cast<float*>(sVw);  // [16][D]
+  float* const sums = reinterpret_cast<float*>(sVw);  // [16][D]
   static_assert(kMfmaHeads * D * 4 <= kTile * RV * 2, "a wave's part fits its block");
 #pragma unroll
-  for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4_t*>(part + i * D + 16 * d + 4 * g) = o[d];
+  for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4_t*>(sums + i * D + 16 * d + 4 * g) = o[d];
   if (g == 0) {
     wm[wave][i] = m;
     wl[wave][i] = lsum;
@@ -513,10 +529,10 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
       ll = fmaf(wl[w][h], a, ll);
       x = fmaf(reinterpret_cast<const float*>(sV[w])[e], a, x);
     }
-    if (chunks == 1) {
+    if (count == 1) {
       store_out<QT>(p.out, h0 * D + e, x / ll);
     } else {
-      const long long at = (h0 + h) * p.splits + split;
+      const long long at = (long long)part.at * p.heads + h;
       p.acc[at * D + d] = x;
       if (d == 0) {
         p.ml[2 * at] = mm;
@@ -526,10 +542,71 @@ __global__ __launch_bounds__(kBlock, 3) void paged_mfma_kernel(PagedDecode p) {
   }
 }
 
+// Workgroups that a CU holds: by registers four waves a SIMD where rows are short, else three.
+constexpr int places(int D) { return D <= 64 ? 4 : 3; }
+
+template <int QT, int CT, int D, bool SHARES>
+__global__ __launch_bounds__(kBlock, places(D)) void paged_mfma_kernel(PagedDecode p) {
+  __shared__ __align__(16) bf16_t sV[kWaves][kTile * Geo<D>::RV];
+  __shared__ float wm[kWaves][kMfmaHeads], wl[kWaves][kMfmaHeads];
+  const int ht = (p.G + kMfmaHeads - 1) / kMfmaHeads;
+  const int units = p.c.Hkv * ht;
+  auto unit = [&](Part& part, int u) {  // unit u of sequence part.b
+    part.unit = part.b * units + u;
+    part.hk = u / ht;
+    part.g0 = (u - part.hk * ht) * kMfmaHeads;
+  };
+  Part part;
+  if constexpr (!SHARES) {
+    part.b = blockIdx.x / units;
+    unit(part, blockIdx.x - part.b * units);
+    part.t0 = blockIdx.y * p.chunk;
+    part.rows = p.chunk;
+    part.at = blockIdx.x * p.splits + blockIdx.y;
+    attend_part<QT, CT, D, false>(p, part, sV, wm, wl);
+  } else {
+    const int w = blockIdx.x;
+    int s, end, begin, per;
+    {
+      const ShareLine line(p);
+      per = line.per;
+      s = w * per;
+      end = min(s + per, line.steps());
+      if (s >= end) return;
+      part.b = line.sequence(p, s);
+      part.n = line.rows(part.b);
+      begin = line.before(p, part.b);
+    }
+#pragma unroll 1
+    while (true) {
+      const int steps = steps_of(p, part.n), u = (s - begin) / steps, at = s - begin - u * steps;
+      const int take = min(end - s, steps - at);
+      unit(part, u);
+      part.t0 = at * kShareRows;
+      part.rows = take * kShareRows;
+      part.at = w + part.unit;
+      // (Of the unit's first part, the count; of the others, whether they are all.)
+      part.count = at == 0 ? (s + steps - 1) / per - w + 1 : 2;
+      attend_part<QT, CT, D, true>(p, part, sV, wm, wl);
+      s += take;
+      if (s >= end) break;
+      if (s == begin + steps * units) {
+        part.n = rows_of(p, ++part.b);
+        begin = s;
+      }
+      __syncthreads();  // (the next part's values go where this one's sums were read)
+    }
+  }
+}
+
 template <int QT, int CT, int D>
 void launch(const PagedDecode& p, hipStream_t st) {
-  const unsigned units = (unsigned)(p.c.B * p.c.Hkv * ((p.G + kMfmaHeads - 1) / kMfmaHeads));
-  hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D>), dim3(units, (unsigned)p.splits), dim3(kBlock), 0, st, p);
+  if (p.shares) {
+    hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, true>), dim3((unsigned)p.shares), dim3(kBlock), 0, st, p);
+  } else {
+    const unsigned units = (unsigned)(p.c.B * p.c.Hkv * ((p.G + kMfmaHeads - 1) / kMfmaHeads));
+    hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, false>), dim3(units, (unsigned)p.splits), dim3(kBlock), 0, st, p);
+  }
 }
 
 template <int QT, int CT>
@@ -547,16 +624,14 @@ void launch_dim(const PagedDecode& p, int D, hipStream_t st) {
 
 bool paged_mfma_takes(const PagedDecode& p, int dtype, int cache_dtype) {
   if (dtype == DSQG_F32) return false;
-  // Offsets inside a half's sixteen rows, and inside a page, are 32 bits; so are the strides of pages.
-  const long long page = 1ll << p.c.shift;
-  if (p.c.kn * page >= (1ll << 31) || p.c.vn * page >= (1ll << 31) || ((p.c.kp | p.c.vp | p.c.ksp | p.c.vsp) >> 31) != 0)
-    return false;
   if (!narrow(cache_dtype)) return true;
-  // Scale bytes come four at a time.
+  // Scale bytes come four at a time, at 32-bit offsets from page to page.
   const long long odd = p.c.ksp | p.c.ksh | p.c.vsp | p.c.vsh | (long long)reinterpret_cast<uintptr_t>(p.c.ks) |
                         (long long)reinterpret_cast<uintptr_t>(p.c.vs);
-  return p.c.ksn == 1 && p.c.vsn == 1 && odd % 4 == 0;
+  return p.c.ksn == 1 && p.c.vsn == 1 && odd % 4 == 0 && p.c.ksp < (1ll << 31) && p.c.vsp < (1ll << 31);
 }
+
+int paged_mfma_places(int D) { return 256 * places(D); }
 
 void launch_paged_mfma(const PagedDecode& p, int dtype, int cache_dtype, int D, hipStream_t st) {
   if (dtype == DSQG_BF16) {
