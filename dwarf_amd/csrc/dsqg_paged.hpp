@@ -50,6 +50,18 @@ __device__ __forceinline__ Raw8<CT> raw_load(const void* p) { return *reinterpre
 template <int CT>
 __device__ __forceinline__ void raw_store(void* p, const Raw8<CT>& x) { *reinterpret_cast<Raw8<CT>*>(p) = x; }
 
+// The same past the caches' retention.
+template <int CT>
+__device__ __forceinline__ void raw_store_stream(void* p, const Raw8<CT>& x) {
+  typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+  if constexpr (narrow(CT)) {
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x2_t, x.a), reinterpret_cast<u32x2_t*>(p));
+  } else {
+    st16_stream(p, x.a);
+    if constexpr (CT == DSQG_F32) st16_stream(static_cast<char*>(p) + 16, x.b);
+  }
+}
+
 template <int CT>
 __device__ __forceinline__ void raw_zero(Raw8<CT>& x) { x = Raw8<CT>{}; }
 

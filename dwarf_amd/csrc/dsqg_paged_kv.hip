@@ -81,6 +81,7 @@ struct ReadParams {
   const long long* lengths;
   char* k; char* v;
   int T;
+  bool stream;     // the output is larger than the caches that the next launch could find it in
   long long rows;  // Hkv * T of one sequence
 };
 
@@ -158,8 +159,9 @@ __device__ __forceinline__ Raw8<OT> get_piece(const Raw8<CT>& r, float scale) {
   }
 }
 
-// Grid: as the write's, over the T positions of the output.
-template <int CT, int OT, int D>
+// Grid: as the write's, over the T positions of the output.  (STREAM: a parameter, as two stores in two branches
+// become one that is neither.)
+template <int CT, int OT, int D, bool STREAM>
 __global__ __launch_bounds__(kBlock) void paged_read_kernel(ReadParams p) {
   using R = RowMap<D>;
   constexpr int rpb = kBlock / R::lanes;
@@ -198,8 +200,14 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(ReadParams p) {
 #pragma unroll
   for (int u = 0; u < R::pieces; ++u)
     if (g + R::lanes * u < R::CPR) {
-      raw_store<OT>(p.k + out + (g + R::lanes * u) * 8 * elem_size(OT), x[u]);
-      raw_store<OT>(p.v + out + (g + R::lanes * u) * 8 * elem_size(OT), y[u]);
+      const long long at = out + (g + R::lanes * u) * 8 * elem_size(OT);
+      if constexpr (STREAM) {
+        raw_store_stream<OT>(p.k + at, x[u]);
+        raw_store_stream<OT>(p.v + at, y[u]);
+      } else {
+        raw_store<OT>(p.k + at, x[u]);
+        raw_store<OT>(p.v + at, y[u]);
+      }
     }
 }
 
@@ -213,8 +221,9 @@ void launch_write(const WriteParams& p, hipStream_t st) {
 template <int CT, int OT, int D>
 void launch_read(const ReadParams& p, hipStream_t st) {
   constexpr int rpb = kBlock / RowMap<D>::lanes;
-  hipLaunchKernelGGL((paged_read_kernel<CT, OT, D>), dim3((unsigned)((p.rows + rpb - 1) / rpb), (unsigned)p.c.B),
-                     dim3(kBlock), 0, st, p);
+  const dim3 grid((unsigned)((p.rows + rpb - 1) / rpb), (unsigned)p.c.B);
+  if (p.stream) hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, true>), grid, dim3(kBlock), 0, st, p);
+  else hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, false>), grid, dim3(kBlock), 0, st, p);
 }
 
 template <int DT, int D>
@@ -308,6 +317,8 @@ extern "C" int dsqg_paged_read(const dsqg_paged_read_args* a, dsqg_stream_t stre
   p.v = static_cast<char*>(a->v);
   p.T = a->T;
   p.rows = (long long)c.Hkv * a->T;
+  // Results that the eight L2s (32 MB) cannot hold push the pool's lines out of them for nothing.
+  p.stream = 2ll * c.B * p.rows * c.D * elem_size(c.dtype) > (32ll << 20);
   if (p.rows >= kMostRows) return DSQG_EUNSUPPORTED;
   for_dim<ReadDim>(c.D, p, c.dtype, c.cache_dtype, reinterpret_cast<hipStream_t>(stream));
   return hipGetLastError() == hipSuccess ? DSQG_OK : DSQG_EHIP;

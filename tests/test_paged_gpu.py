@@ -371,6 +371,37 @@ def test_step_long_sequences(gpu_device, dtype, kv, G, D):
     assert torch.equal(a, b)
 
 
+class RaggedCache(Cache):
+    """A pool of just the pages that the lengths need, under a table for sequences of up to M pages."""
+
+    def __init__(self, dev, H, D, page, M, dtype, kv, lengths, seed=0):
+        used = [-(-max(n, 0) // page) for n in lengths]
+        super().__init__(dev, 1, H, D, page, sum(used), dtype, kv, seed=seed)
+        order, table, at = self.table[0].cpu(), torch.full((len(lengths), M), -1, dtype=torch.int32), 0
+        for b, u in enumerate(used):
+            table[b, :u] = order[at:at + u]
+            at += u
+        self.table, self.lengths = table.to(dev), lengths
+
+
+@pytest.mark.parametrize("B,H,G,D,dtype,kv,most", [
+    (40, 4, 1, 64, BF, None, 2200), (40, 4, 3, 64, F16, None, 2200), (40, 4, 2, 128, BF, None, 1300), (33, 4, 4, 96, BF, E4, 1500),
+    (300, 1, 20, 32, BF, I8, 700), (512, 1, 2, 32, F16, E4, 400), (7, 20, 1, 80, BF, None, 3000)])
+def test_step_shares(gpu_device, B, H, G, D, dtype, kv, most):
+    """Large batches under long tables, whose rows the kernel deals out in equal shares: shares of several
+    sequences, sequences of several shares, rows that end anywhere, sequences without rows."""
+    g = torch.Generator().manual_seed(B)
+    pos = (torch.rand(B, generator=g) ** 2 * most).long().tolist()
+    pos[0], pos[1], pos[2], pos[-1], pos[-2] = 127, 128, -1, 255, 256
+    M = 16 * 768 * 16 * 128 // (B * H * 32) + 64
+    c = RaggedCache(gpu_device, H, D, 32, M * 2, dtype, kv, [p + 1 for p in pos])
+    junk(c, [p + 1 for p in pos])
+    pos[3] = c.table.shape[1] * 32 + 5  # past the table
+    for fresh in (True, False):
+        a = _step(c, pos, G, fresh)
+    same(_step(c, pos, G, False), a)
+
+
 @pytest.mark.parametrize("pool", ["tokens", "wide"])
 @pytest.mark.parametrize("dtype,kv,G", [(BF, None, 1), (F32, None, 2), (BF, E4, 4), (F16, I8, 8), (BF, None, 8)])
 def test_step_pools(gpu_device, dtype, kv, G, pool):
