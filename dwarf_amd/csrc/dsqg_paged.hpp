@@ -223,12 +223,21 @@ struct PagedDecode {
 constexpr int kShareRows = 128;
 constexpr int kShareSeqs = 512;  // sequences that a wave places its share among: eight a lane
 
+// A load from memory that nothing writes while the kernel runs (positions, page numbers): of a uniform address a
+// scalar load, which waits in no queue behind the rows' loads.
+template <typename T>
+__device__ __forceinline__ T load_const(const T* p) {
+  typedef const __attribute__((address_space(4))) T* const_ptr;
+  return *(const_ptr)(unsigned long long)p;
+}
+
 // Rows of sequence b that the step attends (0: none) or -1 where its position has no place in the table.
-__device__ __forceinline__ int rows_of(const PagedDecode& p, int b) {
-  const long long pos = p.pos[b];
+__device__ __forceinline__ int rows_at(const PagedDecode& p, long long pos) {
   if (pos < 0) return 0;
   return pos >= ((long long)p.c.M << p.c.shift) ? -1 : (int)pos + 1;
 }
+
+__device__ __forceinline__ int rows_of(const PagedDecode& p, int b) { return rows_at(p, load_const(p.pos + b)); }
 
 // Rows that are read from the pool (the new one is not), and the chunks or steps that they make.
 __device__ __forceinline__ int stored_of(const PagedDecode& p, int n) { return p.kn ? n - 1 : n; }

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   // their rows are masked, whatever is said of them), so all of them are on their way together.
   const int* table = p.c.table + b * p.c.ts;
   const int last = (p.c.M << p.c.shift) - 1;
-  auto page_of = [&](int t) { return last < 0 ? -1 : table[min((unsigned)t, (unsigned)last) >> p.c.shift]; };
+  auto page_of = [&](int t) { return last < 0 ? -1 : load_const(table + (min((unsigned)t, (unsigned)last) >> p.c.shift)); };
   const int t0 = split * p.chunk, first = t0 + wave * TR;
   auto pages_from = [&](int t) { return page_of(t + lane / U * stride + lane % U * R::rows); };
   int pages = pages_from(first);
@@ -158,7 +158,8 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   Running<GT, PC> s;
   s.clear();
 
-  if (fresh && split == 0 && wave == 0) {  // the new row, in the first row group
+  // The new row, in the first row group of the first chunk's last wave (no other has fewer tiles).
+  if (fresh && split == 0 && wave == kWaves - 1) {
     const char* kn = p.kn + b * p.knb + hk * p.knh;
     const char* vn = p.vn + b * p.vnb + hk * p.vnh;
     Raw8<QT> x[PC], y[PC];
