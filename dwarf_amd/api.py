@@ -209,8 +209,9 @@ def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_
     (float8_e4m3fn or int8) with k_scale, v_scale [P,Hkv,page] float8_e8m0fnu: a row's scale is the
     smallest power of two that brings its largest magnitude to at most 448 or 127, and its values are
     rounded once.  A row that holds an infinity or NaN reads as NaN from 8-bit pages.  Positions without
-    a page (a number that is none of the pool's, a position past the table) are not written.  No gradient
-    passes through the cache.
+    a page (a number that is none of the pool's, a position past the table) are not written.  Sequences may
+    share pages that none of them writes; a page that two of them write, or rows that are views of the pages
+    themselves, have no defined result.  No gradient passes through the cache.
     """
     if ops.traced(k, v, k_pages, v_pages):
         return ops.paged_kv_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
@@ -327,16 +328,23 @@ class PagedKVCache:
         """Write prompts k, v [B,H,N,D] from position 0 on, counts[b] rows of each (default: N); pos becomes
         that."""
         assert k.shape[2] <= self.max_len, f"prompt of {k.shape[2]} rows exceeds the cache ({self.max_len})"
-        self.pos.zero_()
-        self.write(k, v, counts)
+        counts = self._write(k, v, torch.zeros_like(self.pos), counts)
+        if counts is None:
+            self.pos.fill_(k.shape[2])
+        else:
+            self.pos.copy_(counts)
 
     def write(self, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
         """Append rows k, v [B,H,N,D], counts[b] of each (default: N), and advance."""
-        k, v = k.detach().to(self.dtype), v.detach().to(self.dtype)
+        counts = self._write(k, v, self.pos, counts)
+        self.pos += k.shape[2] if counts is None else counts
+
+    def _write(self, k: Tensor, v: Tensor, pos: Tensor, counts: Optional[Tensor]) -> Optional[Tensor]:
         if counts is not None:
             counts = counts.clamp(0, k.shape[2])
-        paged_kv_write(k, v, self.k_pages, self.v_pages, self.page_table, self.pos, counts=counts, **self._state())
-        self.pos += k.shape[2] if counts is None else counts
+        paged_kv_write(k.detach().to(self.dtype), v.detach().to(self.dtype), self.k_pages, self.v_pages,
+                       self.page_table, pos, counts=counts, **self._state())
+        return counts
 
     def step(self, q: Tensor, k_new: Tensor, v_new: Tensor, softmax_scale: Optional[float] = None) -> Tensor:
         """Output [B,H*G,D] of one new token per sequence at its position, which advances."""

@@ -854,11 +854,11 @@ struct Paged {
   }
 };
 
-// No gradient passes through a cache: a call that records one is refused.
+// No gradient passes through a cache: a call that records one, or carries a tangent, is refused.
 void refuse_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
+  const bool grad = at::GradMode::is_enabled();
   for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad())
+    if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(0).defined()))
       raise(PyExc_RuntimeError, "the paged cache has no gradient: detach its operands, or call it under torch.no_grad()");
 }
 

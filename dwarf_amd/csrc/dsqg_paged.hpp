@@ -322,6 +322,12 @@ __device__ __forceinline__ float weight(float a, float b) {
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
 }
 
+// The largest weight is 2^lift, not 1: sums of 2^30 rows of the largest float32 or bfloat16 value stay finite, as
+// their mean is, until the last division (and values above 2^-96 keep their precision); in float16 products
+// weights are larger instead, so that small ones stay clear of its subnormal numbers.
+template <bool F16>
+constexpr float weight_lift() { return F16 ? 14.f : -30.f; }
+
 // Largest group of query heads that one workgroup of the matrix-instruction kernel takes.
 constexpr int kMfmaHeads = 16;
 

@@ -60,6 +60,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   using R = RowMap<D>;
   constexpr int PC = R::pieces, ES = elem_size(CT);
   constexpr int U = CT == DSQG_F32 || PC > 1 ? 2 : 4;  // passes of a tile
+  constexpr float kLift = weight_lift<false>();
   constexpr int TR = U * R::rows, stride = kWaves * TR;
   const int hg = (p.G + GT - 1) / GT;
   const int b = blockIdx.x / (p.c.Hkv * hg), rest = blockIdx.x - b * p.c.Hkv * hg;
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
       d = group_sum<R::lanes>(d) * (p.scale * sk);
       if (!ok) d = __uint_as_float(0x7fc00000u);  // nowhere to keep the row
       if (r == 0) {
-        s.m[g] = fmaxf(d, -INFINITY);
+        s.m[g] = fmaxf(d, -INFINITY) - kLift;
         s.l[g] = weight(d, s.m[g]);
 #pragma unroll
         for (int u = 0; u < PC; ++u) {
@@ -278,9 +279,10 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
     }
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
-      float m = s.m[g];
+      float m = sc[g][0];
 #pragma unroll
-      for (int u = 0; u < U; ++u) m = fmaxf(m, sc[g][u]);
+      for (int u = 1; u < U; ++u) m = fmaxf(m, sc[g][u]);
+      m = fmaxf(s.m[g], m - kLift);
       const float a = weight(s.m[g], m);
       s.m[g] = m;
       s.l[g] *= a;

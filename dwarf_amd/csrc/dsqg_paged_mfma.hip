@@ -67,8 +67,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo
 }
 
 // Eight weights (none negative) as two 16-bit terms, hi rounded down and lo what remains, so that neither is
-// negative.  Where values may be infinite (INF: not in 8 bits) lo is the type's smallest number (2^-126,
-// 2^-24) where nothing remains: an infinity times both terms is that infinity, but times zero NaN.
+// negative.  Where values may be infinite (INF: not in 8 bits) lo of a weight above zero is above zero too, the
+// type's smallest number (2^-126, 2^-24) where nothing remains: an infinity times both terms is that infinity,
+// but times zero NaN.
 template <bool F16, bool INF>
 __device__ __forceinline__ void split_weights(const float (&w)[8], uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
@@ -78,13 +79,14 @@ __device__ __forceinline__ void split_weights(const float (&w)[8], uint4& hi, ui
     if constexpr (F16) {
       h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
       const f16x2_t q = __builtin_bit_cast(f16x2_t, h[i]);
-      l[i] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)fmaxf(a - (float)q[0], 0x1p-24f), (_Float16)fmaxf(b - (float)q[1], 0x1p-24f)});
+      l[i] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)fmaxf(a - (float)q[0], fminf(a, 0x1p-24f)),
+                                                  (_Float16)fmaxf(b - (float)q[1], fminf(b, 0x1p-24f))});
     } else {
       h[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // the upper halves
       float x = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), y = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
       if constexpr (INF) {
-        x = fmaxf(x, 0x1p-126f);
-        y = fmaxf(y, 0x1p-126f);
+        x = fmaxf(x, fminf(a, 0x1p-126f));
+        y = fmaxf(y, fminf(b, 0x1p-126f));
       }
       l[i] = cvt_pk_bf16(x, y);
     }
@@ -130,7 +132,7 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
   constexpr bool F16 = CT == DSQG_F16;                       // operands in float16 (else bf16)
   constexpr bool QLO = QT == DSQG_F16 && narrow(CT);         // queries in two terms
   constexpr int ES = elem_size(CT), KS = S::count, DB = D / 16, RV = Geo<D>::RV;
-  constexpr float kLift = F16 ? 14.f : 0.f;                  // weights are 2^kLift of the largest's
+  constexpr float kLift = weight_lift<F16>();
 
   const int b = part.b, hk = part.hk, g0 = part.g0;
   // (Opaque, so that what follows from it is worked out for each part and not held in registers across them.)

@@ -86,7 +86,7 @@ def bound(out, mass, size, D, T, dtype):
     normalised one twice that.  The sums over T rows: T u each, twice; joining parts: a few roundings each,
     16 u.  All of these are relative to ``mass[:, 0]``.  A weight, or its product with the factor that a
     larger maximum brings, that lies below the normal numbers may come out as zero, which three such
-    products in turn (tile, wave, chunk) add up to 4 * 2^-126 for each row, as the largest weight is 1:
+    products in turn (tile, wave, chunk) add up to 4 * 2^-96 for each row, as the largest weight is 2^-30:
     that much of ``mass[:, 1]``.  Weights that enter a product in two 16-bit terms are 2^-16 off in bfloat16
     (a term of 8 bits rounded down and one of 8 bits rounded: 2^-7 * 2^-9) and, in float16, 2^-21 (2^-10 *
     2^-11) or its subnormal step where the largest weight is 2^14: 2 * 2^-38 of ``mass[:, 1]`` (a float32
@@ -95,7 +95,7 @@ def bound(out, mass, size, D, T, dtype):
     """
     u = 2.0 ** -24
     w = 2 * ((D + 7) * u * size + 2 * u)
-    tol = mass[:, 0] * (w + (2 * T + 16) * u) + mass[:, 1] * 4 * 2.0 ** -126
+    tol = mass[:, 0] * (w + (2 * T + 16) * u) + mass[:, 1] * 4 * 2.0 ** -96
     if dtype != torch.float32:
         tol = tol + mass[:, 0] * 2.0 ** -16 + (mass[:, 1] * 2.0 ** -37 if dtype == torch.float16 else 0)
     fi = torch.finfo(dtype)

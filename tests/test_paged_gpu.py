@@ -460,6 +460,71 @@ def test_step_special_values(gpu_device, dtype, kv, G):
     assert not nan[4:].any()
 
 
+@pytest.mark.parametrize("dtype,kv,G", [(BF, None, 1), (BF, None, 8), (F16, None, 4), (F32, None, 1), (F32, None, 4)])
+def test_step_ignores_values_of_no_weight(gpu_device, dtype, kv, G):
+    """Values at the type's limits count for nothing where their weight is zero, in front of the row that has
+    it all, behind it, and in the same tile."""
+    n, D = 400, 64
+    c = Cache(gpu_device, 1, 1, D, 16, 25, dtype, kv)
+    table = c.table.cpu()[0]
+    c.k.zero_()
+    c.v.fill_(torch.finfo(dtype).max)
+    c.k[int(table[200 // 16]), 0, 200 % 16] = 100.0
+    c.v[int(table[200 // 16]), 0, 200 % 16] = torch.arange(D, device=gpu_device).to(dtype)
+    q = torch.ones(1, G, D, device=gpu_device, dtype=dtype)  # a score of 800 against zeros
+    out = paged_decode_step(q, None, None, c.k, c.v, c.table, torch.tensor([n - 1], device=gpu_device))
+    assert torch.equal(out[0].float().cpu(), torch.arange(D).float().expand(G, D))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("kv", [E4, I8])
+def test_every_code_reads_alike(gpu_device, kv, G, dtype):
+    """All 256 codes under scales from the smallest to ones that overflow: what is read back, and the output of
+    a step over one row, which is its value."""
+    bytes_ = [0, 1, 60, 120, 127, 130, 200, 247, 254, 255]
+    n = 8 * len(bytes_)
+    c = Cache(gpu_device, n, 1, 32, 16, 1, dtype, kv)
+    codes = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(8, 32).repeat(len(bytes_), 1)
+    e = torch.tensor(bytes_, dtype=torch.uint8).repeat_interleave(8)
+    page = c.table[:, 0].long()
+    c.v.view(torch.uint8)[page, 0, 0] = codes.to(gpu_device)
+    c.v_scale.view(torch.uint8)[page, 0, 0] = e.to(gpu_device)
+    c.k.view(torch.uint8)[page, 0, 0] = 0
+    want = po.values(codes.view(kv), e.view(torch.float8_e8m0fnu)).float().to(dtype)
+    _, v = paged_kv_read(c.k, c.v, c.table, torch.ones(n, dtype=torch.int64, device=gpu_device), 1, dtype=dtype, **c.state)
+    q = torch.ones(n, G, 32, device=gpu_device, dtype=dtype)
+    out = paged_decode_step(q, None, None, c.k, c.v, c.table, torch.zeros(n, dtype=torch.int64, device=gpu_device), **c.state)
+    for x in (v[:, 0, 0].cpu(), *out.unbind(1)):
+        x = x.cpu()
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(x), nan)
+        ok = ~nan
+        # (The one weight is 2^-30 until the last division, in two terms of 8 bits: values below 2^-90 come near
+        # the numbers that float32 holds to fewer bits, and the step promises them to 2^-94 only.)
+        ok &= (want.float().abs() > 2.0 ** -90) | (want == 0)
+        assert torch.equal(x[ok], want[ok])
+
+
+def test_refuses_what_is_more_than_values(gpu_device):
+    """Tangents, vmap's wrappers and gradients on a pool."""
+    import torch.autograd.forward_ad as fw
+    c = Cache(gpu_device, 1, 1, 32, 16, 1, BF)
+    row, pos = torch.zeros(1, 1, 32, device=gpu_device, dtype=BF), torch.zeros(1, dtype=torch.int64, device=gpu_device)
+    with fw.dual_level():
+        for i in range(3):
+            ops = [row, row.clone(), row.clone()]
+            ops[i] = fw.make_dual(ops[i], ops[i].clone())
+            with pytest.raises(RuntimeError):
+                paged_decode_step(*ops, c.k, c.v, c.table, pos)
+        with pytest.raises(RuntimeError):
+            paged_kv_write(fw.make_dual(row[:, :, None], row[:, :, None].clone()), row[:, :, None], c.k, c.v, c.table, pos)
+    before = c.k.clone()
+    with pytest.raises(Exception):
+        torch.vmap(lambda q: paged_decode_step(q, q, q, c.k, c.v, c.table, pos))(row[None])
+    same(c.k, before)
+
+
 @pytest.mark.parametrize("form", ["strided", "unaligned", "negated", "expanded"])
 def test_step_operand_layouts(gpu_device, form):
     B, H, G, D = 3, 2, 4, 64
