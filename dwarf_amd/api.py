@@ -299,6 +299,8 @@ class PagedKVCache:
     v_t)`` runs one decode step and advances, ``read()`` returns the rows.  Every sequence owns its pages,
     sequence b those from b * M on; a caller that shares or moves pages sets ``page_table``.  The host
     does not know the positions: rows past a sequence's last page are not kept, and its steps give NaN.
+    A sequence at a negative position is not in use: its pages and position stay as they are and its steps
+    give zeros, until ``pos`` is set again.
     """
 
     def __init__(self, B: int, H: int, D: int, max_len: int, dtype=torch.bfloat16, device="cuda",
@@ -336,8 +338,9 @@ class PagedKVCache:
 
     def write(self, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
         """Append rows k, v [B,H,N,D], counts[b] of each (default: N), and advance."""
-        counts = self._write(k, v, self.pos, counts)
-        self.pos += k.shape[2] if counts is None else counts
+        used = self.pos >= 0
+        counts = used * (k.shape[2] if counts is None else counts)
+        self.pos += self._write(k, v, self.pos, counts)
 
     def _write(self, k: Tensor, v: Tensor, pos: Tensor, counts: Optional[Tensor]) -> Optional[Tensor]:
         if counts is not None:
@@ -352,7 +355,7 @@ class PagedKVCache:
         out = paged_decode_step(q.detach().to(dt), k_new.detach().to(dt), v_new.detach().to(dt), self.k_pages,
                                 self.v_pages, self.page_table, self.pos, softmax_scale=softmax_scale,
                                 **self._state())
-        self.pos += 1
+        self.pos += self.pos >= 0
         return out.to(q.dtype)
 
     def read(self, max_len: Optional[int] = None, dtype: Optional[torch.dtype] = None):

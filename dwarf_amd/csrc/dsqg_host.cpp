@@ -928,8 +928,8 @@ Tensor paged_decode(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, 
   Paged c(kp, vp, table, ks, vs, dt, kn.defined());
   require(ks.has_value() || kp.scalar_type() == dt, "queries of ", dt, " do not go with pages of ", kp.scalar_type());
   const int64_t B = c.a.B, Hkv = c.a.Hkv, D = c.a.D, H = q0.size(1);
-  require(q0.size(0) == B && q0.size(2) == D && (Hkv > 0 ? H % Hkv == 0 : H == 0), "q must be [", B, ",H,", D,
-          "] with H a multiple of ", Hkv, ", got ", shape_str(q0.sizes()));
+  require(q0.size(0) == B && q0.size(2) == D && (Hkv > 0 ? H > 0 && H % Hkv == 0 : H == 0), "q must be [", B, ",H,", D,
+          "] with H a positive multiple of ", Hkv, ", got ", shape_str(q0.sizes()));
   for (const Tensor* t : {&kn, &vn})
     if (t->defined())
       require(t->sizes() == c10::IntArrayRef({B, Hkv, D}) && t->scalar_type() == dt, "k_new and v_new must be ", dt, " ",

@@ -529,7 +529,7 @@ int check_decode(const dsqg_paged_decode_args* a, PagedDecode* p, bool* mfma, lo
   if (const int st = check_paged_cache(a->cache, &p->c)) return st;
   const dsqg_paged_cache& c = a->cache;
   if (c.cache_dtype <= DSQG_F16 && c.cache_dtype != c.dtype) return DSQG_EINVAL;
-  if (c.Hkv > 0 ? a->H % c.Hkv != 0 : a->H != 0) return DSQG_EINVAL;
+  if (c.Hkv > 0 ? a->H == 0 || a->H % c.Hkv != 0 : a->H != 0) return DSQG_EINVAL;
   if ((long long)c.B * a->H == 0) return DSQG_OK;
   if ((long long)c.B * a->H >= (1ll << 21)) return DSQG_EUNSUPPORTED;  // grid: a join of 1024 for each, rounded up to units
   // Offsets inside a page, and from page to page, are 32 bits.

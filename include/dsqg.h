@@ -380,7 +380,7 @@ typedef struct {
 
 int dsqg_paged_read(const dsqg_paged_read_args* args, dsqg_stream_t stream);
 
-/* Decode step: one new token per sequence.  q and out are [B,H,D], H a multiple of Hkv (query head h
+/* Decode step: one new token per sequence.  q and out are [B,H,D], H a positive multiple of Hkv (query head h
  * attends key/value head h / (H / Hkv)), k_new and v_new [B,Hkv,D]; each but out (contiguous) has unit
  * inner stride, strides {b, h} and 16-byte aligned rows.  The step writes k_new and v_new to position
  * pos[b] (as dsqg_paged_write does) and gives

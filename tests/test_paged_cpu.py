@@ -116,6 +116,7 @@ BAD = [
     ("write", dict(k=z(1, 2, 3, 32), v=z(1, 2, 3, 32)), "k and v must be"),
     ("write", dict(k=z(2, 1, 3, 32), v=z(2, 1, 3, 32)), "k and v must be"),
     ("step", dict(q=z(2, 3, 32)), "multiple of 2"),
+    ("step", dict(q=z(2, 0, 32)), "multiple of 2"),
     ("step", dict(q=z(2, 2, 64)), "q must be"),
     ("step", dict(q=z(1, 2, 32)), "q must be"),
     ("step", dict(q=z(2, 2, 32, dtype=torch.float16)), "do not go with"),
@@ -243,7 +244,7 @@ def test_abi_checks_the_cache(name):
     ("dsqg_paged_write", dict(pos=None)), ("dsqg_paged_write", dict(k_stride=(960, 320, 68))),
     ("dsqg_paged_write", dict(v_stride=(960, -320, 64))), ("dsqg_paged_read", dict(T=-1)),
     ("dsqg_paged_read", dict(lengths=None)), ("dsqg_paged_read", dict(k=0x1004)), ("dsqg_paged_read", dict(v=None)),
-    ("dsqg_paged_decode", dict(H=5)), ("dsqg_paged_decode", dict(H=-3)), ("dsqg_paged_decode", dict(q=None)),
+    ("dsqg_paged_decode", dict(H=5)), ("dsqg_paged_decode", dict(H=-3)), ("dsqg_paged_decode", dict(H=0)), ("dsqg_paged_decode", dict(q=None)),
     ("dsqg_paged_decode", dict(q_stride=(384, 60))), ("dsqg_paged_decode", dict(k_new=None)),
     ("dsqg_paged_decode", dict(v_new=0x1004)), ("dsqg_paged_decode", dict(pos=None)), ("dsqg_paged_decode", dict(out=0x1002)),
 ])

@@ -755,6 +755,31 @@ def test_prompts_steps_and_reading_back(gpu_device, dtype, kv):
             assert torch.equal(rk[b, :, counts[b]:counts[b] + 5], k[b, :, :5])
 
 
+def test_sequences_that_are_not_in_use(gpu_device):
+    """At a negative position nothing is written, steps give zeros and the position stays; the others go on."""
+    B, H, D = 3, 2, 64
+    g = torch.Generator().manual_seed(7)
+    c, only = PagedKVCache(B, H, D, 40, BF, gpu_device, page_size=16), PagedKVCache(B, H, D, 40, BF, gpu_device, page_size=16)
+    k, v = (torch.randn(B, H, 9, D, generator=g).to(gpu_device, BF) for _ in range(2))
+    for x in (c, only):
+        x.prefill(k, v)
+    c.pos[1] = -1
+    c.write(k[:, :, :4], v[:, :, :4])
+    only.write(k[:, :, :4], v[:, :, :4])
+    assert c.pos.tolist() == [13, -1, 13]
+    c.write(k[:, :, :4], v[:, :, :4], torch.tensor([2, 3, 0], device=gpu_device))
+    only.write(k[:, :, :4], v[:, :, :4], torch.tensor([2, 0, 0], device=gpu_device))
+    assert c.pos.tolist() == [15, -1, 13]
+    for i in range(3):
+        q, kt, vt = (torch.randn(B, H, D, generator=g).to(gpu_device, BF) for _ in range(3))
+        a, b = c.step(q, kt, vt), only.step(q, kt, vt)
+        same(a[0], b[0])
+        same(a[2], b[2])
+        assert (a[1] == 0).all() and c.pos.tolist() == [16 + i, -1, 14 + i]
+    assert torch.equal(c.k_pages[3:6, :, 9:], torch.zeros_like(c.k_pages[3:6, :, 9:]))
+    assert torch.equal(c.k_pages[3, :, :9], k[1])
+
+
 def _model(dev, dtype):
     torch.manual_seed(0)
     m = dwarf_amd.CondMTransformer(101, 64, 3, 2, 128, 96, full_attn_layer=1, interference_interval=3)
