@@ -177,10 +177,12 @@ struct RowMap {
   static constexpr int rows = 64 / lanes;  // rows of a wave's pass
 };
 
-// Largest of x over aligned groups of G lanes (G = 4, 8, 16), in every lane; a NaN is kept.
+// The larger of two magnitudes, as bits (no sign is set): a NaN is larger than an infinity and so is kept.
 __device__ __forceinline__ float max_nan(float a, float b) {
-  return a > b || a != a ? a : b;
+  return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
+
+// Largest of x over aligned groups of G lanes (G = 4, 8, 16), in every lane.
 template <int G>
 __device__ __forceinline__ float group_max_nan(float x) {
   if constexpr (G >= 2) x = max_nan(x, dpp_f32<0xb1>(x));
