@@ -5,11 +5,14 @@
 //
 // One pass over the rows with a running maximum and sum: of the rows seen so far a group of lanes keeps
 // m = max s_t, l = sum 2^(s_t - m) and acc = sum 2^(s_t - m) v_t (scores in base 2), and the parts of
-// different rows join as  acc = sum_i 2^(m_i - m) acc_i.  Every key and value is read once, so memory bounds
-// the step, and short ones the launches and the round trips from the position to the rows.
+// different rows join as  acc = sum_i 2^(m_i - m) acc_i.  (m carries an offset, weight_lift: the largest weight
+// is not 1.)  Every key and value is read once, so memory bounds the step, and short ones the launches and the
+// round trips from the position to the rows.
 //
-// 16-bit queries take the matrix instructions (dsqg_paged_mfma.hip).  The kernel here takes float32 ones, whose
-// products those instructions would round, and 8-bit pools whose scales they cannot read four at a time.
+// 16-bit queries take the matrix instructions (dsqg_paged_mfma.hip, with the figures of long steps).  The kernel
+// here takes float32 ones, whose products those instructions would round, and 8-bit pools whose scales they
+// cannot read four at a time.  4 float32 sequences of up to 2048 positions, 8 heads of 32 (10 MB): 5.2 us and
+// 3.8 for the join; a launch alone is about 3 of each.
 //
 // Its workgroup has one key/value head of one sequence, up to GT of the query heads that share it, and a
 // chunk of the sequence's rows; its four waves take tiles in turn.  In a tile a row is 4, 8 or 16
@@ -466,12 +469,19 @@ long long plan(PagedDecode& p, int dtype, int cache_dtype, int D, bool* mfma) {
   const long long units = units_of(p), steps = units * ((T + kShareRows - 1) / kShareRows);
   const long long places = *mfma ? paged_mfma_places(D) : 1536;
   p.shares = p.splits = 0;
+  // Shares pay where a place gets many steps, so that the lengths' differences and not the shares' beginnings
+  // cost: 43 steps a place (64 sequences of up to 8192, 8 heads of 128 over e4m3) 121 us against 128 in chunks,
+  // but 6 (32 of up to 2048, 12 heads of 64) 31.1 against 30.7 and 2.6 (16 of up to 16001, one head of 96) 23.6
+  // against 20.7.  One sequence's chunks are equal as they are.
   if (*mfma && p.c.B > 1 && p.c.B <= kShareSeqs && steps >= 16 * places && steps < (1ll << 30)) {
     p.shares = (int)places;
     return places + units;
   }
   // Rows of a chunk, a power of two: about as many workgroups as places on the chip, not so short that a
-  // workgroup's beginning and end outweigh its rows.
+  // workgroup's beginning and end outweigh its rows.  Measured at 256 / 512 / 1024 / 2048 rows: one sequence of
+  // 131072, 8 heads of 64: 47.7 / 46.3 / 46.0 / 46.2 us (1024 taken); 32 of up to 2048, 12 heads of 64: 30.4 /
+  // 30.5 / 32.1 / 33.4 (512); 16 of up to 16001, one head of 96: 21.0 / 20.1 / 19.8 / 23.6 (256); 5 of up to
+  // 5001, 3 heads of 80 over int8: 13.6 / 16.4 / 22.2 / 35 (256; 13.2 at 128).
   long long chunk = *mfma ? 256 : 128;
   while (chunk < 4096 && chunk * 3 * places < T * units * 2) chunk *= 2;
   while ((T + chunk - 1) / chunk > 65535) chunk *= 2;  // (the grid's limit)
@@ -594,7 +604,8 @@ extern "C" int dsqg_paged_decode(const dsqg_paged_decode_args* a, dsqg_stream_t 
     p.joins = reinterpret_cast<int2*>(p.ml + parts * p.heads * 2);
   }
   // Pools of more than a third of the 256 MB Infinity Cache are not found there by the next step, or only at
-  // the cost of what else it holds.
+  // the cost of what else it holds: rows read past it take 10 % less time at 130 to 680 MB, but 11 to 14 % more
+  // at 62 MB, which the cache serves.
   p.stream = 2ll * c.P * c.Hkv * c.page * c.D * elem_size(c.cache_dtype) > (85ll << 20);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (c.dtype == DSQG_F32) launch_dim<DSQG_F32>(p, mfma, c.cache_dtype, c.D, st);
