@@ -196,8 +196,9 @@ __device__ __forceinline__ float group_max_nan(float x) {
 
 // A step's work is split over workgroups in one of two ways.
 //  * Chunks (shares = 0): a workgroup for each unit (a sequence's key/value head and up to `heads` of its query
-//    heads) and chunk of `chunk` rows, as many chunks as the longest sequence that the table could hold would
-//    have; those behind a sequence's end leave at once.
+//    heads) and chunk of `chunk` rows (all that the table holds, where it is short or units are many), as many
+//    chunks as the longest sequence that the table could hold would have; those behind a sequence's end leave at
+//    once.
 //  * Shares: the rows of all units in one line, in steps of kShareRows, cut into `shares` equal parts, one a
 //    workgroup: however the lengths differ, every workgroup has the same number of steps and no place on the chip
 //    waits for the longest sequence.  A share may cover parts of several units; part w of unit u is number w + u
@@ -337,7 +338,8 @@ constexpr int kMfmaHeads = 16;
 // over p.splits chunks (the join is the caller's).
 bool paged_mfma_takes(const PagedDecode& p, int dtype, int cache_dtype);
 void launch_paged_mfma(const PagedDecode& p, int dtype, int cache_dtype, int D, hipStream_t st);
-// Workgroups of it that the chip holds.
+// Workgroups of it that the chip holds, and whether it takes shares of these rows.
 int paged_mfma_places(int D);
+constexpr bool paged_mfma_shares(int cache_dtype, int D) { return D < 128 || narrow(cache_dtype); }
 
 }  // namespace dsqg

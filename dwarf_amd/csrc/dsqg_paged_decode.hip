@@ -465,25 +465,34 @@ long long plan(PagedDecode& p, int dtype, int cache_dtype, int D, bool* mfma) {
   *mfma = dtype != DSQG_F32 && paged_mfma_takes(p, dtype, cache_dtype);
   // Three groups of eight a lane leave registers for two heads of the vector kernel.
   p.heads = *mfma ? std::min(p.G, kMfmaHeads) : p.G == 1 ? 1 : p.G == 2 || D == 80 || D == 96 ? 2 : 4;
+  const bool small = narrow(cache_dtype);
   const long long T = std::max(1ll, (long long)p.c.M << p.c.shift);
   const long long units = units_of(p), steps = units * ((T + kShareRows - 1) / kShareRows);
   const long long places = *mfma ? paged_mfma_places(D) : 1536;
   p.shares = p.splits = 0;
-  // Shares pay where a place gets many steps, so that the lengths' differences and not the shares' beginnings
-  // cost: 43 steps a place (64 sequences of up to 8192, 8 heads of 128 over e4m3) 121 us against 128 in chunks,
-  // but 6 (32 of up to 2048, 12 heads of 64) 31.1 against 30.7 and 2.6 (16 of up to 16001, one head of 96) 23.6
-  // against 20.7.  One sequence's chunks are equal as they are.
-  if (*mfma && p.c.B > 1 && p.c.B <= kShareSeqs && steps >= 16 * places && steps < (1ll << 30)) {
+  // One workgroup for each unit needs no second launch: it pays until a unit's rows take longer than that (3 us and
+  // a memory round trip; a pass of 128 8-bit rows costs more), and where there are units enough for the chip,
+  // longer.  In one / in parts, us: 1 unit of 64 elements in bfloat16 over 500 rows 7.2 / 10.1, 700 7.7 / 10.1, 1000
+  // 9.7 / 10.2, 1500 11.7 / 10.2; 128 elements in e4m3, 4 heads, 300 rows 8.2 / 9.8, 500 10.6 / 9.9; 256 such
+  // units of 1000 18.1 / 23.9, of up to 4000 45.8 / 40.1; 512 of 2000 44.9 / 54.4, of up to 4000 67.7 / 69.1, of
+  // up to 8000 130 / 121.
+  const bool one = T <= (units >= 512 ? 4096 : units >= 256 ? 1024 : small ? 384 : 768);
+  // Shares pay where a place gets many steps and the units' rows differ: 64 sequences of up to 8000, 8 heads of 64 in
+  // bfloat16 110 us against 121 in chunks (equal ones 164 against 162), 8 of 128 in e4m3 121 against 123.  Not
+  // over wide rows of 16 bits, whose registers they spill (the same of 128 in bfloat16, 8 heads each: 242 against
+  // 239, equal ones 359 against 321).  One sequence's chunks are equal as they are.
+  if (*mfma && !one && p.c.B > 1 && p.c.B <= kShareSeqs && paged_mfma_shares(cache_dtype, D) && steps >= 16 * places &&
+      steps < (1ll << 30)) {
     p.shares = (int)places;
     return places + units;
   }
   // Rows of a chunk, a power of two: about as many workgroups as places on the chip, not so short that a
-  // workgroup's beginning and end outweigh its rows.  Measured at 256 / 512 / 1024 / 2048 rows: one sequence of
-  // 131072, 8 heads of 64: 47.7 / 46.3 / 46.0 / 46.2 us (1024 taken); 32 of up to 2048, 12 heads of 64: 30.4 /
-  // 30.5 / 32.1 / 33.4 (512); 16 of up to 16001, one head of 96: 21.0 / 20.1 / 19.8 / 23.6 (256); 5 of up to
-  // 5001, 3 heads of 80 over int8: 13.6 / 16.4 / 22.2 / 35 (256; 13.2 at 128).
-  long long chunk = *mfma ? 256 : 128;
-  while (chunk < 4096 && chunk * 3 * places < T * units * 2) chunk *= 2;
+  // workgroup's beginning and end outweigh its rows.  Measured at 128 / 256 / 512 / 1024 / 2048 rows: one sequence
+  // of 131072, 8 heads of 64: 50.5 / 47.7 / 46.3 / 46.0 / 46.2 us (1024 taken); 32 of up to 2048, 12 heads of
+  // 64: - / 30.4 / 30.5 / 32.1 / 33.4 (512); 16 of up to 16001, one head of 96: 24.7 / 21.0 / 20.1 / 19.8 / 23.6
+  // (256); 5 of up to 5001, 3 heads of 80 over int8: 13.2 / 13.6 / 16.4 / 22.2 / 35 (128).
+  long long chunk = 128;
+  while (chunk < (one ? T : 4096) && (one || chunk * 3 * places < T * units * 2)) chunk *= 2;
   while ((T + chunk - 1) / chunk > 65535) chunk *= 2;  // (the grid's limit)
   p.splits = (int)((T + chunk - 1) / chunk);
   p.chunk = (int)chunk;

@@ -617,12 +617,14 @@ __global__ __launch_bounds__(kBlock, places(D)) void paged_mfma_kernel(PagedDeco
 
 template <int QT, int CT, int D>
 void launch(const PagedDecode& p, hipStream_t st) {
-  if (p.shares) {
-    hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, true>), dim3((unsigned)p.shares), dim3(kBlock), 0, st, p);
-  } else {
-    const unsigned units = (unsigned)(p.c.B * p.c.Hkv * ((p.G + kMfmaHeads - 1) / kMfmaHeads));
-    hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, false>), dim3(units, (unsigned)p.splits), dim3(kBlock), 0, st, p);
+  if constexpr (paged_mfma_shares(CT, D)) {
+    if (p.shares) {
+      hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, true>), dim3((unsigned)p.shares), dim3(kBlock), 0, st, p);
+      return;
+    }
   }
+  const unsigned units = (unsigned)(p.c.B * p.c.Hkv * ((p.G + kMfmaHeads - 1) / kMfmaHeads));
+  hipLaunchKernelGGL((paged_mfma_kernel<QT, CT, D, false>), dim3(units, (unsigned)p.splits), dim3(kBlock), 0, st, p);
 }
 
 template <int QT, int CT>

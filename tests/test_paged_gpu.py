@@ -371,6 +371,30 @@ def test_step_long_sequences(gpu_device, dtype, kv, G, D):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D", [32, 64, 80, 96, 128])
+@pytest.mark.parametrize("dtype,kv,G", [(F32, None, 1), (BF, None, 3), (F16, None, 17), (BF, E4, 8), (F16, I8, 5), (F32, E4, 4),
+                                        (F32, I8, 2)])
+def test_step_joins(gpu_device, dtype, kv, G, D):
+    """Sequences of one part to a dozen, whose last parts have a row or are full."""
+    pos = [1500, 127, 128, 129, 640, 383, 0, -1, 896]
+    c = Cache(gpu_device, len(pos), 2, D, 32, 48, dtype, kv, [p + 1 for p in pos])
+    junk(c, [p + 1 for p in pos])
+    for fresh in (True, False):
+        _step(c, pos, G, fresh)
+
+
+@pytest.mark.parametrize("B,H,dtype,kv,D,G", [(64, 4, BF, None, 64, 2), (32, 16, BF, E4, 128, 4), (47, 11, F32, None, 32, 1),
+                                              (26, 20, F16, I8, 80, 5)])
+def test_step_many_units(gpu_device, B, H, dtype, kv, D, G):
+    """Heads and sequences enough that a workgroup takes all rows of one."""
+    g = torch.Generator().manual_seed(B)
+    pos = (torch.rand(B, generator=g) ** 2 * 1023).long().tolist()
+    pos[0], pos[1], pos[2], pos[3] = 1023, -1, 0, 1024
+    c = Cache(gpu_device, B, H, D, 64, 16, dtype, kv, [min(p, 1023) + 1 for p in pos])
+    junk(c, [p + 1 for p in pos])
+    _step(c, pos, G)
+
+
 class RaggedCache(Cache):
     """A pool of just the pages that the lengths need, under a table for sequences of up to M pages."""
 
