@@ -65,11 +65,15 @@ void check(int status, const char* what) {
     raise(api.library_error, c10::str(what, " failed: status ", status, " (", api.status_string(status), ")"));
 }
 
-// Python's spelling of a shape, for the assertion messages.
-std::string shape_str(c10::IntArrayRef s) {
-  std::string r = "(";
-  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
-  return r + (s.size() == 1 ? ",)" : ")");
+// Python's spelling of a shape, for the assertion messages (spelled only when one is raised: six of them took 0.8 us of a call).
+struct ShapeStr {
+  c10::IntArrayRef s;
+};
+ShapeStr shape_str(c10::IntArrayRef s) { return {s}; }
+std::ostream& operator<<(std::ostream& o, const ShapeStr& x) {
+  o << "(";
+  for (size_t i = 0; i < x.s.size(); ++i) o << (i ? ", " : "") << x.s[i];
+  return o << (x.s.size() == 1 ? ",)" : ")");
 }
 
 c10::Device require_gpu(std::initializer_list<const Tensor*> ts) {
@@ -850,7 +854,7 @@ struct Paged {
             "] tensor, got ", shape_str(t.sizes()));
     if (t.device() != dev)
       raise(PyExc_RuntimeError, c10::str("tensors on different devices: ", dev, " and ", t.device()));
-    return t.to(at::kLong).contiguous();
+    return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous();
   }
 };
 

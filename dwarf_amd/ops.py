@@ -456,7 +456,10 @@ def traced(*tensors) -> bool:
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 \
             or torch._C._get_tracing_state() is not None:
         return True
-    return any(isinstance(t, FakeTensor) or t.device.type == "meta" for t in tensors)
+    for t in tensors:
+        if t.is_meta or isinstance(t, FakeTensor):
+            return True
+    return False
 
 
 # ------------------------------------------------------------------------------------------
