@@ -470,13 +470,18 @@ long long plan(PagedDecode& p, int dtype, int cache_dtype, int D, bool* mfma) {
   const long long units = units_of(p), steps = units * ((T + kShareRows - 1) / kShareRows);
   const long long places = *mfma ? paged_mfma_places(D) : 1536;
   p.shares = p.splits = 0;
-  // One workgroup for each unit needs no second launch: it pays until a unit's rows take longer than that (3 us and
-  // a memory round trip; a pass of 128 8-bit rows costs more), and where there are units enough for the chip,
-  // longer.  In one / in parts, us: 1 unit of 64 elements in bfloat16 over 500 rows 7.2 / 10.1, 700 7.7 / 10.1, 1000
-  // 9.7 / 10.2, 1500 11.7 / 10.2; 128 elements in e4m3, 4 heads, 300 rows 8.2 / 9.8, 500 10.6 / 9.9; 256 such
-  // units of 1000 18.1 / 23.9, of up to 4000 45.8 / 40.1; 512 of 2000 44.9 / 54.4, of up to 4000 67.7 / 69.1, of
-  // up to 8000 130 / 121.
-  const bool one = T <= (units >= 512 ? 4096 : units >= 256 ? 1024 : small ? 384 : 768);
+  // One workgroup for each unit needs no second launch: it pays until a unit's rows take longer than that and, where
+  // units fill the chip, longer.  In one / in parts, us, 1 unit: 64 elements in bfloat16 over 384 rows 6.2 / 8.2, 512
+  // 6.9 / 8.2, 768 8.3 / 8.2; 4 heads of 128 in e4m3 over 256 8.1 / 9.8, 384 9.3 / 9.8, 512 10.5 / 9.9; 64 in float32
+  // over 512 6.9 / 8.2, 768 8.6 / 8.1; 4 heads of 128 in float32 over 256 12.0 / 11.5, 384 15.7 / 11.5.  Many: 256 of 4
+  // heads of 128 in e4m3 over 1000 18.1 / 23.9, up to 4000 45.8 / 40.1; 512 of them over 2000 44.9 / 54.4, up to 4000
+  // 67.7 / 69.1, up to 8000 130 / 121; 512 of 64 in float32 over up to 4000 121 / 126, in int8 under float32 queries
+  // over up to 2000 31 / 28, up to 4000 58 / 48.
+  const long long most = units >= 512 ? (*mfma || !small ? 4096 : 2048)
+                         : units >= 256 ? 1024
+                         : *mfma        ? (small || D > 64 ? 384 : 512)
+                                        : std::min(512, 512 * 64 / (p.heads * D));
+  const bool one = T <= most;
   // Shares pay where a place gets many steps and the units' rows differ: 64 sequences of up to 8000, 8 heads of 64 in
   // bfloat16 110 us against 121 in chunks (equal ones 164 against 162), 8 of 128 in e4m3 121 against 123.  Not
   // over wide rows of 16 bits, whose registers they spill (the same of 128 in bfloat16, 8 heads each: 242 against
