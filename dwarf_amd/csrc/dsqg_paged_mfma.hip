@@ -14,7 +14,7 @@
 // rows' scales multiply scores and weights in fp32.
 //
 // Roundings: the weights enter the second product as two 16-bit terms, w = hi + lo + O(2^-16 w) in bf16 and
-// 2^-21 w in float16, down to its subnormal step (weights are taken times 2^14 there, so that this is 2^-38
+// 2^-21 w in float16, down to two of its subnormal steps (weights are taken times 2^14 there, so that this is 2^-37
 // of the largest); float16 queries against 8-bit keys are two bf16 terms, which hold them exactly.  Scores,
 // statistics and sums are fp32.
 //
@@ -78,9 +78,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo
 }
 
 // Eight weights (none negative) as two 16-bit terms, hi rounded down and lo what remains, so that neither is
-// negative.  Where values may be infinite (INF: not in 8 bits) lo of a weight above zero is above zero too, the
-// type's smallest number (2^-126, 2^-24) where nothing remains: an infinity times both terms is that infinity,
-// but times zero NaN.
+// negative.  Where values may be infinite (INF: not in 8 bits) both terms of a weight above zero are above zero,
+// for an infinity times both is that infinity, but times zero NaN.  In bf16 hi is, and lo is 2^-126 at least; in
+// float16, whose smallest number is 2^-24, both are that at least (so that a weight is up to 2^-23 too large).
 template <bool F16, bool INF>
 __device__ __forceinline__ void split_weights(const float (&w)[8], uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
@@ -88,10 +88,10 @@ __device__ __forceinline__ void split_weights(const float (&w)[8], uint4& hi, ui
   for (int i = 0; i < 4; ++i) {
     const float a = w[2 * i], b = w[2 * i + 1];
     if constexpr (F16) {
-      h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+      const float s = fminf(a * 0x1p126f, 0x1p-24f), t = fminf(b * 0x1p126f, 0x1p-24f);  // 0 for 0
+      h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a + s, b + t));
       const f16x2_t q = __builtin_bit_cast(f16x2_t, h[i]);
-      l[i] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)fmaxf(a - (float)q[0], fminf(a, 0x1p-24f)),
-                                                  (_Float16)fmaxf(b - (float)q[1], fminf(b, 0x1p-24f))});
+      l[i] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)fmaxf(a - (float)q[0], s), (_Float16)fmaxf(b - (float)q[1], t)});
     } else {
       h[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // the upper halves
       float x = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), y = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);

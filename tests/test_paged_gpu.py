@@ -854,3 +854,25 @@ def test_prefill_records_no_gradient_in_the_cache(gpu_device):
     assert y.requires_grad and not cache.k_pages.requires_grad
     y.sum().backward()
     assert x.grad is not None
+
+
+# ---- Infinite values of little weight. ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("drop", [5.0, 20.0, 26.0, 30.0, 60.0])
+@pytest.mark.parametrize("dtype,G", [(F16, 1), (F16, 4), (F16, 16), (BF, 1), (BF, 8), (F32, 1), (F32, 4)])
+def test_step_infinite_values_of_little_weight(gpu_device, dtype, G, drop):
+    """An infinity in a row whose score lies far below the largest is that infinity (times a weight above zero),
+    and the other columns are what they are without it."""
+    n, D = 150, 64
+    c = Cache(gpu_device, 1, 1, D, 16, 10, dtype)
+    at = int(c.table[0, 70 // 16]), 0, 70 % 16
+    c.k.zero_()
+    c.k[at] = -drop / 8  # times 64 ones and a scale of 1/8: a score of -drop
+    q = torch.ones(1, G, D, device=gpu_device, dtype=dtype)
+    pos = torch.tensor([n - 1], device=gpu_device)
+    plain = paged_decode_step(q, None, None, c.k, c.v, c.table, pos)
+    c.v[at][7], c.v[at][40] = math.inf, -math.inf
+    out = paged_decode_step(q, None, None, c.k, c.v, c.table, pos)
+    assert (out[:, :, 7] == math.inf).all() and (out[:, :, 40] == -math.inf).all()
+    rest = [d for d in range(D) if d not in (7, 40)]
+    same(out[:, :, rest], plain[:, :, rest])
