@@ -320,8 +320,10 @@ __device__ __forceinline__ void store_out(char* out, long long e, float x) {
 }
 
 // 2^(a - b), where b is the larger: 0 for a = -inf also where b is, NaN for a NaN (which the maxima that
-// b comes from pass over, so that the sums carry it).
+// b comes from pass over, so that the sums carry it).  a is a score as its maximum was taken of it, rounded: the
+// exact product in one multiply-add with b would leave that rounding as an exponent, past 2^26 one without bounds.
 __device__ __forceinline__ float weight(float a, float b) {
+#pragma clang fp contract(off)
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
 }
 
@@ -330,6 +332,13 @@ __device__ __forceinline__ float weight(float a, float b) {
 // weights are larger instead, so that small ones stay clear of its subnormal numbers.
 template <bool F16>
 constexpr float weight_lift() { return F16 ? 14.f : -30.f; }
+
+// What a row of the largest score m is weighed against (no multiply-add either).
+template <bool F16>
+__device__ __forceinline__ float lifted(float m) {
+#pragma clang fp contract(off)
+  return m - weight_lift<F16>();
+}
 
 // Largest group of query heads that one workgroup of the matrix-instruction kernel takes.
 constexpr int kMfmaHeads = 16;

@@ -63,7 +63,6 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
   using R = RowMap<D>;
   constexpr int PC = R::pieces, ES = elem_size(CT);
   constexpr int U = CT == DSQG_F32 || PC > 1 ? 2 : 4;  // passes of a tile
-  constexpr float kLift = weight_lift<false>();
   constexpr int TR = U * R::rows, stride = kWaves * TR;
   const int hg = (p.G + GT - 1) / GT;
   const int b = blockIdx.x / (p.c.Hkv * hg), rest = blockIdx.x - b * p.c.Hkv * hg;
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
       d = group_sum<R::lanes>(d) * (p.scale * sk);
       if (!ok) d = __uint_as_float(0x7fc00000u);  // nowhere to keep the row
       if (r == 0) {
-        s.m[g] = fmaxf(d, -INFINITY) - kLift;
+        s.m[g] = lifted<false>(fmaxf(d, -INFINITY));
         s.l[g] = weight(d, s.m[g]);
 #pragma unroll
         for (int u = 0; u < PC; ++u) {
@@ -285,7 +284,7 @@ __global__ __launch_bounds__(kBlock) void paged_decode_kernel(PagedDecode p) {
       float m = sc[g][0];
 #pragma unroll
       for (int u = 1; u < U; ++u) m = fmaxf(m, sc[g][u]);
-      m = fmaxf(s.m[g], m - kLift);
+      m = fmaxf(s.m[g], lifted<false>(m));
       const float a = weight(s.m[g], m);
       s.m[g] = m;
       s.l[g] *= a;

@@ -143,7 +143,6 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
   constexpr bool F16 = CT == DSQG_F16;                       // operands in float16 (else bf16)
   constexpr bool QLO = QT == DSQG_F16 && narrow(CT);         // queries in two terms
   constexpr int ES = elem_size(CT), KS = S::count, DB = D / 16, RV = Geo<D>::RV;
-  constexpr float kLift = weight_lift<F16>();
 
   const int b = part.b, hk = part.hk, g0 = part.g0;
   // (Opaque, so that what follows from it is worked out for each part and not held in registers across them.)
@@ -303,20 +302,15 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
   if (first < t1) load(0);
   __builtin_amdgcn_sched_barrier(0);
 
-  // Scores are taken times |scale|, so that their maximum may be found before it: a negative scale's sign
-  // goes to the queries.
-  const float scale = fabsf(p.scale);
-  const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
   uint4 qh[KS], ql[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const Raw8<QT> r = {make_uint4(qraw[s].a.x ^ sign, qraw[s].a.y ^ sign, qraw[s].a.z ^ sign, qraw[s].a.w ^ sign)};
     if constexpr (QLO) {
       float x[8];
-      raw_floats<QT>(r, x);
+      raw_floats<QT>(qraw[s], x);
       split8(x, qh[s], ql[s]);
     } else {
-      qh[s] = r.a;
+      qh[s] = qraw[s].a;
     }
   }
 
@@ -390,9 +384,9 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
       x = scores(kc)[0];
       if constexpr (narrow(CT)) x *= scale_value(byte);
     }
-    x = __shfl(x, i, 64) * scale;  // (row 0 is in the lanes of g = 0)
+    x = __shfl(x, i, 64) * p.scale;  // (row 0 is in the lanes of g = 0)
     if (!ok) x = nan;
-    m = fmaxf(x, -INFINITY) - kLift;
+    m = lifted<F16>(fmaxf(x, -INFINITY));
     const float e = weight(x, m);
     lsum = g == 0 ? e : 0.f;
     // Values in the result's layout: four elements at 16 d + 4 g.
@@ -450,7 +444,7 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
     float x[8], w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = e < 4 ? s0[e % 4] : s1[e % 4];
+      x[e] = (e < 4 ? s0[e % 4] : s1[e % 4]) * p.scale;
       if constexpr (narrow(CT)) x[e] = __builtin_amdgcn_ldexpf(x[e], (int)((ek[e / 4] >> (8 * (e % 4))) & 255) - 127);
     }
     // (255 - byte is zero nowhere, by the usual test of a word's bytes, unless a row reads as NaN.)
@@ -470,7 +464,7 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
     float mx = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-    mx = fmaf(col_max(mx), scale, -kLift);
+    mx = lifted<F16>(col_max(mx));
     if (__any(mx > m)) {
       const float mn = fmaxf(m, mx), a = weight(m, mn);
       m = mn;
@@ -478,9 +472,8 @@ __device__ __forceinline__ void attend_part(const PagedDecode& p, Part part, bf1
 #pragma unroll
       for (int d = 0; d < DB; ++d) o[d] *= a;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(x[e], scale, -ref));
+    for (int e = 0; e < 8; ++e) w[e] = weight(x[e], m);
     if (live < kTile) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = 16 * (e / 4) + 4 * g + e % 4 < live ? w[e] : 0.f;

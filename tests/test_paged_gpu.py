@@ -876,3 +876,28 @@ def test_step_infinite_values_of_little_weight(gpu_device, dtype, G, drop):
     assert (out[:, :, 7] == math.inf).all() and (out[:, :, 40] == -math.inf).all()
     rest = [d for d in range(D) if d not in (7, 40)]
     same(out[:, :, rest], plain[:, :, rest])
+
+
+# ---- Large scores. --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("fresh", [False, True])
+@pytest.mark.parametrize("dtype,kv", [(F16, None), (BF, None), (F32, None), (BF, E4), (BF, I8), (F16, E4), (F16, I8), (F32, I8)])
+def test_step_large_scores(gpu_device, dtype, kv, fresh, G):
+    """Scores far past 2^24, where a rounding is larger than any softmax's range: the largest one's row has all
+    the weight, be it a stored one or the new one."""
+    n, D = 150, 64
+    for c0 in (3e2, 1e3, 3e3, 1.7e4, 4e4) + ((3e5, 1e6, 7e7, 1e10, 1e15) if dtype != F16 else ()):
+        for at in (3, 70, n - 1):
+            c = PagedKVCache(1, 1, D, 160, dtype, gpu_device, kv_dtype=kv, page_size=16)
+            k = torch.full((1, 1, n, D), -c0, device=gpu_device)
+            k[:, :, at] = c0
+            v = torch.randn(1, 1, n, D, generator=torch.Generator().manual_seed(at)).to(gpu_device, dtype)
+            k, q = k.to(dtype), torch.full((1, G, D), c0, device=gpu_device).to(dtype)
+            c.prefill(k[:, :, :n - fresh], v[:, :, :n - fresh])
+            out = c.step(q, k[:, :, -1], v[:, :, -1]) if fresh else \
+                paged_decode_step(q, None, None, c.k_pages, c.v_pages, c.page_table, c.pos - 1, k_scale=c.k_scale, v_scale=c.v_scale)
+            want = c.read(dtype=F32)[1][0, 0, at].expand(G, D)
+            # One row's value, its weight in two 16-bit terms at worst (2^-16), then rounded to the type.
+            err = (out[0].float() - want).abs()
+            assert (err <= want.abs() * (2.0 ** -16 + torch.finfo(dtype).eps / 2)).all(), (c0, at)
