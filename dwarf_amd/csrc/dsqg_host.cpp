@@ -139,13 +139,14 @@ void fill_shape(dsqg_shape& s, at::ScalarType dt, int64_t B, int64_t H, int64_t 
 
 void* ptr(const Tensor& t) { return !t.defined() || t.numel() == 0 ? nullptr : t.data_ptr(); }
 
-// t if the kernels can read it in place (unit inner stride, 16-byte aligned rows), else a copy.
+// t if the kernels can read it in place (unit inner stride, 16-byte aligned rows), else a copy (a clone: what
+// counts as contiguous may start at any address, and have any stride in a dimension of one entry).
 Tensor rows_ready(const Tensor& t) {
   if (t.numel() == 0) return t;
   const int64_t es = t.element_size(), d = t.dim();
   bool ok = t.stride(d - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; ok && i < d - 1; ++i) ok = t.stride(i) >= 0 && (t.stride(i) * es) % 16 == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // fp32, contiguous and 16-byte aligned (the kernels read scale_embed as 16-byte pieces).

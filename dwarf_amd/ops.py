@@ -51,11 +51,12 @@ def _require_gpu(*ts: Optional[Tensor]) -> torch.device:
 
 
 def _rows_ready(t: Tensor) -> Tensor:
-    """Keep t if the kernels can read it in place (unit inner stride, 16-byte aligned rows)."""
+    """Keep t if the kernels can read it in place (unit inner stride, 16-byte aligned rows), else a clone: what
+    counts as contiguous may start at any address, and have any stride in a dimension of one entry."""
     es = t.element_size()
     ok = (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
           and all(s >= 0 and (s * es) % 16 == 0 for s in t.stride()[:-1]))
-    return t if ok or t.numel() == 0 else t.contiguous()
+    return t if ok or t.numel() == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _param(t: Optional[Tensor]) -> Optional[Tensor]:

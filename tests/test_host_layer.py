@@ -196,3 +196,45 @@ def test_absent_output_gradient_is_zero(gpu_device, call):
                                            kv_inject=tuple(deltas) if call == "inject" else None)
     for g in torch.autograd.grad(_NoGrad.apply(out).sum(), leaves, allow_unused=True):
         assert g is None or not g.any()
+
+
+def _odd(t):
+    """t, contiguous, 8 bytes past a 16-byte boundary."""
+    at = 8 // t.element_size()
+    out = torch.empty(t.numel() + at, dtype=t.dtype, device=t.device)[at:].view(t.shape).copy_(t.detach())
+    assert out.is_contiguous() and out.data_ptr() % 16 == 8
+    return out.requires_grad_(t.requires_grad)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("path", ["eager", "op"])
+def test_contiguous_operands_at_an_odd_address(gpu_device, path, dtype):
+    """Rows off the kernels' alignment, in tensors that count as contiguous: aligned copies' results."""
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(B, H, N, D, generator=g).to(gpu_device, dtype).requires_grad_() for _ in range(3))
+    pb = torch.randn(len(OFFSETS_V3), H, generator=g).to(gpu_device)
+    x, gate = (torch.randn(B, N, 64, generator=g).to(gpu_device, dtype).requires_grad_() for _ in range(2))
+    attend = dwarf_amd.dsqg_attention if path == "eager" else \
+        lambda q, k, v, p: ops.dsqg_fwd(q, k, v, p, None, None, None, list(OFFSETS_V3))[0]
+    pool = dwarf_amd.causal_mean_pool_gate if path == "eager" else ops.pool_gate_fwd
+    res = []
+    for put in (lambda t: t, _odd):
+        heads, rows = [put(t) for t in (q, k, v)], [put(t) for t in (x, gate)]
+        res.append([*_grads(lambda *t: attend(*t, pb), heads, lambda o: put(torch.ones_like(o).contiguous())),
+                    *_grads(pool, rows, lambda o: put(torch.ones_like(o)))])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_one_head_projection_with_an_odd_row(gpu_device):
+    """One head over one sequence: the head views count as contiguous whatever the idle strides are."""
+    g = torch.Generator().manual_seed(3)
+    t = torch.randn(1, 1, 3 * D + 7, generator=g).to(gpu_device, torch.bfloat16)[..., :3 * D]
+    pb = torch.randn(len(OFFSETS_V3), 1, generator=g).to(gpu_device)
+    res = []
+    for qkv in (t.clone().requires_grad_(), t.requires_grad_()):
+        res.append(_grads(lambda x: dwarf_amd.dsqg_attention_qkv(x, 1, pb), [qkv], torch.ones_like))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)

@@ -901,3 +901,39 @@ def test_step_large_scores(gpu_device, dtype, kv, fresh, G):
             # One row's value, its weight in two 16-bit terms at worst (2^-16), then rounded to the type.
             err = (out[0].float() - want).abs()
             assert (err <= want.abs() * (2.0 ** -16 + torch.finfo(dtype).eps / 2)).all(), (c0, at)
+
+
+# ---- Operands that count as contiguous. --------------------------------------------
+
+def _odd_base(t, by=4):
+    """t at an address that is no multiple of 16 bytes, contiguous as it was."""
+    flat = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)
+    out = flat[by if t.element_size() == 2 else by // 2:][:t.numel()].view(t.shape)
+    assert out.is_contiguous() and out.data_ptr() % 16
+    return out.copy_(t)
+
+
+def _odd_ones(t):
+    """t with a stride of 3 elements in its dimensions of one entry (which count for nothing)."""
+    strides = [3 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    out = torch.empty(t.numel() + 64, dtype=t.dtype, device=t.device).as_strided(t.shape, strides)
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("form", [_odd_base, _odd_ones])
+@pytest.mark.parametrize("B,H,N", [(1, 12, 5), (2, 12, 5), (1, 3, 1), (2, 1, 5), (2, 3, 1), (1, 1, 1)])
+@pytest.mark.parametrize("dtype,kv", [(BF, None), (F32, None), (F16, I8)])
+def test_operands_that_count_as_contiguous(gpu_device, dtype, kv, B, H, N, form):
+    """Rows whose base or whose idle strides are odd: the results of aligned copies."""
+    g = torch.Generator().manual_seed(8)
+    rows = [torch.randn(B, H, N, 64, generator=g).to(gpu_device, dtype) for _ in range(2)]
+    step = [torch.randn(B, h, 64, generator=g).to(gpu_device, dtype) for h in (2 * H, H, H)]
+    pos = torch.tensor([9, 30][:B], device=gpu_device)
+    res = []
+    for put in (lambda t: t, form):
+        c = Cache(gpu_device, B, H, 64, 16, 3, dtype, kv)
+        paged_kv_write(*(put(t) for t in rows), c.k, c.v, c.table, pos, **c.state)
+        out = paged_decode_step(*(put(t) for t in step), c.k, c.v, c.table, pos + N, **c.state)
+        res.append([out, c.k, c.v, *(s for s in (c.k_scale, c.v_scale) if s is not None)])
+    for a, b in zip(*res):
+        same(a, b)
