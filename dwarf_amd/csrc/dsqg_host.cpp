@@ -824,7 +824,7 @@ struct Paged {
     const int64_t es = k.element_size();
     for (const Tensor* t : {&k, &v}) {
       bool ok = t->numel() == 0 || (t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0);
-      for (int i = 0; ok && t->numel() && i < 3; ++i) ok = t->stride(i) * es % 16 == 0;
+      for (int i = 0; ok && t->numel() && i < 3; ++i) ok = t->size(i) == 1 || t->stride(i) * es % 16 == 0;
       require(ok, "pages must have unit inner stride and 16-byte aligned rows");
     }
     table = table0.stride(1) == 1 || table0.size(1) <= 1 ? table0 : table0.contiguous();

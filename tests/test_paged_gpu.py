@@ -937,3 +937,29 @@ def test_operands_that_count_as_contiguous(gpu_device, dtype, kv, B, H, N, form)
         res.append([out, c.k, c.v, *(s for s in (c.k_scale, c.v_scale) if s is not None)])
     for a, b in zip(*res):
         same(a, b)
+
+
+def _odd_pool(t):
+    u = t.view(torch.uint8) if t.element_size() == 1 else t
+    strides = [3 if n == 1 else s for n, s in zip(u.shape, u.stride())]
+    return u.clone().as_strided(u.shape, strides).view(t.dtype)
+
+
+@pytest.mark.parametrize("P,H", [(1, 2), (5, 1), (1, 1)])
+@pytest.mark.parametrize("kv", [None, E4])
+def test_pools_with_idle_strides(gpu_device, kv, P, H):
+    """A pool of one page or one head may have any stride there."""
+    g = torch.Generator().manual_seed(8)
+    row = [torch.randn(1, h, 32, generator=g).to(gpu_device, BF) for h in (3 * H, H, H)]
+    pos = torch.tensor([7], device=gpu_device)
+    res = []
+    for put in (lambda t: t, _odd_pool):
+        c = Cache(gpu_device, 1, H, 32, 16, 1, BF, kv, spare=P - 1)
+        c.k, c.v = put(c.k), put(c.v)
+        if kv is not None:
+            c.k_scale, c.v_scale = put(c.k_scale), put(c.v_scale)
+        out = paged_decode_step(*row, c.k, c.v, c.table, pos, **c.state)
+        paged_kv_write(row[1][:, :, None], row[2][:, :, None], c.k, c.v, c.table, pos + 1, **c.state)
+        res.append([out, *paged_kv_read(c.k, c.v, c.table, pos + 2, 16, **c.state)])
+    for a, b in zip(*res):
+        same(a, b)
