@@ -787,10 +787,12 @@ Tensor linear(const Tensor& x0, const Tensor& w0, const OptTensor& b0) {
 
 // A cache's tensors, checked, and their argument block (for tensors of the type dt on the caller's side).
 // The pools are taken as they are (they are written in place); the small tensors are kept alive here.
+// Shapes and types come first, the caller's too, and devices last (place): every refusal can be had without a GPU.
 struct Paged {
   dsqg_paged_cache a = {};
   c10::Device dev{c10::kCPU};
   Tensor table;
+  const Tensor* tensors[5] = {};  // pools, table and scales (the caller's)
 
   Paged(const Tensor& k, const Tensor& v, const Tensor& table0, const OptTensor& ks0, const OptTensor& vs0, at::ScalarType dt,
         bool written) {
@@ -810,8 +812,6 @@ struct Paged {
       if (s)
         require(s->sizes() == c10::IntArrayRef({P, H, page}) && s->scalar_type() == at::kFloat8_e8m0fnu,
                 "scales must be float8_e8m0fnu ", shape_str({P, H, page}), " tensors, got ", shape_str(s->sizes()));
-    dev = require_gpu({&k, &v, &table0});
-    if (narrow) dev = require_gpu({&k, &*ks0, &*vs0});
     const bool inference = c10::InferenceMode::is_enabled();
     for (const Tensor* t : {&k, &v, narrow ? &*ks0 : nullptr, narrow ? &*vs0 : nullptr}) {
       if (!t) continue;
@@ -847,6 +847,15 @@ struct Paged {
     }
     a.page_table = static_cast<const int32_t*>(ptr(table));
     a.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
+    const Tensor* all[5] = {&k, &v, &table0, narrow ? &*ks0 : nullptr, narrow ? &*vs0 : nullptr};
+    std::copy(std::begin(all), std::end(all), tensors);
+  }
+
+  // The device that the cache's tensors and the caller's are on.
+  void place(std::initializer_list<const Tensor*> rows) {
+    dev = require_gpu({tensors[0], tensors[1], tensors[2]});
+    if (tensors[3]) require_gpu({tensors[0], tensors[3], tensors[4]});
+    for (const Tensor* t : rows) require_gpu({tensors[0], t});
   }
 
   // [B] positions or counts as the kernels read them.
@@ -886,7 +895,7 @@ void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Ten
   require(ks.has_value() || kp.scalar_type() == dt, "rows of ", dt, " do not go into pages of ", kp.scalar_type());
   require(k0.size(0) == c.a.B && k0.size(1) == c.a.Hkv && k0.size(3) == c.a.D, "k and v must be [", c.a.B, ",", c.a.Hkv, ",N,", c.a.D,
           "], got ", shape_str(k0.sizes()));
-  require_gpu({&kp, &k0, &v0});
+  c.place({&k0, &v0});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor k = plain_rows(k0), v = plain_rows(v0), pos = c.index(pos0, "pos");
   const Tensor counts = counts0 ? c.index(*counts0, "counts") : Tensor();
@@ -909,6 +918,7 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor& kp, const Tensor& vp, const 
   refuse_grad({&kp, &vp});
   Paged c(kp, vp, table, ks, vs, dt, false);
   require(T >= 0 && T < (1ll << 31), "max_len must be from 0 to 2^31 - 1, got ", T);
+  c.place({});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor lengths = c.index(lengths0, "lengths");
   const auto o = kp.options().dtype(dt);
@@ -939,7 +949,7 @@ Tensor paged_decode(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, 
     if (t->defined())
       require(t->sizes() == c10::IntArrayRef({B, Hkv, D}) && t->scalar_type() == dt, "k_new and v_new must be ", dt, " ",
               shape_str({B, Hkv, D}), " tensors, got ", t->scalar_type(), " ", shape_str(t->sizes()));
-  require_gpu({&kp, &q0, &kn, &vn});
+  c.place({&q0, &kn, &vn});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor q = plain_rows(q0), pos = c.index(pos0, "pos");
   const Tensor out = at::empty({B, H, D}, q0.options());

@@ -298,3 +298,31 @@ def test_ctypes_layout_matches_c(tmp_path):
     for s in probes.values():
         want += [ctypes.sizeof(s)] + [getattr(s, f).offset for f, _ in s._fields_]
     assert got == want
+
+
+# ---- Refusals by their own message, whatever the device. ------------------------------------------------------------
+
+@pytest.mark.parametrize("name,bad,match", [(n, b, m) for n, b, m in BAD for n in (["write", "step", "read"] if n == "any" else [n])])
+def test_refuses_bad_arguments_by_name(name, bad, match):
+    """Shapes and types are looked at before the device, so each check is the one that refuses."""
+    fn, args = _calls()[name]
+    with pytest.raises(AssertionError, match=match):
+        fn(**{**args, **bad})
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(k=z(2, 2, 3, 64), v=z(2, 2, 3, 64)), "k and v must be"), (dict(k=z(2, 4, 3, 32), v=z(2, 4, 3, 32)), "k and v must be"),
+    (dict(k=z(3, 2, 3, 32), v=z(3, 2, 3, 32)), "k and v must be"), (dict(k=z(2, 2, 32), v=z(2, 2, 32)), "same shape")])
+def test_write_refuses_rows_of_another_cache(bad, match):
+    fn, args = _calls()["write"]
+    with pytest.raises(AssertionError, match=match):
+        fn(**{**args, **bad})
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(q=z(3, 2, 32)), "q must be"), (dict(q=z(2, 2)), "q must be"), (dict(k_new=z(2, 1, 32), v_new=z(2, 1, 32)), "k_new and v_new"),
+    (dict(k_new=z(1, 2, 32)), "k_new and v_new"), (dict(v_new=z(2, 2, 64)), "k_new and v_new"), (dict(v_new=None), "go together")])
+def test_step_refuses_rows_of_another_cache(bad, match):
+    fn, args = _calls()["step"]
+    with pytest.raises(AssertionError, match=match):
+        fn(**{**args, **bad})
