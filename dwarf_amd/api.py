@@ -344,7 +344,10 @@ class PagedKVCache:
 
     def _write(self, k: Tensor, v: Tensor, pos: Tensor, counts: Optional[Tensor]) -> Optional[Tensor]:
         if counts is not None:
-            counts = counts.clamp(0, k.shape[2])
+            assert not (counts.is_floating_point() or counts.is_complex() or counts.dtype == torch.bool), \
+                f"counts must be integers, got {counts.dtype}"
+            # (As int64: a narrow type may not hold the number of rows that they are limited to.)
+            counts = counts.long().clamp(0, k.shape[2])
         paged_kv_write(k.detach().to(self.dtype), v.detach().to(self.dtype), self.k_pages, self.v_pages,
                        self.page_table, pos, counts=counts, **self._state())
         return counts

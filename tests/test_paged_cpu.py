@@ -326,3 +326,24 @@ def test_step_refuses_rows_of_another_cache(bad, match):
     fn, args = _calls()["step"]
     with pytest.raises(AssertionError, match=match):
         fn(**{**args, **bad})
+
+
+# ---- Counts of narrow types. -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+@pytest.mark.parametrize("name", ["prefill", "write"])
+def test_cache_takes_counts_of_any_integer_type(name, dtype):
+    """A prompt of more rows than the counts' type can say (the call goes on until it finds no GPU)."""
+    c = PagedKVCache(2, 1, 32, 70000, device="cpu")
+    rows = torch.zeros(2, 1, 1, 32, dtype=BF).expand(2, 1, 70000, 32)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        getattr(c, name)(rows, rows, torch.tensor([100, 7], dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bool])
+@pytest.mark.parametrize("name", ["prefill", "write"])
+def test_cache_refuses_counts_that_are_no_integers(name, dtype):
+    c = PagedKVCache(2, 1, 32, 100, device="cpu")
+    rows = torch.zeros(2, 1, 5, 32, dtype=BF)
+    with pytest.raises(AssertionError, match="counts must be"):
+        getattr(c, name)(rows, rows, torch.ones(2, dtype=dtype))
