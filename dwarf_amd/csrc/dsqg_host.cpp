@@ -895,6 +895,7 @@ void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Ten
   require(ks.has_value() || kp.scalar_type() == dt, "rows of ", dt, " do not go into pages of ", kp.scalar_type());
   require(k0.size(0) == c.a.B && k0.size(1) == c.a.Hkv && k0.size(3) == c.a.D, "k and v must be [", c.a.B, ",", c.a.Hkv, ",N,", c.a.D,
           "], got ", shape_str(k0.sizes()));
+  require(k0.size(2) * std::max(c.a.Hkv, 1) < (1ll << 31), "k and v must have less than 2^31 rows a sequence (H * N), got ", k0.size(2));
   c.place({&k0, &v0});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor k = plain_rows(k0), v = plain_rows(v0), pos = c.index(pos0, "pos");
@@ -902,7 +903,6 @@ void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Ten
   dsqg_paged_write_args a = {};
   a.cache = c.a;
   a.N = (int32_t)k.size(2);
-  require(k.size(2) < (1ll << 31), "k and v have too many rows: ", k.size(2));
   a.k = ptr(k); a.v = ptr(v);
   for (int i = 0; i < 3; ++i) { a.k_stride[i] = k.stride(i); a.v_stride[i] = v.stride(i); }
   a.pos = static_cast<const int64_t*>(ptr(pos));
@@ -917,7 +917,7 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor& kp, const Tensor& vp, const 
   py::gil_scoped_release nogil;
   refuse_grad({&kp, &vp});
   Paged c(kp, vp, table, ks, vs, dt, false);
-  require(T >= 0 && T < (1ll << 31), "max_len must be from 0 to 2^31 - 1, got ", T);
+  require(T >= 0 && T < (1ll << 31) && T * std::max(c.a.Hkv, 1) < (1ll << 31), "max_len must be from 0 to less than 2^31 rows (H * max_len), got ", T);
   c.place({});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor lengths = c.index(lengths0, "lengths");

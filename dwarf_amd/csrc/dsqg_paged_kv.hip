@@ -8,6 +8,8 @@
 // 8 x 2048 positions, 12 heads of 64, from bfloat16 into e4m3 (76 MB): 16.2 us, 4.7 TB/s, a copy's rate;
 // 16 x 4096 positions (63 % of them in use), 8 heads of 128, from int8 to float16 (354 MB): 59 us, 6.0 TB/s;
 // 2 x 65536, 8 heads of 128, from e4m3 to bfloat16 (807 MB): 147 us, 5.5 TB/s.
+#include <algorithm>
+
 #include "dsqg_launch.hpp"
 #include "dsqg_mfma.hpp"
 #include "dsqg_paged.hpp"
@@ -67,8 +69,9 @@ int check_paged_cache(const dsqg_paged_cache& a, PagedCache* c) {
 
 namespace {
 
-// Rows of one sequence that a grid takes: sixteen lanes a row, 2^32 lanes in x.
-constexpr long long kMostRows = 1ll << 27;
+// Rows of one sequence that a grid takes (sixteen lanes a row, below 2^32 lanes in x); more are several launches,
+// up to a limit that outputs cannot reach (2^31 rows are 274 GB at least).
+constexpr long long kGridRows = 1ll << 27, kMostRows = 1ll << 31;
 
 struct WriteParams {
   PagedCache c;
@@ -77,6 +80,7 @@ struct WriteParams {
   const long long* pos; const long long* counts;
   int N;
   long long rows;  // Hkv * N of one sequence
+  long long row0;  // the launch's first
 };
 
 struct ReadParams {
@@ -86,6 +90,7 @@ struct ReadParams {
   int T;
   bool stream;     // the output is larger than the caches that the next launch could find it in
   long long rows;  // Hkv * T of one sequence
+  long long row0;  // the launch's first
 };
 
 // A row of the caller's type DT as the pool keeps it.
@@ -119,7 +124,7 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteParams p) {
   using R = RowMap<D>;
   constexpr int rpb = kBlock / R::lanes;
   const int b = blockIdx.y, g = threadIdx.x % R::lanes;
-  const long long row = (long long)blockIdx.x * rpb + threadIdx.x / R::lanes;
+  const long long row = p.row0 + (long long)blockIdx.x * rpb + threadIdx.x / R::lanes;
   if (row >= p.rows) return;
   const int h = (int)(row / p.N), n = (int)(row - (long long)h * p.N);
   if (p.counts && n >= p.counts[b]) return;
@@ -169,7 +174,7 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(ReadParams p) {
   using R = RowMap<D>;
   constexpr int rpb = kBlock / R::lanes;
   const int b = blockIdx.y, g = threadIdx.x % R::lanes;
-  const long long row = (long long)blockIdx.x * rpb + threadIdx.x / R::lanes;
+  const long long row = p.row0 + (long long)blockIdx.x * rpb + threadIdx.x / R::lanes;
   if (row >= p.rows) return;
   const int h = (int)(row / p.T), t = (int)(row - (long long)h * p.T);
   const long long out = ((long long)b * p.rows + row) * D * elem_size(OT);
@@ -214,19 +219,29 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(ReadParams p) {
     }
 }
 
-template <int DT, int CT, int D>
-void launch_write(const WriteParams& p, hipStream_t st) {
+// The rows in launches of what a grid takes: f(its grid), p.row0 being its first row.
+template <int D, typename P, typename F>
+void for_grids(P p, F&& f) {
   constexpr int rpb = kBlock / RowMap<D>::lanes;
-  hipLaunchKernelGGL((paged_write_kernel<DT, CT, D>), dim3((unsigned)((p.rows + rpb - 1) / rpb), (unsigned)p.c.B),
-                     dim3(kBlock), 0, st, p);
+  for (; p.row0 < p.rows; p.row0 += kGridRows) {
+    const long long n = std::min(p.rows - p.row0, kGridRows);
+    f(p, dim3((unsigned)((n + rpb - 1) / rpb), (unsigned)p.c.B));
+  }
+}
+
+template <int DT, int CT, int D>
+void launch_write(const WriteParams& a, hipStream_t st) {
+  for_grids<D>(a, [&](const WriteParams& p, dim3 grid) {
+    hipLaunchKernelGGL((paged_write_kernel<DT, CT, D>), grid, dim3(kBlock), 0, st, p);
+  });
 }
 
 template <int CT, int OT, int D>
-void launch_read(const ReadParams& p, hipStream_t st) {
-  constexpr int rpb = kBlock / RowMap<D>::lanes;
-  const dim3 grid((unsigned)((p.rows + rpb - 1) / rpb), (unsigned)p.c.B);
-  if (p.stream) hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, true>), grid, dim3(kBlock), 0, st, p);
-  else hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, false>), grid, dim3(kBlock), 0, st, p);
+void launch_read(const ReadParams& a, hipStream_t st) {
+  for_grids<D>(a, [&](const ReadParams& p, dim3 grid) {
+    if (p.stream) hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, true>), grid, dim3(kBlock), 0, st, p);
+    else hipLaunchKernelGGL((paged_read_kernel<CT, OT, D, false>), grid, dim3(kBlock), 0, st, p);
+  });
 }
 
 template <int DT, int D>
@@ -320,10 +335,10 @@ extern "C" int dsqg_paged_read(const dsqg_paged_read_args* a, dsqg_stream_t stre
   p.v = static_cast<char*>(a->v);
   p.T = a->T;
   p.rows = (long long)c.Hkv * a->T;
+  if (p.rows >= kMostRows) return DSQG_EUNSUPPORTED;
   // Results that the eight L2s (32 MB) cannot hold push the pool's lines out of them for nothing: 537 MB of them
   // leave in 147 us, 156 the ordinary way.  Smaller ones are left where the next launch finds them.
   p.stream = 2ll * c.B * p.rows * c.D * elem_size(c.dtype) > (32ll << 20);
-  if (p.rows >= kMostRows) return DSQG_EUNSUPPORTED;
   for_dim<ReadDim>(c.D, p, c.dtype, c.cache_dtype, reinterpret_cast<hipStream_t>(stream));
   return hipGetLastError() == hipSuccess ? DSQG_OK : DSQG_EHIP;
 }

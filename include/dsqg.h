@@ -338,8 +338,9 @@ int dsqg_linear_wgrad(const dsqg_linear_wgrad_args* args, dsqg_stream_t stream);
  * page is a power of two from 16 to 65536, M * page at most 2^30; D is one of dsqg_supported_head_dims
  * (EUNSUPPORTED otherwise).  Pools have unit inner stride, other strides {page, head, row} in elements and
  * bases that keep every row 16-byte aligned, and rows that do not overlap; the scales' strides are
- * {page, head, row} as well.  B and Hkv are at most 65535.  (dsqg_paged_decode: the page strides, and a
- * page's rows times the row stride, are less than 2^31 bytes, and B * H less than 2^21.) */
+ * {page, head, row} as well.  B and Hkv are at most 65535.  (dsqg_paged_write and dsqg_paged_read: Hkv * N and
+ * Hkv * T are less than 2^31.  dsqg_paged_decode: the page strides, and a page's rows times the row stride, are
+ * less than 2^31 bytes, and B * H less than 2^21.) */
 typedef struct {
     int32_t dtype;             /* DSQG_F32, DSQG_BF16 or DSQG_F16 */
     int32_t cache_dtype;       /* that, DSQG_E4M3 or DSQG_INT8 */

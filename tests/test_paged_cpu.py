@@ -347,3 +347,20 @@ def test_cache_refuses_counts_that_are_no_integers(name, dtype):
     rows = torch.zeros(2, 1, 5, 32, dtype=BF)
     with pytest.raises(AssertionError, match="counts must be"):
         getattr(c, name)(rows, rows, torch.ones(2, dtype=dtype))
+
+
+# ---- Calls of very many rows. ----------------------------------------------------------------------------------------
+
+def test_refuses_more_rows_than_memory_has():
+    fn, args = _calls()["read"]
+    for bad in (-1, 2 ** 30, 2 ** 31, 2 ** 62):
+        with pytest.raises(AssertionError, match="max_len must be"):
+            fn(**{**args, "max_len": bad})
+    fn, args = _calls()["write"]
+    rows = z(1, 1, 1, 32).expand(2, 2, 2 ** 30, 32)
+    with pytest.raises(AssertionError, match="less than 2\\^31 rows"):
+        fn(**{**args, "k": rows, "v": rows})
+    for name, field in (("dsqg_paged_write", "N"), ("dsqg_paged_read", "T")):
+        a = _abi()[name]
+        setattr(a, field, 2 ** 31 // 3 + 1)
+        assert _call(name, a) == _lib.DSQG_EUNSUPPORTED

@@ -963,3 +963,39 @@ def test_pools_with_idle_strides(gpu_device, kv, P, H):
         res.append([out, *paged_kv_read(c.k, c.v, c.table, pos + 2, 16, **c.state)])
     for a, b in zip(*res):
         same(a, b)
+
+
+# ---- Calls of more rows than one grid has. ------------------------------------------------------------------------
+
+def test_read_of_more_rows_than_a_grid(gpu_device):
+    """2^27 rows of a sequence and a few: pages come round again and again, so that every row is known."""
+    H, D, page = 8, 32, 65536
+    T = 2 ** 24 + 70000
+    M = -(-T // page)
+    g = torch.Generator(gpu_device).manual_seed(1)
+    k, v = (torch.randn(3, H, page, D, device=gpu_device, dtype=BF, generator=g) for _ in range(2))
+    table = (torch.arange(M, device=gpu_device) % 3).to(torch.int32)[None]
+    n = T - 300
+    got = paged_kv_read(k, v, table, torch.tensor([n], device=gpu_device), T)
+    for x, pool in zip(got, (k, v)):
+        assert x.shape == (1, H, T, D)
+        for j in range(M):
+            live = min(page, n - j * page)
+            if live > 0:
+                assert torch.equal(x[0, :, j * page:j * page + live], pool[j % 3, :, :live]), j
+        assert not x[0, :, n:].any()
+
+
+def test_write_of_more_rows_than_a_grid(gpu_device):
+    """The last rows of the last head lie behind the 2^27th; those in front of the sequence are left out."""
+    H, D, N = 8, 32, 2 ** 24 + 5
+    g = torch.Generator(gpu_device).manual_seed(1)
+    k = torch.randn(1, H, N, D, device=gpu_device, dtype=BF, generator=g)
+    v = k.flip(-1)
+    kp, vp = (torch.zeros(2, H, 64, D, device=gpu_device, dtype=BF) for _ in range(2))
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=gpu_device)
+    paged_kv_write(k, v, kp, vp, table, torch.tensor([100 - N], device=gpu_device))
+    for pool, x in ((kp, k), (vp, v)):
+        same(pool[1], x[0, :, N - 100:N - 36])
+        same(pool[0, :, :36], x[0, :, N - 36:])
+        assert not pool[0, :, 36:].any()
