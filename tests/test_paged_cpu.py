@@ -364,3 +364,47 @@ def test_refuses_more_rows_than_memory_has():
         a = _abi()[name]
         setattr(a, field, 2 ** 31 // 3 + 1)
         assert _call(name, a) == _lib.DSQG_EUNSUPPORTED
+
+
+# ---- How a step is split. --------------------------------------------------------------------------------------------
+
+CODE = {torch.float32: 0, BF: 1, torch.float16: 2, E4: 3, I8: 4}
+
+
+def split_of(dtype, kv, B, Hkv, H, D, page, M):
+    """("one", 0), ("chunks", their number) or ("shares", their number): a step's split, from the size of its
+    workspace (each part has D + 2 floats a head, each unit two integers)."""
+    c = _lib.PagedCache()
+    c.dtype, c.cache_dtype, c.B, c.Hkv, c.D, c.P, c.page, c.M = CODE[dtype], CODE[kv or dtype], B, Hkv, D, 64, page, M
+    c.k_pages = c.v_pages = 0x10000
+    c.k_stride = c.v_stride = (Hkv * page * D, page * D, D)
+    if kv is not None:
+        c.k_scale = c.v_scale = 0x20000
+        c.k_scale_stride = c.v_scale_stride = (Hkv * page, page, 1)
+    c.page_table, c.table_stride = 0x30000, M
+    a, n = _lib.PagedDecodeArgs(cache=c, H=H), ctypes.c_size_t(0)
+    assert _lib.load().dsqg_paged_decode_workspace_size(ctypes.byref(a), ctypes.byref(n)) == 0
+    if n.value == 0:
+        return "one", 0
+    G = H // Hkv
+    heads = min(G, 16) if dtype != torch.float32 else 1 if G == 1 else 2 if G == 2 or D in (80, 96) else 4
+    units = B * Hkv * -(-G // heads)
+    parts, rest = divmod(n.value - units * 8, heads * (D + 2) * 4)
+    assert rest == 0
+    places = 256 * (4 if D <= 64 else 3)
+    if parts == places + units:
+        return "shares", places
+    assert parts % units == 0
+    return "chunks", parts // units
+
+
+@pytest.mark.parametrize("want,B,Hkv,G,D,dtype,kv,page,M", [
+    ("one", 1, 8, 1, 32, BF, None, 64, 2), ("one", 512, 1, 1, 64, BF, None, 64, 64), ("chunks", 1, 8, 1, 64, BF, None, 64, 2048),
+    ("chunks", 4, 8, 1, 32, torch.float32, None, 64, 32), ("chunks", 5, 3, 5, 80, torch.float16, I8, 64, 80),
+    ("shares", 64, 8, 4, 128, BF, E4, 128, 64), ("shares", 64, 8, 4, 128, torch.float16, I8, 128, 64),
+    ("shares", 64, 8, 1, 64, BF, None, 64, 125), ("chunks", 64, 8, 4, 128, BF, None, 128, 64),
+    ("chunks", 64, 8, 1, 64, torch.float32, None, 64, 125)])
+def test_split(want, B, Hkv, G, D, dtype, kv, page, M):
+    """One workgroup a unit under short tables, chunks under long ones, equal shares of large batches, but not of
+    16-bit rows of 128 and not of float32."""
+    assert split_of(dtype, kv, B, Hkv, Hkv * G, D, page, M)[0] == want

@@ -999,3 +999,26 @@ def test_write_of_more_rows_than_a_grid(gpu_device):
         same(pool[1], x[0, :, N - 100:N - 36])
         same(pool[0, :, :36], x[0, :, N - 36:])
         assert not pool[0, :, 36:].any()
+
+
+# ---- Equal shares of wide rows. -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,H,G,most", [(12, 4, 3, 12000), (64, 16, 1, 260), (3, 8, 16, 30000)])
+@pytest.mark.parametrize("dtype,kv", [(BF, E4), (BF, I8), (F16, E4), (F16, I8)])
+def test_step_shares_of_wide_rows(gpu_device, dtype, kv, B, H, G, most):
+    """128 elements in 8 bits: units of several shares, shares of several units, sequences without rows."""
+    from test_paged_cpu import split_of
+    g = torch.Generator().manual_seed(B)
+    pos = (torch.rand(B, generator=g) ** 2 * most).long().tolist()
+    pos[0], pos[1], pos[2] = most, -1, 128
+    if B > 3:
+        pos[-1], pos[-2] = 255, 256
+    M = 16 * 768 * 128 // (B * H * 32) * 2 + 1024
+    c = RaggedCache(gpu_device, H, 128, 32, M, dtype, kv, [p + 1 for p in pos])
+    assert split_of(dtype, kv, B, H, H * G, 128, 32, M)[0] == "shares"
+    junk(c, [p + 1 for p in pos])
+    if B > 3:
+        pos[3] = M * 32 + 5  # past the table
+    for fresh in (True, False):
+        a = _step(c, pos, G, fresh)
+    same(_step(c, pos, G, False), a)
