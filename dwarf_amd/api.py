@@ -243,7 +243,9 @@ def paged_decode_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
     softmax_scale defaults to D ** -0.5.  With k_new = v_new = None nothing is written and position
     pos[b] is attended as the pages hold it.  A sequence with pos[b] < 0 attends nothing and gets zeros;
     one that attends a position without a page gets NaN.  Sums are fp32 and the result does not change
-    from call to call.  The step has no gradient.
+    from call to call.  Values below 2^-90 (8-bit rows: whose largest is below 2^-70) lose bits or vanish, a
+    row of less than 2^-96 of the heaviest one's weight weighs nothing (an infinite value there gives NaN), and
+    queries over 8-bit pages must be below 2^112.  The step has no gradient.
     """
     if ops.traced(q, k_pages, v_pages):
         return ops.paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale)

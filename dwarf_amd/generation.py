@@ -126,7 +126,8 @@ class FullAttentionBlock(nn.Module):
 
     def new_cache(self, batch: int, max_len: int, device=None, dtype=None, paged: bool = False,
                   kv_dtype: Optional[torch.dtype] = None) -> KVCache:
-        """A flat cache, or (``paged``, or any ``kv_dtype``) a PagedKVCache of that page type."""
+        """A flat cache, or (``paged``, or any ``kv_dtype``) a PagedKVCache of that page type, which takes
+        the kernels' head dims only (32, 64, 80, 96 and 128)."""
         w = self.attn.qkv_proj.weight
         if paged or kv_dtype is not None:
             return PagedKVCache(batch, self.attn.num_heads, self.attn.head_dim, max_len, dtype or w.dtype,
@@ -202,7 +203,8 @@ class CondMTransformer(nn.Module):
     def new_cache(self, batch: int, paged: bool = False,
                   kv_dtype: Optional[torch.dtype] = None) -> "GenerationCache":
         """Per-block caches (DSQG rings and pool sums, the full-attention K/V rows; ``paged`` and
-        ``kv_dtype`` as FullAttentionBlock.new_cache takes them) and the position of the next token."""
+        ``kv_dtype`` as FullAttentionBlock.new_cache takes them, head dims included) and the position of the
+        next token."""
         caches = [b.new_cache(batch, self.seq_len, paged=paged, kv_dtype=kv_dtype)
                   if isinstance(b, FullAttentionBlock) else b.new_cache(batch) for b in self.blocks]
         dev = self.embedding.weight.device
@@ -245,7 +247,7 @@ class CondMTransformer(nn.Module):
 
         After the prefill, the first step runs eagerly and the next ones replay it from a HIP
         graph (``use_graph``); sampling stays outside the graph.  ``paged`` and ``kv_dtype`` choose the
-        full-attention layer's cache (``new_cache``).
+        full-attention layer's cache (``new_cache``; a paged one refuses head dims without kernels).
         """
         was_training = self.training
         self.eval()

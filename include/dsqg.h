@@ -391,6 +391,10 @@ int dsqg_paged_read(const dsqg_paged_read_args* args, dsqg_stream_t stream);
  * of the rows as the cache holds them.  With k_new = v_new = NULL nothing is written and position pos[b]
  * is attended as it is.  A sequence with pos[b] < 0 attends nothing: its output is zeros and nothing is
  * written.  Sums and softmax statistics are fp32, in an order that does not change between calls.
+ * Weights are kept relative to the largest, so the range is smaller than the types': values below 2^-90, and rows
+ * of 8 bits whose largest is below 2^-70, lose bits or vanish; a row that weighs less than 2^-96 of the heaviest
+ * (2^-140 in float16 pages) weighs nothing, and gives NaN where its value is infinite.  Queries over 8-bit pages
+ * are below 2^112, so that their products with the codes are finite.
  * No two sequences may have the same page at the position that a step writes.
  * The workspace (256-byte aligned) holds the parts of sequences that are split over workgroups. */
 typedef struct {

@@ -1022,3 +1022,26 @@ def test_step_shares_of_wide_rows(gpu_device, dtype, kv, B, H, G, most):
     for fresh in (True, False):
         a = _step(c, pos, G, fresh)
     same(_step(c, pos, G, False), a)
+
+
+# ---- The range of values that the step keeps. -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("dtype,kv,e", [(BF, None, -90), (F32, None, -90), (BF, E4, -70), (BF, I8, -70), (F32, E4, -70), (F32, I8, -70),
+                                        (BF, None, 126), (F32, None, 126), (BF, E4, 126), (F32, I8, 126)])
+def test_step_small_and_large_values(gpu_device, dtype, kv, e, G):
+    """Values near the ends of the stated range, under weights of all sizes, within the bound that holds elsewhere."""
+    n, D = 700, 64
+    g = torch.Generator().manual_seed(2)
+    c = PagedKVCache(2, 2, D, n, dtype, gpu_device, kv_dtype=kv, page_size=16)
+    k, v = (torch.randn(2, 2, n, D, generator=g) for _ in range(2))
+    # Rows whose largest magnitude is from 2^e to 2^(e + 1).
+    v = v / v.abs().amax(-1, keepdim=True) * 2.0 ** e * (1 + torch.rand(2, 2, n, 1, generator=g))
+    k, v = k.to(gpu_device, dtype), v.to(gpu_device, dtype)
+    c.prefill(k, v)
+    q = (torch.randn(2, 2 * G, D, generator=g) * 2).to(gpu_device, dtype)
+    out = paged_decode_step(q, None, None, c.k_pages, c.v_pages, c.page_table, c.pos - 1, k_scale=c.k_scale, v_scale=c.v_scale)
+    rk, rv = c.read(dtype=F32)
+    for b in range(2):
+        ref, mass, size = po.attend(q[b].cpu(), rk[b].cpu().double(), rv[b].cpu().double(), D ** -0.5)
+        assert ((out[b].double().cpu() - ref).abs() <= po.bound(ref, mass, size, D, n, dtype)).all()
