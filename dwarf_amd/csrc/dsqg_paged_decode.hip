@@ -6,13 +6,16 @@
 // One pass over the rows with a running maximum and sum: of the rows seen so far a group of lanes keeps
 // m = max s_t, l = sum 2^(s_t - m) and acc = sum 2^(s_t - m) v_t (scores in base 2), and the parts of
 // different rows join as  acc = sum_i 2^(m_i - m) acc_i.  (m carries an offset, weight_lift: the largest weight
-// is not 1.)  Every key and value is read once, so memory bounds the step, and short ones the launches and the
-// round trips from the position to the rows.
+// is not 1.)  Every key and value is read once for each group of up to 1, 2 or 4 query heads that share it
+// (plan's p.heads), so memory bounds the step, and short ones the launches and the round trips from the position to
+// the rows; the groups of one key/value head are neighbouring workgroups, which lie on different XCDs.
 //
 // 16-bit queries take the matrix instructions (dsqg_paged_mfma.hip, with the figures of long steps).  The kernel
-// here takes float32 ones, whose products those instructions would round, and 8-bit pools whose scales they
-// cannot read four at a time.  4 float32 sequences of up to 2048 positions, 8 heads of 32 (10 MB): 5.2 us and
-// 3.8 for the join; a launch alone is about 3 of each.
+// here takes float32 ones, whose products the 16-bit instructions would round (those of float32 operands would
+// not, but have sixteen columns for what is one head in the float32 steps that are listed; with many heads they
+// would read the pages once where this kernel reads them for each group: not built), and 8-bit pools whose scales
+// the other kernel cannot read four at a time.  4 float32 sequences of up to 2048 positions, 8 heads of 32 (10 MB):
+// 5.2 us and 3.7 for the join; a launch alone is about 3 of each.
 //
 // Its workgroup has one key/value head of one sequence, up to GT of the query heads that share it, and a
 // chunk of the sequence's rows; its four waves take tiles in turn.  In a tile a row is 4, 8 or 16
@@ -462,13 +465,20 @@ long long units_of(const PagedDecode& p) { return (long long)p.c.B * p.c.Hkv * (
 // to be joined.
 long long plan(PagedDecode& p, int dtype, int cache_dtype, int D, bool* mfma) {
   *mfma = dtype != DSQG_F32 && paged_mfma_takes(p, dtype, cache_dtype);
-  // Three groups of eight a lane leave registers for two heads of the vector kernel.
+  // Four heads of the vector kernel take 146 to 155 registers, three waves a SIMD; at D = 80 and 96, three groups
+  // of eight a lane, two heads take 178 to 212 over 8 bits (two waves) and all 256 over float32 (one wave).
   p.heads = *mfma ? std::min(p.G, kMfmaHeads) : p.G == 1 ? 1 : p.G == 2 || D == 80 || D == 96 ? 2 : 4;
   const bool small = narrow(cache_dtype);
   const long long T = std::max(1ll, (long long)p.c.M << p.c.shift);
   const long long units = units_of(p), steps = units * ((T + kShareRows - 1) / kShareRows);
+  // (The vector kernel's is a number of workgroups that chunks were found to be well cut for, six a CU; by registers
+  // a CU holds five of one head, four of two and three of four, at D = 80 and 96 four to one.)
   const long long places = *mfma ? paged_mfma_places(D) : 1536;
   p.shares = p.splits = 0;
+  // T is what the table holds, for the host knows no positions.  Under a table longer than its sequences the split is
+  // the table's: 8 heads of 32 at 77 positions 3.6 us (in a replayed graph) under a table of 128 or 512, 5.5 under
+  // 2048; 8 of 64 at 8000 10.4 under 8064, 13.1 under 131072; 16 x 8 x 4 of 128 at 4000 50.9 under 4032, 69.0 under
+  // 32768.
   // One workgroup for each unit needs no second launch: it pays until a unit's rows take longer than that and, where
   // units fill the chip, longer.  In one / in parts, us, 1 unit: 64 elements in bfloat16 over 384 rows 6.2 / 8.2, 512
   // 6.9 / 8.2, 768 8.3 / 8.2; 4 heads of 128 in e4m3 over 256 8.1 / 9.8, 384 9.3 / 9.8, 512 10.5 / 9.9; 64 in float32

@@ -5,9 +5,9 @@
 // elements of a key row and the same eight of the value row, a row being 4, 8 or 16 neighbouring lanes
 // (four lanes of three groups at D = 80 and 96), so that a wave's accesses are whole rows.  The largest
 // magnitude that a scale needs is a maximum over those lanes (DPP), without LDS or a second pass.
-// 8 x 2048 positions, 12 heads of 64, from bfloat16 into e4m3 (76 MB): 16.2 us, 4.7 TB/s, a copy's rate;
-// 16 x 4096 positions (63 % of them in use), 8 heads of 128, from int8 to float16 (354 MB): 59 us, 6.0 TB/s;
-// 2 x 65536, 8 heads of 128, from e4m3 to bfloat16 (807 MB): 147 us, 5.5 TB/s.
+// Medians: 8 x 2048 positions, 12 heads of 64, from bfloat16 into e4m3 (76 MB): 15.8 us, 4.8 TB/s, a copy's rate;
+// 16 x 4096 positions (63 % of them in use), 8 heads of 128, from int8 to float16 (354 MB): 60 us, 5.9 TB/s;
+// 2 x 65536, 8 heads of 128, from e4m3 to bfloat16 (807 MB): 162 us, 5.0 TB/s (147 at the least).
 #include <algorithm>
 
 #include "dsqg_launch.hpp"
@@ -337,7 +337,8 @@ extern "C" int dsqg_paged_read(const dsqg_paged_read_args* a, dsqg_stream_t stre
   p.rows = (long long)c.Hkv * a->T;
   if (p.rows >= kMostRows) return DSQG_EUNSUPPORTED;
   // Results that the eight L2s (32 MB) cannot hold push the pool's lines out of them for nothing: 537 MB of them
-  // leave in 147 us, 156 the ordinary way.  Smaller ones are left where the next launch finds them.
+  // leave in 161 to 163 us, 168 to 170 the ordinary way (medians of two runs each).  Smaller ones are left where
+  // the next launch finds them.
   p.stream = 2ll * c.B * p.rows * c.D * elem_size(c.dtype) > (32ll << 20);
   for_dim<ReadDim>(c.D, p, c.dtype, c.cache_dtype, reinterpret_cast<hipStream_t>(stream));
   return hipGetLastError() == hipSuccess ? DSQG_OK : DSQG_EHIP;
