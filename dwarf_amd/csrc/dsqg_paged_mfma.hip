@@ -23,12 +23,13 @@
 // up to 8192, 8 x 4 heads of 128 over e4m3 (680 MB): 116 to 125 us; 32 of up to 2048, 12 heads of 64 (127 MB): 27;
 // 16 of up to 16001, 1 x 8 heads of 96 (62 MB): 16.  The same kernel without its products takes the same time.
 // What the short ones lose is the launch (3 us), two memory round trips and the last workgroup's wait: 8 heads of
-// 32 over 77 positions take 3.5 us.  5 x 3 x 5 heads of 80 in float16 over int8, up to 5001 positions, take 9.3: 5.7
-// up to 16 positions, 7.1 in bfloat16 over bfloat16, the rest the conversions and the queries' second term.  Against the vector instructions (dsqg_paged_decode.hip), which need a
-// multiply-add for each head and element: four heads over e4m3 400 -> 132 us, eight of 96 94 -> 20, and also
-// one head of 64, 38 -> 30 (the same steps otherwise).  A tile of 32 rows a wave leaves registers for four waves a
-// SIMD (three above 64 elements), each with a tile in flight; eight and sixteen waves a workgroup, chunks placed
-// by XCD and keys through LDS in whole rows were no faster, or slower.
+// 32 over 77 positions take 3.5 us.  5 x 3 x 5 heads of 80 in float16 over int8, up to 5001 positions, take 9.3:
+// 5.7 up to 16 positions, 7.1 in bfloat16 over bfloat16, the rest the conversions and the queries' second term.
+// Against the vector instructions (dsqg_paged_decode.hip), which need a multiply-add for each head and element:
+// four heads over e4m3 400 -> 132 us, eight of 96 94 -> 20, and also one head of 64, 38 -> 30 (the same steps
+// otherwise).  A tile of 32 rows a wave leaves registers for four waves a SIMD (three above 64 elements), each with
+// a tile in flight; eight and sixteen waves a workgroup, chunks placed by XCD and keys through LDS in whole rows
+// were no faster, or slower.
 #include <type_traits>
 
 #include "dsqg_launch.hpp"

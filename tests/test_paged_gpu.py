@@ -1045,3 +1045,14 @@ def test_step_small_and_large_values(gpu_device, dtype, kv, e, G):
     for b in range(2):
         ref, mass, size = po.attend(q[b].cpu(), rk[b].cpu().double(), rv[b].cpu().double(), D ** -0.5)
         assert ((out[b].double().cpu() - ref).abs() <= po.bound(ref, mass, size, D, n, dtype)).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
+@pytest.mark.parametrize("dtype,kv,G", [(BF, None, 1), (F16, None, 4), (BF, E4, 4), (F16, I8, 3), (F32, I8, 2)])
+def test_step_softmax_scale_of_narrow_types(gpu_device, dtype, kv, G, scale):
+    """A flat softmax, a sharp one and a reversed one, with and without a new row, in one part and in several."""
+    for pos, M in (([300, 45], 5), ([3000, 129], 60)):
+        for fresh in (True, False):
+            c = Cache(gpu_device, 2, 2, 64, 64, M, dtype, kv, [p + 1 for p in pos])
+            junk(c, [p + 1 for p in pos])
+            _step(c, pos, G, fresh, scale=scale)
