@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DSQG_HIP_LIB", PKG_DIR / "libdsqg_hip.so"))
 
 MAX_OFFSETS = 64
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DSQG_OK, DSQG_EINVAL, DSQG_EUNSUPPORTED, DSQG_EHIP, DSQG_EWORKSPACE = 0, 1, 2, 3, 4
 DSQG_ETOOLARGE = 5
@@ -134,7 +134,7 @@ class PagedCache(ctypes.Structure):
 class PagedWriteArgs(ctypes.Structure):
     _fields_ = [("cache", PagedCache), ("N", ctypes.c_int32),
                 ("k", _vp), ("k_stride", _i64x3), ("v", _vp), ("v_stride", _i64x3),
-                ("pos", _vp), ("counts", _vp)]
+                ("pos", _vp), ("counts", _vp), ("rows", _vp), ("src_rows", ctypes.c_int32)]
 
 
 class PagedReadArgs(ctypes.Structure):
@@ -146,6 +146,24 @@ class PagedDecodeArgs(ctypes.Structure):
                 ("q", _vp), ("q_stride", _i64x2), ("k_new", _vp), ("k_new_stride", _i64x2),
                 ("v_new", _vp), ("v_new_stride", _i64x2), ("pos", _vp), ("out", _vp),
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+MAX_TREE = 64  # DSQG_MAX_TREE
+
+
+class TreeAcceptArgs(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32),
+                ("tokens", _vp), ("tokens_stride", ctypes.c_int64), ("parents", _vp), ("parents_stride", ctypes.c_int64),
+                ("picks", _vp), ("picks_stride", ctypes.c_int64), ("counts", _vp),
+                ("path", _vp), ("n", _vp), ("next", _vp)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32), ("u_is_double", ctypes.c_int32),
+                ("logits", _vp), ("logits_stride", ctypes.c_int64), ("u", _vp),
+                ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double),
+                ("top_k", ctypes.c_int64), ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp),
+                ("tokens", _vp), ("logprobs", _vp)]
 
 
 # Every symbol include/dsqg.h declares, with its ctypes signature.
@@ -179,6 +197,8 @@ SIGNATURES = {
     "dsqg_paged_decode_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs),
                                                         ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs), _vp]),
+    "dsqg_tree_accept": (ctypes.c_int, [ctypes.POINTER(TreeAcceptArgs), _vp]),
+    "dsqg_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
 }
 
 _LIB = None

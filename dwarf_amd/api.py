@@ -16,6 +16,9 @@
 * ``paged_kv_write`` / ``paged_decode_step`` / ``paged_kv_read`` and ``PagedKVCache`` -- full attention
   over a paged key/value cache, of the rows' type or 8 bits wide (no counterpart in the reference,
   whose full-attention layer, train/train_2048_condU.py:210-245, keeps no cache).
+* ``draft_tree_accept`` -- which of the tokens drafted as a tree the model's picks keep.
+* ``sample_tokens`` -- the next token from logits and given random numbers: the sampling of
+  train/train_2048_condU.py:474-484 with top-k and min-p, in one kernel.
 
 The output [B,H,N,HD] is stored token-major ([B,N,H,HD] memory), so the callers'
 ``out.permute(0, 2, 1, 3).reshape(B, N, H * HD)`` (train/train_2048_condU.py:186) is a view.
@@ -28,7 +31,7 @@ Shape errors raise AssertionError, as the reference's asserts do (:363-365).
 
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Union
 
 import torch
 from torch import Tensor
@@ -198,10 +201,12 @@ def causal_mean_pool_gate(x: Tensor, gate_pre: Tensor) -> Tensor:
 
 
 def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor, *,
-                   counts: Optional[Tensor] = None, k_scale: Optional[Tensor] = None,
-                   v_scale: Optional[Tensor] = None) -> None:
+                   counts: Optional[Tensor] = None, rows: Optional[Tensor] = None,
+                   k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None) -> None:
     """Write row i of each sequence of k and v [B,Hkv,N,D] to position pos[b] + i of a paged cache, for
-    i < counts[b] (default: all N); every other row of the pages stays as it is.
+    i < counts[b] (default: all N); every other row of the pages stays as it is.  With rows [B,M], integers, row
+    rows[b,i] goes to position pos[b] + i instead, for i < M; a number that is no row of k and v writes nothing
+    (``draft_tree_accept`` returns such paths).
 
     k_pages, v_pages [P,Hkv,page,D] are pools of pages (page a power of two from 16) and page_table [B,M]
     int32 names the page that holds positions page * j .. page * (j + 1) - 1 of each sequence.  Rows are
@@ -214,8 +219,10 @@ def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_
     themselves, have no defined result.  No gradient passes through the cache.
     """
     if ops.traced(k, v, k_pages, v_pages):
+        if rows is not None:
+            return ops.paged_kv_write_rows(k, v, k_pages, v_pages, page_table, pos, counts, rows, k_scale, v_scale)
         return ops.paged_kv_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
-    return _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
+    return _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, rows, k_scale, v_scale)
 
 
 def paged_kv_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor,
@@ -251,6 +258,45 @@ def paged_decode_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
         return ops.paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale)
     return _lib.host().paged_decode(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale,
                                     softmax_scale)
+
+
+def draft_tree_accept(tokens: Tensor, parents: Tensor, picks: Tensor, counts: Optional[Tensor] = None):
+    """(path [B,T], n [B], next [B]), int64: which of the tokens drafted as a tree are kept.
+
+    Node i of sequence b has the token tokens[b,i] and hangs on the node parents[i] (or parents[b,i]); picks[b,i] is
+    what the model chose after it.  Node 0, the token that was certain before, is kept; from a node the walk goes to its
+    first child behind it whose token is the node's pick.  path lists the nodes on the way, -1 behind them, n counts
+    them, and next is the pick after the last: the next draft's node 0.  With counts, sequence b has counts[b] nodes (of
+    none: n 0 and next -1).  T is at most 64.  ``paged_kv_write(..., counts=n, rows=path)`` keeps their rows.
+    """
+    if ops.traced(tokens, parents, picks):
+        return ops.tree_accept(tokens, parents, picks, counts)
+    return _lib.host().tree_accept(tokens, parents, picks, counts)
+
+
+def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
+                  top_p: Union[float, Tensor] = 1.0, min_p: Union[float, Tensor] = 0.0, *,
+                  return_logprobs: bool = False):
+    """Tokens [...] (int64) drawn from logits [...,V] with one number u [...] from [0, 1) for each row; with
+    ``return_logprobs`` also the log probabilities (float32) that they were drawn with.
+
+    Weights are exp((x - max x) / temperature).  In the order of x, the largest first and of equal ones the lower
+    index, the tokens that stay are the first top_k, of those the ones before which at most top_p of their mass
+    lies (train/train_2048_condU.py:478-482), of those the ones of at least min_p of the largest weight; the drawn one
+    is the first, by index, whose running mass is above u times the mass that stays.  top_k = 0, top_p = 1 and min_p
+    = 0 limit nothing; temperature 0 takes the largest logit (the first of equal ones, log probability 0).  Each
+    setting is a number or a tensor of one for each row, where values past a limit's range mean its end (a
+    temperature that is not above 0 is 0) and a NaN no limit.  A NaN logit is no candidate, as -infinity is; a
+    row without candidates gives -1 and -infinity.  Masses are summed as whole numbers: the result depends on nothing but
+    the row.  Nothing here has a gradient.
+    """
+    def split(x, none):
+        return (none, x) if isinstance(x, Tensor) else (x, None)
+
+    (t, ts), (k, ks), (p, ps), (m, ms) = split(temperature, 1.0), split(top_k, 0), split(top_p, 1.0), split(min_p, 0.0)
+    fn = ops.sample_tokens if ops.traced(logits, u) else _lib.host().sample
+    tokens, logprobs = fn(logits, u, t, k, p, m, ts, ks, ps, ms, return_logprobs)
+    return (tokens, logprobs) if return_logprobs else tokens
 
 
 class DSQGRingCache:

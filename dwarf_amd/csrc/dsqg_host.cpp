@@ -44,6 +44,8 @@ struct Api {
   decltype(&dsqg_paged_read) paged_read = nullptr;
   decltype(&dsqg_paged_decode_workspace_size) paged_decode_workspace_size = nullptr;
   decltype(&dsqg_paged_decode) paged_decode = nullptr;
+  decltype(&dsqg_tree_accept) tree_accept = nullptr;
+  decltype(&dsqg_sample) sample = nullptr;
   PyObject* library_error = nullptr;  // dwarf_amd._lib.DSQGLibraryError
 } api;
 
@@ -884,7 +886,7 @@ void cache_changed(std::initializer_list<const Tensor*> ts) {
 Tensor plain_rows(const Tensor& t) { return rows_ready(t.is_neg() ? t.resolve_neg() : t); }
 
 void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& pos0,
-                 const OptTensor& counts0, const OptTensor& ks, const OptTensor& vs) {
+                 const OptTensor& counts0, const OptTensor& rows0, const OptTensor& ks, const OptTensor& vs) {
   py::gil_scoped_release nogil;
   refuse_grad({&k0, &v0, &kp, &vp});
   require(k0.dim() == 4 && v0.sizes() == k0.sizes(), "k and v must be [B,H,N,D] of the same shape, got ", shape_str(k0.sizes()),
@@ -896,13 +898,23 @@ void paged_write(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Ten
   require(k0.size(0) == c.a.B && k0.size(1) == c.a.Hkv && k0.size(3) == c.a.D, "k and v must be [", c.a.B, ",", c.a.Hkv, ",N,", c.a.D,
           "], got ", shape_str(k0.sizes()));
   require(k0.size(2) * std::max(c.a.Hkv, 1) < (1ll << 31), "k and v must have less than 2^31 rows a sequence (H * N), got ", k0.size(2));
+  if (rows0) {
+    require(at::isIntegralType(rows0->scalar_type(), false) && rows0->dim() == 2 && rows0->size(0) == c.a.B, "rows must be an integer [",
+            c.a.B, ",N] tensor, got ", rows0->scalar_type(), " ", shape_str(rows0->sizes()));
+    require(rows0->size(1) * std::max(c.a.Hkv, 1) < (1ll << 31), "rows must name less than 2^31 rows a sequence (H * N), got ",
+            rows0->size(1));
+  }
   c.place({&k0, &v0});
+  if (rows0) require_gpu({&kp, &*rows0});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor k = plain_rows(k0), v = plain_rows(v0), pos = c.index(pos0, "pos");
   const Tensor counts = counts0 ? c.index(*counts0, "counts") : Tensor();
+  const Tensor rows = rows0 ? rows0->to(at::kLong).contiguous() : Tensor();
   dsqg_paged_write_args a = {};
   a.cache = c.a;
-  a.N = (int32_t)k.size(2);
+  a.N = (int32_t)(rows0 ? rows.size(1) : k.size(2));
+  a.rows = static_cast<const int64_t*>(ptr(rows));
+  a.src_rows = (int32_t)k.size(2);
   a.k = ptr(k); a.v = ptr(v);
   for (int i = 0; i < 3; ++i) { a.k_stride[i] = k.stride(i); a.v_stride[i] = v.stride(i); }
   a.pos = static_cast<const int64_t*>(ptr(pos));
@@ -982,6 +994,117 @@ Tensor paged_decode(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, 
   return out;
 }
 
+// ---- Drafted tokens and sampling. ----------------------------------------------------------------------------------
+
+// Integers [B,T] as the kernels read them (unit inner stride), or of one row for all (stride 0): [T].
+Tensor node_table(const Tensor& t, at::ScalarType dt) {
+  const Tensor x = t.scalar_type() == dt ? t : t.to(dt);
+  return x.numel() == 0 || x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous();
+}
+
+// Shapes of a tree: parents [T] or [B,T], counts [B] or none.
+void check_tree(const Tensor& parents, const OptTensor& counts, int64_t B, int64_t T) {
+  require(at::isIntegralType(parents.scalar_type(), false) &&
+              (parents.sizes() == c10::IntArrayRef({T}) || parents.sizes() == c10::IntArrayRef({B, T})),
+          "parents must be integers ", shape_str({T}), " or ", shape_str({B, T}), ", got ", parents.scalar_type(), " ",
+          shape_str(parents.sizes()));
+  require(T >= 1 && T <= DSQG_MAX_TREE, "a tree has 1 to ", DSQG_MAX_TREE, " nodes, got ", T);
+  if (counts)
+    require(at::isIntegralType(counts->scalar_type(), false) && counts->sizes() == c10::IntArrayRef({B}), "counts must be an integer [", B,
+            "] tensor, got ", counts->scalar_type(), " ", shape_str(counts->sizes()));
+}
+
+std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& tokens0, const Tensor& parents0, const Tensor& picks0,
+                                               const OptTensor& counts0) {
+  py::gil_scoped_release nogil;
+  auto whole = [](const Tensor& t) { return at::isIntegralType(t.scalar_type(), false); };
+  require(tokens0.dim() == 2 && whole(tokens0), "tokens must be integers [B,T], got ", tokens0.scalar_type(), " ",
+          shape_str(tokens0.sizes()));
+  const int64_t B = tokens0.size(0), T = tokens0.size(1);
+  require(picks0.sizes() == tokens0.sizes() && whole(picks0), "picks must be integers ", shape_str(tokens0.sizes()), ", got ",
+          picks0.scalar_type(), " ", shape_str(picks0.sizes()));
+  check_tree(parents0, counts0, B, T);
+  require(B < (1ll << 31), "too many sequences: ", B);
+  const c10::Device dev = require_gpu({&tokens0, &parents0, &picks0});
+  if (counts0) require_gpu({&tokens0, &*counts0});
+  const c10::OptionalDeviceGuard guard(dev);
+  const Tensor tokens = node_table(tokens0, at::kLong), parents = node_table(parents0, at::kInt), picks = node_table(picks0, at::kLong);
+  const Tensor counts = counts0 ? counts0->to(at::kLong).contiguous() : Tensor();
+  const auto o = tokens.options().dtype(at::kLong);
+  const Tensor path = at::empty({B, T}, o), n = at::empty({B}, o), next = at::empty({B}, o);
+  dsqg_tree_accept_args a = {};
+  a.B = (int32_t)B; a.T = (int32_t)T;
+  auto stride = [](const Tensor& t) { return t.dim() == 2 && t.size(0) > 1 ? t.stride(0) : 0; };
+  a.tokens = static_cast<const int64_t*>(ptr(tokens)); a.tokens_stride = stride(tokens);
+  a.parents = static_cast<const int32_t*>(ptr(parents)); a.parents_stride = stride(parents);
+  a.picks = static_cast<const int64_t*>(ptr(picks)); a.picks_stride = stride(picks);
+  a.counts = static_cast<const int64_t*>(ptr(counts));
+  a.path = static_cast<int64_t*>(ptr(path)); a.n = static_cast<int64_t*>(ptr(n)); a.next = static_cast<int64_t*>(ptr(next));
+  check(api.tree_accept(&a, stream_of(dev)), "dsqg_tree_accept");
+  return {path, n, next};
+}
+
+std::tuple<Tensor, OptTensor> sample(const Tensor& logits0, const Tensor& u0, double temperature, int64_t top_k, double top_p, double min_p,
+                                     const OptTensor& temperatures0, const OptTensor& top_ks0, const OptTensor& top_ps0,
+                                     const OptTensor& min_ps0, bool logprobs) {
+  py::gil_scoped_release nogil;
+  const auto dt = logits0.scalar_type();
+  require(logits0.dim() >= 1, "logits must be [...,V], got ", shape_str(logits0.sizes()));
+  require(dt == at::kFloat || dt == at::kBFloat16 || dt == at::kHalf, "logits must be float32, bfloat16 or float16, got ", dt);
+  const int64_t V = logits0.size(-1);
+  const auto rows = logits0.sizes().slice(0, logits0.dim() - 1);
+  int64_t B = 1;
+  for (int64_t n : rows) B *= n;
+  require(V >= 1 && V <= (1ll << 30) && B < (1ll << 31), "logits must have 1 to 2^30 tokens and less than 2^31 rows, got ",
+          shape_str(logits0.sizes()));
+  require(u0.sizes() == rows && (u0.scalar_type() == at::kFloat || u0.scalar_type() == at::kDouble),
+          "u must be float32 or float64 ", shape_str(rows), ", got ", u0.scalar_type(), " ", shape_str(u0.sizes()));
+  require(temperature >= 0.0, "temperature must be a number from 0 on, got ", temperature);
+  require(top_k >= 0, "top_k must be 0 (no limit) or more, got ", top_k);
+  require(top_p >= 0.0 && top_p <= 1.0, "top_p must be from 0 to 1, got ", top_p);
+  require(min_p >= 0.0 && min_p <= 1.0, "min_p must be from 0 to 1, got ", min_p);
+  auto setting = [&](const OptTensor& t, const char* name, bool whole) {
+    if (t)
+      require(t->sizes() == rows && (whole ? at::isIntegralType(t->scalar_type(), false) : at::isFloatingType(t->scalar_type())), name,
+              " must be a number or ", whole ? "integers " : "floats ", shape_str(rows), ", got ", t->scalar_type(), " ",
+              shape_str(t->sizes()));
+  };
+  setting(temperatures0, "temperature", false);
+  setting(top_ks0, "top_k", true);
+  setting(top_ps0, "top_p", false);
+  setting(min_ps0, "min_p", false);
+  if (logprobs && ((at::GradMode::is_enabled() && logits0.requires_grad()) || logits0._fw_grad(0).defined()))
+    raise(PyExc_RuntimeError, "sampled log probabilities have no gradient: detach the logits, or call it under torch.no_grad()");
+  const c10::Device dev = require_gpu({&logits0, &u0});
+  for (const OptTensor* t : {&temperatures0, &top_ks0, &top_ps0, &min_ps0})
+    if (*t) require_gpu({&logits0, &**t});
+  const c10::OptionalDeviceGuard guard(dev);
+  Tensor x = logits0.detach().reshape({B, V});
+  if (x.is_neg()) x = x.resolve_neg();
+  if (x.numel() && x.stride(1) != 1 && V > 1) x = x.contiguous();
+  auto flat = [&](const OptTensor& t, at::ScalarType type) { return t ? t->detach().to(type).contiguous().resolve_neg() : Tensor(); };
+  const Tensor u = u0.detach().contiguous().resolve_neg();
+  const Tensor temperatures = flat(temperatures0, at::kFloat), top_ps = flat(top_ps0, at::kFloat), min_ps = flat(min_ps0, at::kFloat);
+  const Tensor top_ks = flat(top_ks0, at::kLong);
+  const Tensor tokens = at::empty(rows, x.options().dtype(at::kLong));
+  const Tensor logp = logprobs ? at::empty(rows, x.options().dtype(at::kFloat)) : Tensor();
+  dsqg_sample_args a = {};
+  a.B = (int32_t)B; a.V = (int32_t)V;
+  a.dtype = dt == at::kFloat ? DSQG_F32 : dt == at::kBFloat16 ? DSQG_BF16 : DSQG_F16;
+  a.u_is_double = u.scalar_type() == at::kDouble;
+  a.logits = ptr(x); a.logits_stride = B > 1 ? x.stride(0) : 0;
+  a.u = ptr(u);
+  a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
+  a.temperatures = static_cast<const float*>(ptr(temperatures));
+  a.top_ks = static_cast<const int64_t*>(ptr(top_ks));
+  a.top_ps = static_cast<const float*>(ptr(top_ps));
+  a.min_ps = static_cast<const float*>(ptr(min_ps));
+  a.tokens = static_cast<int64_t*>(ptr(tokens));
+  a.logprobs = static_cast<float*>(ptr(logp));
+  check(api.sample(&a, stream_of(dev)), "dsqg_sample");
+  return {tokens, opt(logp)};
+}
+
 void init(const py::dict& addresses, const py::object& library_error) {
   auto get = [&](auto& fn, const char* name) {
     fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addresses[name].cast<uintptr_t>());
@@ -1002,6 +1125,8 @@ void init(const py::dict& addresses, const py::object& library_error) {
   get(api.paged_read, "dsqg_paged_read");
   get(api.paged_decode_workspace_size, "dsqg_paged_decode_workspace_size");
   get(api.paged_decode, "dsqg_paged_decode");
+  get(api.tree_accept, "dsqg_tree_accept");
+  get(api.sample, "dsqg_sample");
   api.library_error = library_error.inc_ref().ptr();  // lives as long as the process
 }
 
@@ -1020,4 +1145,6 @@ PYBIND11_MODULE(_dsqg_host, m) {
   m.def("paged_write", &paged_write);
   m.def("paged_read", &paged_read);
   m.def("paged_decode", &paged_decode);
+  m.def("tree_accept", &tree_accept);
+  m.def("sample", &sample);
 }

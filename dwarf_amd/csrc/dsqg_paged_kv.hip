@@ -78,7 +78,8 @@ struct WriteParams {
   const char* k; long long kb, kh, kn;  // strides in bytes
   const char* v; long long vb, vh, vn;
   const long long* pos; const long long* counts;
-  int N;
+  const long long* src;  // [B, N]: rows of k and v, below S, in the place of 0 .. N - 1; or null
+  int N, S;
   long long rows;  // Hkv * N of one sequence
   long long row0;  // the launch's first
 };
@@ -132,9 +133,11 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteParams p) {
   if (t < 0 || t >= ((long long)p.c.M << p.c.shift)) return;
   const int page = p.c.table[b * p.c.ts + (t >> p.c.shift)];
   if ((unsigned)page >= (unsigned)p.c.P) return;
+  const long long from = p.src ? p.src[(long long)b * p.N + n] : n;
+  if ((unsigned long long)from >= (unsigned long long)p.S) return;
   const long long slot = t & ((1 << p.c.shift) - 1);
-  const char* ks = p.k + b * p.kb + h * p.kh + n * p.kn;
-  const char* vs = p.v + b * p.vb + h * p.vh + n * p.vn;
+  const char* ks = p.k + b * p.kb + h * p.kh + from * p.kn;
+  const char* vs = p.v + b * p.vb + h * p.vh + from * p.vn;
   Raw8<DT> x[R::pieces], y[R::pieces];
 #pragma unroll
   for (int u = 0; u < R::pieces; ++u) {
@@ -306,7 +309,8 @@ extern "C" int dsqg_paged_write(const dsqg_paged_write_args* a, dsqg_stream_t st
   if ((long long)c.B * c.Hkv * a->N == 0) return DSQG_OK;
   const long long es = elem_size(c.dtype);
   auto bad = [](const void* ptr) { return !ptr || (reinterpret_cast<uintptr_t>(ptr) & 15u) != 0; };
-  if (bad(a->k) || bad(a->v) || !a->pos) return DSQG_EINVAL;
+  const bool none = a->rows && a->src_rows == 0;  // (nothing to take rows from: no pointers either)
+  if ((!none && (bad(a->k) || bad(a->v))) || !a->pos) return DSQG_EINVAL;
   for (int i = 0; i < 3; ++i)
     if (a->k_stride[i] < 0 || a->v_stride[i] < 0 || a->k_stride[i] > (1ll << 50) || a->v_stride[i] > (1ll << 50) ||
         a->k_stride[i] * es % 16 != 0 || a->v_stride[i] * es % 16 != 0)
@@ -315,7 +319,11 @@ extern "C" int dsqg_paged_write(const dsqg_paged_write_args* a, dsqg_stream_t st
   p.v = static_cast<const char*>(a->v); p.vb = a->v_stride[0] * es; p.vh = a->v_stride[1] * es; p.vn = a->v_stride[2] * es;
   p.pos = reinterpret_cast<const long long*>(a->pos);
   p.counts = reinterpret_cast<const long long*>(a->counts);
+  p.src = reinterpret_cast<const long long*>(a->rows);
+  if (p.src && a->src_rows < 0) return DSQG_EINVAL;
   p.N = a->N;
+  p.S = p.src ? a->src_rows : a->N;
+  if (p.S == 0) return DSQG_OK;
   p.rows = (long long)c.Hkv * a->N;
   if (p.rows >= kMostRows) return DSQG_EUNSUPPORTED;
   for_dim<WriteDim>(c.D, p, c.dtype, c.cache_dtype, reinterpret_cast<hipStream_t>(stream));

@@ -1,6 +1,7 @@
 """torch custom ops over the C ABI: ``dwarf::dsqg_fwd``, ``dwarf::dsqg_fwd_qkv``, ``dwarf::dsqg_bwd``,
 ``dwarf::dsqg_decode``, the interference pool ``dwarf::pool_gate_fwd`` / ``_bwd``, and the paged cache's
-``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``.
+``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``; ``dwarf::tree_accept`` and
+``dwarf::sample_tokens``.
 
 The ops take device tensors, pass raw pointers, element strides and the current HIP stream
 to libdsqg_hip.so through ctypes, and allocate their outputs (and the backward workspace) with
@@ -668,11 +669,24 @@ torch.library.register_autograd("dwarf::pool_gate_fwd", _pool_backward,
 def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor,
                    counts: Optional[Tensor], k_scale: Optional[Tensor], v_scale: Optional[Tensor]) -> None:
     """Rows of k and v [B,H,N,D] to positions pos .. pos + counts - 1 of the pages."""
-    _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale)
+    _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, None, k_scale, v_scale)
 
 
 @paged_kv_write.register_fake
 def _(k, v, k_pages, v_pages, page_table, pos, counts, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op("dwarf::paged_kv_write_rows", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def paged_kv_write_rows(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor,
+                        counts: Optional[Tensor], rows: Tensor, k_scale: Optional[Tensor],
+                        v_scale: Optional[Tensor]) -> None:
+    """paged_kv_write of the rows that ``rows`` [B,M] names."""
+    _lib.host().paged_write(k, v, k_pages, v_pages, page_table, pos, counts, rows, k_scale, v_scale)
+
+
+@paged_kv_write_rows.register_fake
+def _(k, v, k_pages, v_pages, page_table, pos, counts, rows, k_scale, v_scale):
     return None
 
 
@@ -703,3 +717,38 @@ def paged_decode(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_
 @paged_decode.register_fake
 def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale):
     return q.new_empty(q.shape)
+
+
+# ------------------------------------------------------------------------------------------
+# Drafted tokens and sampling
+# ------------------------------------------------------------------------------------------
+
+@torch.library.custom_op("dwarf::tree_accept", mutates_args=())
+def tree_accept(tokens: Tensor, parents: Tensor, picks: Tensor,
+                counts: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    """(path [B,T], n [B], next [B]) of a tree of drafted tokens."""
+    return _lib.host().tree_accept(tokens, parents, picks, counts)
+
+
+@tree_accept.register_fake
+def _(tokens, parents, picks, counts):
+    B, T = tokens.shape
+    i64 = dict(dtype=torch.int64)
+    return tokens.new_empty((B, T), **i64), tokens.new_empty((B,), **i64), tokens.new_empty((B,), **i64)
+
+
+@torch.library.custom_op("dwarf::sample_tokens", mutates_args=())
+def sample_tokens(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: float, min_p: float,
+                  temperatures: Optional[Tensor], top_ks: Optional[Tensor], top_ps: Optional[Tensor],
+                  min_ps: Optional[Tensor], return_logprobs: bool) -> Tuple[Tensor, Tensor]:
+    """Tokens [...] of logits [...,V], and their log probabilities (empty unless asked for)."""
+    tokens, logprobs = _lib.host().sample(logits, u, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps,
+                                          min_ps, return_logprobs)
+    return tokens, logits.new_empty((0,), dtype=torch.float32) if logprobs is None else logprobs
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, return_logprobs):
+    rows = logits.shape[:-1]
+    return (logits.new_empty(rows, dtype=torch.int64),
+            logits.new_empty(rows if return_logprobs else (0,), dtype=torch.float32))

@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DSQG_ABI_VERSION 5
+#define DSQG_ABI_VERSION 6
 #define DSQG_MAX_OFFSETS 64
 
 /* Same type as hipStream_t; NULL is the null stream. */
@@ -356,7 +356,8 @@ typedef struct {
 
 /* Row i of sequence b of k and v [B,Hkv,N,D] (unit inner stride, strides {b, h, n}, rows 16-byte
  * aligned) goes to position pos[b] + i, for i < N and, where counts is given, i < counts[b]; every
- * other row of the pools stays as it is. */
+ * other row of the pools stays as it is.  Where rows [B,N] is given (contiguous), row rows[b,i] of
+ * k and v [B,Hkv,S,D], S = src_rows, goes there instead, and one whose number is none of theirs is not written. */
 typedef struct {
     dsqg_paged_cache cache;
     int32_t N;
@@ -364,6 +365,8 @@ typedef struct {
     const void* v;  int64_t v_stride[3];
     const int64_t* pos;        /* [B] */
     const int64_t* counts;     /* [B] or NULL */
+    const int64_t* rows;       /* [B,N] or NULL */
+    int32_t src_rows;          /* with rows: rows of k and v */
 } dsqg_paged_write_args;
 
 int dsqg_paged_write(const dsqg_paged_write_args* args, dsqg_stream_t stream);
@@ -412,6 +415,65 @@ typedef struct {
 
 int dsqg_paged_decode_workspace_size(const dsqg_paged_decode_args* args, size_t* bytes);
 int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
+
+/* The accepted path of a tree of drafted tokens (no counterpart in the reference).  Node i of sequence b has
+ * the token tokens[b,i] and hangs on the node parents[b,i] (parents_stride 0: one tree for all); picks[b,i] is the
+ * token that the model chose after node i.  Node 0 is accepted; from a node the walk goes to its first child behind it
+ * whose token is the node's pick.  With counts given, only nodes i < counts[b] exist.
+ *
+ *     path[b,0..n[b]-1]: the nodes on the way, -1 behind them;  next[b]: the last one's pick
+ *
+ * A sequence without nodes has n = 0 and next = -1.  tokens and picks have unit inner stride, path [B,T], n [B] and
+ * next [B] are contiguous; T is at most DSQG_MAX_TREE (EUNSUPPORTED otherwise). */
+#define DSQG_MAX_TREE 64
+
+typedef struct {
+    int32_t B, T;
+    const int64_t* tokens;   int64_t tokens_stride;
+    const int32_t* parents;  int64_t parents_stride;
+    const int64_t* picks;    int64_t picks_stride;
+    const int64_t* counts;     /* [B] or NULL */
+    int64_t* path;
+    int64_t* n;
+    int64_t* next;
+} dsqg_tree_accept_args;
+
+int dsqg_tree_accept(const dsqg_tree_accept_args* args, dsqg_stream_t stream);
+
+/* A token of each row of logits by one number from [0, 1) (the reference's sampling, greedy or a nucleus,
+ * train/train_2048_condU.py:474-484, with the limits in use since).  With w_i = exp((x_i - max x) / T) and the order of
+ * x descending, of equal ones the lower index first, the tokens that stay are the first top_k, of those the ones
+ * before which at most top_p of their mass lies, of those the ones with w >= min_p.
+ *
+ *     tokens[b] = the first i whose running mass, by index, is above u[b] times the mass that stays
+ *     logprobs[b] = log(w / mass that stays)
+ *
+ * A temperature that is not above zero takes the largest logit (logprobs 0).  A NaN is no candidate, and neither is
+ * -infinity; a row without candidates gives -1 and -infinity; infinities share a row's mass.  Masses are whole
+ * multiples of 2^-F, F = 48 up to 2^14 tokens and 62 - ceil(log2 V) beyond, so that no result depends on an order.
+ * top_k <= 0 or >= V, top_p >= 1 and min_p <= 0 limit nothing; min_p above 1 is 1.  A u that is not a
+ * number or below 0 is 0, one of 1 or more takes the last token that stays.
+ *
+ * logits [B,V] have unit inner stride and any row stride and alignment (of an element); V is at most 2^30.  u is
+ * float, or double where u_is_double.  A setting's array, where given, has the rows' own in the place of the
+ * one for all, which must not be NaN. */
+typedef struct {
+    int32_t B, V;
+    int32_t dtype;             /* DSQG_F32, DSQG_BF16 or DSQG_F16 */
+    int32_t u_is_double;
+    const void* logits;  int64_t logits_stride;
+    const void* u;             /* [B] */
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    const float* temperatures; /* [B] or NULL, and so on */
+    const int64_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    int64_t* tokens;           /* [B] */
+    float* logprobs;           /* [B] or NULL */
+} dsqg_sample_args;
+
+int dsqg_sample(const dsqg_sample_args* args, dsqg_stream_t stream);
 
 #ifdef __cplusplus
 }
