@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DSQG_HIP_LIB", PKG_DIR / "libdsqg_hip.so"))
 
 MAX_OFFSETS = 64
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DSQG_OK, DSQG_EINVAL, DSQG_EUNSUPPORTED, DSQG_EHIP, DSQG_EWORKSPACE = 0, 1, 2, 3, 4
 DSQG_ETOOLARGE = 5
@@ -158,6 +158,14 @@ class TreeAcceptArgs(ctypes.Structure):
                 ("path", _vp), ("n", _vp), ("next", _vp)]
 
 
+class PagedTreeArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCache), ("H", ctypes.c_int32), ("T", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+                ("q", _vp), ("q_stride", _i64x3), ("k_new", _vp), ("k_new_stride", _i64x3),
+                ("v_new", _vp), ("v_new_stride", _i64x3), ("parents", _vp), ("parents_stride", ctypes.c_int64),
+                ("counts", _vp), ("pos", _vp), ("out", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class SampleArgs(ctypes.Structure):
     _fields_ = [("B", ctypes.c_int32), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32), ("u_is_double", ctypes.c_int32),
                 ("logits", _vp), ("logits_stride", ctypes.c_int64), ("u", _vp),
@@ -198,6 +206,9 @@ SIGNATURES = {
                                                         ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs), _vp]),
     "dsqg_tree_accept": (ctypes.c_int, [ctypes.POINTER(TreeAcceptArgs), _vp]),
+    "dsqg_paged_tree_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs),
+                                                      ctypes.POINTER(ctypes.c_size_t)]),
+    "dsqg_paged_tree": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs), _vp]),
     "dsqg_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
 }
 

@@ -16,7 +16,8 @@
 * ``paged_kv_write`` / ``paged_decode_step`` / ``paged_kv_read`` and ``PagedKVCache`` -- full attention
   over a paged key/value cache, of the rows' type or 8 bits wide (no counterpart in the reference,
   whose full-attention layer, train/train_2048_condU.py:210-245, keeps no cache).
-* ``draft_tree_accept`` -- which of the tokens drafted as a tree the model's picks keep.
+* ``paged_tree_step`` -- several drafted tokens of each sequence over that cache, as a tree or a chain, whole or within
+  a window; ``draft_tree_accept`` -- which of the tokens drafted as a tree the model's picks keep.
 * ``sample_tokens`` -- the next token from logits and given random numbers: the sampling of
   train/train_2048_condU.py:474-484 with top-k and min-p, in one kernel.
 
@@ -260,6 +261,35 @@ def paged_decode_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
                                     softmax_scale)
 
 
+def paged_tree_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_pages: Tensor, v_pages: Tensor,
+                    page_table: Tensor, pos: Tensor, parents: Optional[Tensor] = None, *,
+                    counts: Optional[Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                    k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None,
+                    softmax_scale: Optional[float] = None) -> Tensor:
+    """A step of T tokens of each sequence, drafted as a tree, over a paged cache (see ``paged_kv_write``): k_new, v_new
+    [B,Hkv,T,D] go to positions pos[b] .. pos[b] + T - 1, and node i of the H = Hkv * G query heads q [B,H,T,D] attends
+    the positions before pos[b], its ancestors and itself; returns out [B,H,T,D] (token-major storage).  T is at most 64.
+
+    Node i hangs on the earlier node parents[i] (or parents[b,i]) or, -1, on the last position before pos[b]; without
+    parents the tokens are a chain.  With counts, sequence b has counts[b] nodes; rows behind them are not written.
+    What is no node, behind counts[b] or on parents that do not lead over earlier nodes to -1, gets zeros.  With a window
+    a node, at the place pos[b] + its depth, sees the window places up to its own and those below ``sinks``
+    (``window_attention``); a chain of one token is a windowed layer's decode step, and pages that no later
+    step sees may be given away.
+
+    With k_new = v_new = None nothing is written and the draft's rows are attended as the pages hold them.  A
+    sequence with pos[b] < 0 gets zeros and writes nothing, a node that sees a position without a page NaN.  A row that a
+    node does not see does not reach it, whatever it holds.  The range of values is ``paged_decode_step``'s.  Weights of
+    T * G > 16 tokens and heads are rounded once, to the cache's 16-bit type (8 bits: bfloat16), before they multiply
+    the values.  The step has no gradient.  ``draft_tree_accept`` says which rows to keep.
+    """
+    if ops.traced(q, k_pages, v_pages):
+        return ops.paged_tree(q, k_new, v_new, k_pages, v_pages, page_table, pos, parents, counts, window, sinks, k_scale,
+                              v_scale, softmax_scale)
+    return _lib.host().paged_tree(q, k_new, v_new, k_pages, v_pages, page_table, pos, parents, counts, window, sinks,
+                                  k_scale, v_scale, softmax_scale)
+
+
 def draft_tree_accept(tokens: Tensor, parents: Tensor, picks: Tensor, counts: Optional[Tensor] = None):
     """(path [B,T], n [B], next [B]), int64: which of the tokens drafted as a tree are kept.
 
@@ -344,7 +374,8 @@ class PagedKVCache:
 
     ``dtype`` is the type of the rows and, unless ``kv_dtype`` (torch.float8_e4m3fn or torch.int8) asks for
     8 bits, of the pages.  ``prefill(k, v)`` loads a prompt, ``write(k, v)`` appends rows, ``step(q, k_t,
-    v_t)`` runs one decode step and advances, ``read()`` returns the rows.  Every sequence owns its pages,
+    v_t)`` runs one decode step and advances, ``tree_step`` and ``accept`` try several drafted tokens and keep some of
+    them, ``read()`` returns the rows.  Every sequence owns its pages,
     sequence b those from b * M on; a caller that shares or moves pages sets ``page_table``.  The host
     does not know the positions: rows past a sequence's last page are not kept, and its steps give NaN.
     A sequence at a negative position is not in use: its pages and position stay as they are and its steps
@@ -408,6 +439,24 @@ class PagedKVCache:
                                 **self._state())
         self.pos += self.pos >= 0
         return out.to(q.dtype)
+
+    def tree_step(self, q: Tensor, k_new: Tensor, v_new: Tensor, parents: Optional[Tensor] = None,
+                  counts: Optional[Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                  softmax_scale: Optional[float] = None) -> Tensor:
+        """Output [B,H*G,T,D] of T tokens drafted as a tree (``paged_tree_step``).  Their rows lie behind the sequences'
+        positions, which stay as they are until ``accept`` says what is kept."""
+        dt = self.dtype
+        out = paged_tree_step(q.detach().to(dt), k_new.detach().to(dt), v_new.detach().to(dt), self.k_pages, self.v_pages,
+                              self.page_table, self.pos, parents, counts=counts, window=window, sinks=sinks,
+                              softmax_scale=softmax_scale, **self._state())
+        return out.to(q.dtype)
+
+    def accept(self, k_new: Tensor, v_new: Tensor, path: Tensor, n: Tensor) -> None:
+        """Keep the rows of the nodes path[b,:n[b]] (``draft_tree_accept``) of a draft's k_new, v_new, and advance by n."""
+        n = (self.pos >= 0) * n.long().clamp(0, path.shape[1])
+        paged_kv_write(k_new.detach().to(self.dtype), v_new.detach().to(self.dtype), self.k_pages, self.v_pages,
+                       self.page_table, self.pos, counts=n, rows=path, **self._state())
+        self.pos += n
 
     def read(self, max_len: Optional[int] = None, dtype: Optional[torch.dtype] = None):
         """(k, v) [B,H,max_len,D] (default: the cache's max_len) of the positions written so far, zeros

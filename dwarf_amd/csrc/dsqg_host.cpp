@@ -44,6 +44,8 @@ struct Api {
   decltype(&dsqg_paged_read) paged_read = nullptr;
   decltype(&dsqg_paged_decode_workspace_size) paged_decode_workspace_size = nullptr;
   decltype(&dsqg_paged_decode) paged_decode = nullptr;
+  decltype(&dsqg_paged_tree_workspace_size) paged_tree_workspace_size = nullptr;
+  decltype(&dsqg_paged_tree) paged_tree = nullptr;
   decltype(&dsqg_tree_accept) tree_accept = nullptr;
   decltype(&dsqg_sample) sample = nullptr;
   PyObject* library_error = nullptr;  // dwarf_amd._lib.DSQGLibraryError
@@ -1044,6 +1046,78 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& tokens0, const Tens
   return {path, n, next};
 }
 
+// A window (none: 0) and its sinks as the kernels read them: no place is 2^30 positions from another.
+void set_window(int32_t* window, int32_t* sinks, std::optional<int64_t> w, int64_t s) {
+  require(!w || *w >= 1, "window must be positive (or None), got ", w.value_or(0));
+  require(s >= 0, "sinks must be 0 or more, got ", s);
+  *window = w ? (int32_t)std::min<int64_t>(*w, 1 << 30) : 0;
+  *sinks = w ? (int32_t)std::min<int64_t>(s, 1 << 30) : 0;
+}
+
+Tensor paged_tree(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, const Tensor& kp, const Tensor& vp, const Tensor& table,
+                  const Tensor& pos0, const OptTensor& parents0, const OptTensor& counts0, std::optional<int64_t> window, int64_t sinks,
+                  const OptTensor& ks, const OptTensor& vs, std::optional<double> scale) {
+  py::gil_scoped_release nogil;
+  const Tensor kn = undef(k0), vn = undef(v0);
+  refuse_grad({&q0, &kn, &vn, &kp, &vp});
+  const auto dt = q0.scalar_type();
+  require(q0.dim() == 4, "q must be [B,H,T,D], got ", shape_str(q0.sizes()));
+  require(kn.defined() == vn.defined(), "k_new and v_new go together");
+  Paged c(kp, vp, table, ks, vs, dt, kn.defined());
+  require(ks.has_value() || kp.scalar_type() == dt, "queries of ", dt, " do not go with pages of ", kp.scalar_type());
+  const int64_t B = c.a.B, Hkv = c.a.Hkv, D = c.a.D, H = q0.size(1), T = q0.size(2);
+  require(q0.size(0) == B && q0.size(3) == D && (Hkv > 0 ? H > 0 && H % Hkv == 0 : H == 0), "q must be [", B, ",H,T,", D,
+          "] with H a positive multiple of ", Hkv, ", got ", shape_str(q0.sizes()));
+  for (const Tensor* t : {&kn, &vn})
+    if (t->defined())
+      require(t->sizes() == c10::IntArrayRef({B, Hkv, T, D}) && t->scalar_type() == dt, "k_new and v_new must be ", dt, " ",
+              shape_str({B, Hkv, T, D}), " tensors, got ", t->scalar_type(), " ", shape_str(t->sizes()));
+  require(T >= 1 && T <= DSQG_MAX_TREE, "a step has 1 to ", DSQG_MAX_TREE, " tokens, got ", T);
+  if (parents0) check_tree(*parents0, counts0, B, T);
+  else if (counts0)
+    require(at::isIntegralType(counts0->scalar_type(), false) && counts0->sizes() == c10::IntArrayRef({B}), "counts must be an integer [", B,
+            "] tensor, got ", counts0->scalar_type(), " ", shape_str(counts0->sizes()));
+  dsqg_paged_tree_args a = {};
+  set_window(&a.window, &a.sinks, window, sinks);
+  c.place({&q0, &kn, &vn});
+  if (parents0) require_gpu({&kp, &*parents0});
+  const c10::OptionalDeviceGuard guard(c.dev);
+  const Tensor q = plain_rows(q0), pos = c.index(pos0, "pos");
+  const Tensor parents = parents0 ? node_table(*parents0, at::kInt) : Tensor();
+  const Tensor counts = counts0 ? c.index(*counts0, "counts") : Tensor();
+  const Tensor k = kn.defined() ? plain_rows(kn) : kn, v = vn.defined() ? plain_rows(vn) : vn;
+  // Token-major storage: the callers' head merge is a view.
+  const Tensor out = at::empty_strided({B, H, T, D}, {T * H * D, D, H * D, 1}, q0.options());
+  a.cache = c.a;
+  a.H = (int32_t)H; a.T = (int32_t)T;
+  a.softmax_scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
+  a.q = ptr(q);
+  if (kn.defined()) { a.k_new = ptr(k); a.v_new = ptr(v); }
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = q.stride(i);
+    if (kn.defined()) { a.k_new_stride[i] = k.stride(i); a.v_new_stride[i] = v.stride(i); }
+  }
+  a.parents = static_cast<const int32_t*>(ptr(parents));
+  a.parents_stride = parents0 && parents.dim() == 2 && B > 1 ? parents.stride(0) : 0;
+  a.counts = static_cast<const int64_t*>(ptr(counts));
+  a.pos = static_cast<const int64_t*>(ptr(pos));
+  a.out = ptr(out);
+  size_t nbytes = 0;
+  check(api.paged_tree_workspace_size(&a, &nbytes), "dsqg_paged_tree_workspace_size");
+  Tensor ws;
+  if (nbytes) {
+    ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = nbytes;
+  }
+  check(api.paged_tree(&a, stream_of(c.dev)), "dsqg_paged_tree");
+  if (kn.defined()) {
+    cache_changed({&kp, &vp});
+    if (ks) cache_changed({&*ks, &*vs});
+  }
+  return out;
+}
+
 std::tuple<Tensor, OptTensor> sample(const Tensor& logits0, const Tensor& u0, double temperature, int64_t top_k, double top_p, double min_p,
                                      const OptTensor& temperatures0, const OptTensor& top_ks0, const OptTensor& top_ps0,
                                      const OptTensor& min_ps0, bool logprobs) {
@@ -1125,6 +1199,8 @@ void init(const py::dict& addresses, const py::object& library_error) {
   get(api.paged_read, "dsqg_paged_read");
   get(api.paged_decode_workspace_size, "dsqg_paged_decode_workspace_size");
   get(api.paged_decode, "dsqg_paged_decode");
+  get(api.paged_tree_workspace_size, "dsqg_paged_tree_workspace_size");
+  get(api.paged_tree, "dsqg_paged_tree");
   get(api.tree_accept, "dsqg_tree_accept");
   get(api.sample, "dsqg_sample");
   api.library_error = library_error.inc_ref().ptr();  // lives as long as the process
@@ -1145,6 +1221,7 @@ PYBIND11_MODULE(_dsqg_host, m) {
   m.def("paged_write", &paged_write);
   m.def("paged_read", &paged_read);
   m.def("paged_decode", &paged_decode);
+  m.def("paged_tree", &paged_tree);
   m.def("tree_accept", &tree_accept);
   m.def("sample", &sample);
 }

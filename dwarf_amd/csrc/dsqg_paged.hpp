@@ -192,6 +192,31 @@ __device__ __forceinline__ float group_max_nan(float x) {
   return x;
 }
 
+// A row of the caller's type DT as the pool keeps it.
+template <int DT, int CT, int D>
+__device__ __forceinline__ void put_row(char* dst, unsigned char* sc, const Raw8<DT> (&x)[RowMap<D>::pieces], int g) {
+  using R = RowMap<D>;
+  if constexpr (!narrow(CT)) {
+    static_assert(DT == CT, "a 16- or 32-bit pool has the rows' type");
+#pragma unroll
+    for (int u = 0; u < R::pieces; ++u)
+      if (g + R::lanes * u < R::CPR) raw_store<CT>(dst + (g + R::lanes * u) * 8 * elem_size(CT), x[u]);
+  } else {
+    float f[R::pieces][8], m = 0.f;
+#pragma unroll
+    for (int u = 0; u < R::pieces; ++u) {
+      raw_floats<DT>(x[u], f[u]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(f[u][i]));
+    }
+    const int byte = scale_byte<CT>(group_max_nan<R::lanes>(m));
+#pragma unroll
+    for (int u = 0; u < R::pieces; ++u)
+      if (g + R::lanes * u < R::CPR) raw_store<CT>(dst + (g + R::lanes * u) * 8, raw_encode<CT>(f[u], byte));
+    if (g == 0) *sc = (unsigned char)byte;
+  }
+}
+
 // ---- The decode step. -----------------------------------------------------------------------------------
 
 // A step's work is split over workgroups in one of two ways.

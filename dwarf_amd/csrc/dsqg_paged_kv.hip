@@ -94,31 +94,6 @@ struct ReadParams {
   long long row0;  // the launch's first
 };
 
-// A row of the caller's type DT as the pool keeps it.
-template <int DT, int CT, int D>
-__device__ __forceinline__ void put_row(char* dst, unsigned char* sc, const Raw8<DT> (&x)[RowMap<D>::pieces], int g) {
-  using R = RowMap<D>;
-  if constexpr (!narrow(CT)) {
-    static_assert(DT == CT, "a 16- or 32-bit pool has the rows' type");
-#pragma unroll
-    for (int u = 0; u < R::pieces; ++u)
-      if (g + R::lanes * u < R::CPR) raw_store<CT>(dst + (g + R::lanes * u) * 8 * elem_size(CT), x[u]);
-  } else {
-    float f[R::pieces][8], m = 0.f;
-#pragma unroll
-    for (int u = 0; u < R::pieces; ++u) {
-      raw_floats<DT>(x[u], f[u]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(f[u][i]));
-    }
-    const int byte = scale_byte<CT>(group_max_nan<R::lanes>(m));
-#pragma unroll
-    for (int u = 0; u < R::pieces; ++u)
-      if (g + R::lanes * u < R::CPR) raw_store<CT>(dst + (g + R::lanes * u) * 8, raw_encode<CT>(f[u], byte));
-    if (g == 0) *sc = (unsigned char)byte;
-  }
-}
-
 // Grid: x over rows (h, n) of a sequence, n fastest; y over sequences.
 template <int DT, int CT, int D>
 __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteParams p) {

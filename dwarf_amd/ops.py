@@ -1,7 +1,7 @@
 """torch custom ops over the C ABI: ``dwarf::dsqg_fwd``, ``dwarf::dsqg_fwd_qkv``, ``dwarf::dsqg_bwd``,
 ``dwarf::dsqg_decode``, the interference pool ``dwarf::pool_gate_fwd`` / ``_bwd``, and the paged cache's
-``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``; ``dwarf::tree_accept`` and
-``dwarf::sample_tokens``.
+``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``; ``dwarf::paged_tree``,
+``dwarf::tree_accept`` and ``dwarf::sample_tokens``.
 
 The ops take device tensors, pass raw pointers, element strides and the current HIP stream
 to libdsqg_hip.so through ctypes, and allocate their outputs (and the backward workspace) with
@@ -722,6 +722,23 @@ def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, soft
 # ------------------------------------------------------------------------------------------
 # Drafted tokens and sampling
 # ------------------------------------------------------------------------------------------
+
+@torch.library.custom_op("dwarf::paged_tree", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def paged_tree(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_pages: Tensor, v_pages: Tensor,
+               page_table: Tensor, pos: Tensor, parents: Optional[Tensor], counts: Optional[Tensor],
+               window: Optional[int], sinks: int, k_scale: Optional[Tensor], v_scale: Optional[Tensor],
+               softmax_scale: Optional[float]) -> Tensor:
+    """out [B,H,T,D] (token-major storage) of T drafted tokens per sequence; their rows go to the pages."""
+    return _lib.host().paged_tree(q, k_new, v_new, k_pages, v_pages, page_table, pos, parents, counts, window, sinks,
+                                  k_scale, v_scale, softmax_scale)
+
+
+@paged_tree.register_fake
+def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, parents, counts, window, sinks, k_scale, v_scale,
+      softmax_scale):
+    B, H, T, D = q.shape
+    return q.new_empty((B, T, H, D)).permute(0, 2, 1, 3)
+
 
 @torch.library.custom_op("dwarf::tree_accept", mutates_args=())
 def tree_accept(tokens: Tensor, parents: Tensor, picks: Tensor,

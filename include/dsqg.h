@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DSQG_ABI_VERSION 6
+#define DSQG_ABI_VERSION 7
 #define DSQG_MAX_OFFSETS 64
 
 /* Same type as hipStream_t; NULL is the null stream. */
@@ -439,6 +439,45 @@ typedef struct {
 } dsqg_tree_accept_args;
 
 int dsqg_tree_accept(const dsqg_tree_accept_args* args, dsqg_stream_t stream);
+
+/* A step of T tokens of each sequence over a paged cache, drafted as a tree: k_new and v_new [B,Hkv,T,D] go to positions
+ * pos[b] .. pos[b] + T - 1 (as dsqg_paged_write puts them there), and node i attends the positions before pos[b], its
+ * ancestors and itself:
+ *
+ *     out[b,h,i] = sum_t softmax_t(softmax_scale * q[b,h,i] . k_t) v_t
+ *
+ * of the rows as the cache holds them (H a multiple of Hkv, as in dsqg_paged_decode).  Node i hangs on the earlier node
+ * parents[b,i] or, -1, on the position before pos[b] (parents_stride 0: one tree for all; parents NULL: a chain).  With
+ * counts given only nodes i < counts[b] exist.  What is no node, behind counts[b] or on parents that do not lead to -1
+ * over earlier nodes, gets zeros; rows of the former are not written.
+ *
+ * With a window (0: none) a node at place pos[b] + depth sees the places above its own less window, and those below
+ * sinks; a stored position is its own place.
+ *
+ * With k_new = v_new = NULL nothing is written and the draft's rows are attended as the pages hold them.  A sequence with
+ * pos[b] < 0 is not in use: zeros, and nothing is written.  A node that sees a position without a page gets NaN.  A row
+ * that a node does not see does not reach it, whatever it holds.  The range of values is dsqg_paged_decode's; its rules
+ * for strides, q_stride {b, h, t} and so on, and workspace hold; out is contiguous [B,T,H,D].  Weights enter the sum as
+ * two 16-bit terms where T * H / Hkv is at most 16, else as one (16-bit queries).  T is at most DSQG_MAX_TREE and B * H * T
+ * less than 2^30 (EUNSUPPORTED otherwise).  No two sequences may have the same page at positions that a step writes. */
+typedef struct {
+    dsqg_paged_cache cache;
+    int32_t H, T;
+    int32_t window, sinks;
+    float softmax_scale;
+    const void* q;      int64_t q_stride[3];
+    const void* k_new;  int64_t k_new_stride[3];
+    const void* v_new;  int64_t v_new_stride[3];
+    const int32_t* parents;  int64_t parents_stride;
+    const int64_t* counts;     /* [B] or NULL */
+    const int64_t* pos;        /* [B] */
+    void* out;
+    void* workspace;
+    size_t workspace_bytes;
+} dsqg_paged_tree_args;
+
+int dsqg_paged_tree_workspace_size(const dsqg_paged_tree_args* args, size_t* bytes);
+int dsqg_paged_tree(const dsqg_paged_tree_args* args, dsqg_stream_t stream);
 
 /* A token of each row of logits by one number from [0, 1) (the reference's sampling, greedy or a nucleus,
  * train/train_2048_condU.py:474-484, with the limits in use since).  With w_i = exp((x_i - max x) / T) and the order of

@@ -100,3 +100,36 @@ def bound(out, mass, size, D, T, dtype):
         tol = tol + mass[:, 0] * 2.0 ** -16 + (mass[:, 1] * 2.0 ** -37 if dtype == torch.float16 else 0)
     fi = torch.finfo(dtype)
     return tol + (out.abs() + tol) * (fi.eps / 2) + fi.smallest_normal * fi.eps
+
+
+def tree_rows(parents, count):
+    """(ancestors and itself, depth) of each node of a tree, or None for what is no node."""
+    res = []
+    for i, p in enumerate(parents):
+        line = None
+        if i < count and -1 <= p < i:
+            if p == -1:
+                line = [i]
+            elif res[p] is not None:
+                line = res[p][0] + [i]
+        res.append(None if line is None else (line, len(line) - 1))
+    return res
+
+
+def tree_sees(node, nodes, n, window=None, sinks=0):
+    """Rows (positions, the draft's from n on) that a node sees behind n stored positions."""
+    line, depth = node
+    place = {t: t for t in range(n)}
+    place.update({n + j: n + nodes[j][1] for j in line})
+    return [t for t, at in place.items() if window is None or at > n + depth - window or at < sinks]
+
+
+def tree_bound(out, mass, size, D, T, dtype, kv_dtype, columns):
+    """``bound`` for the drafted tokens' step, whose weights are one 16-bit term where more than 16 columns (tokens and
+    heads of a key/value head) share the cache: half a step of it, eps / 2 of each weight, and in float16 where the largest
+    weight is 2^14 its subnormal step, 2^-24, in its place: 2^-38 of ``mass[:, 1]``.  Weights over 8 bits are bfloat16."""
+    tol = bound(out, mass, size, D, T, dtype)
+    if dtype != torch.float32 and columns > 16:
+        one = torch.finfo(torch.bfloat16 if kv_dtype.itemsize == 1 else dtype).eps / 2
+        tol = tol + mass[:, 0] * one * (1 + torch.finfo(dtype).eps) + mass[:, 1] * 2.0 ** -38
+    return tol
