@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DSQG_HIP_LIB", PKG_DIR / "libdsqg_hip.so"))
 
 MAX_OFFSETS = 64
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DSQG_OK, DSQG_EINVAL, DSQG_EUNSUPPORTED, DSQG_EHIP, DSQG_EWORKSPACE = 0, 1, 2, 3, 4
 DSQG_ETOOLARGE = 5
@@ -148,6 +148,25 @@ class PagedDecodeArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class WindowShape(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+                ("N", ctypes.c_int32), ("D", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("softmax_scale", ctypes.c_float), ("lengths", _vp)]
+
+
+class WindowFwdArgs(ctypes.Structure):
+    _fields_ = [("shape", WindowShape), ("q", _vp), ("q_stride", _i64x3), ("k", _vp), ("k_stride", _i64x3),
+                ("v", _vp), ("v_stride", _i64x3), ("out", _vp), ("out_stride", _i64x3), ("stats", _vp)]
+
+
+class WindowBwdArgs(ctypes.Structure):
+    _fields_ = [("shape", WindowShape), ("q", _vp), ("q_stride", _i64x3), ("k", _vp), ("k_stride", _i64x3),
+                ("v", _vp), ("v_stride", _i64x3), ("out", _vp), ("out_stride", _i64x3),
+                ("dout", _vp), ("dout_stride", _i64x3), ("stats", _vp),
+                ("dq", _vp), ("dq_stride", _i64x3), ("dk", _vp), ("dk_stride", _i64x3),
+                ("dv", _vp), ("dv_stride", _i64x3), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 MAX_TREE = 64  # DSQG_MAX_TREE
 
 
@@ -206,6 +225,10 @@ SIGNATURES = {
                                                         ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDecodeArgs), _vp]),
     "dsqg_tree_accept": (ctypes.c_int, [ctypes.POINTER(TreeAcceptArgs), _vp]),
+    "dsqg_window_fwd": (ctypes.c_int, [ctypes.POINTER(WindowFwdArgs), _vp]),
+    "dsqg_window_bwd_workspace_size": (ctypes.c_int, [ctypes.POINTER(WindowShape),
+                                                      ctypes.POINTER(ctypes.c_size_t)]),
+    "dsqg_window_bwd": (ctypes.c_int, [ctypes.POINTER(WindowBwdArgs), _vp]),
     "dsqg_paged_tree_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs),
                                                       ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_paged_tree": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs), _vp]),

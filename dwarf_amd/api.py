@@ -16,6 +16,7 @@
 * ``paged_kv_write`` / ``paged_decode_step`` / ``paged_kv_read`` and ``PagedKVCache`` -- full attention
   over a paged key/value cache, of the rows' type or 8 bits wide (no counterpart in the reference,
   whose full-attention layer, train/train_2048_condU.py:210-245, keeps no cache).
+* ``window_attention`` -- full attention narrowed to a window and a few first positions, with gradients.
 * ``paged_tree_step`` -- several drafted tokens of each sequence over that cache, as a tree or a chain, whole or within
   a window; ``draft_tree_accept`` -- which of the tokens drafted as a tree the model's picks keep.
 * ``sample_tokens`` -- the next token from logits and given random numbers: the sampling of
@@ -199,6 +200,23 @@ def causal_mean_pool_gate(x: Tensor, gate_pre: Tensor) -> Tensor:
     if ops.traced(x, gate_pre):
         return ops.pool_gate_fwd(x, gate_pre)
     return _lib.host().pool_gate(x, gate_pre)
+
+
+def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int = 0, *,
+                     lengths: Optional[Tensor] = None, softmax_scale: Optional[float] = None) -> Tensor:
+    """Causal softmax attention within a window, forward and backward on the HIP kernels: position i of q [B,H,N,D] sees
+    position j <= i of k, v [B,Hkv,N,D] if i - j < window or j < sinks, query head h the key/value head h // (H // Hkv);
+    returns out [B,H,N,D] (token-major storage).  A window of N or more is full causal attention.
+
+    With lengths [B], integers, rows from lengths[b] on are not there: nothing sees them, their outputs and gradients
+    are zeros.  softmax_scale defaults to D ** -0.5.  float32, bfloat16 and float16, head dims 32, 64, 80, 96 and 128;
+    sums and softmax statistics are fp32 and deterministic, and weights (in the backward their gradients too) are
+    rounded once to a 16-bit type before they multiply rows.  What a query does not see does not reach it, whatever
+    it holds.  There is no second derivative.  ``paged_tree_step`` with the same window and sinks continues over a cache.
+    """
+    if ops.traced(q, k, v):
+        return ops.window_fwd(q, k, v, lengths, window, sinks, softmax_scale)[0]
+    return _lib.host().window(q, k, v, lengths, window, sinks, softmax_scale)
 
 
 def paged_kv_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, pos: Tensor, *,

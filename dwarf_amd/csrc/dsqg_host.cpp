@@ -44,6 +44,9 @@ struct Api {
   decltype(&dsqg_paged_read) paged_read = nullptr;
   decltype(&dsqg_paged_decode_workspace_size) paged_decode_workspace_size = nullptr;
   decltype(&dsqg_paged_decode) paged_decode = nullptr;
+  decltype(&dsqg_window_fwd) window_fwd = nullptr;
+  decltype(&dsqg_window_bwd_workspace_size) window_bwd_workspace_size = nullptr;
+  decltype(&dsqg_window_bwd) window_bwd = nullptr;
   decltype(&dsqg_paged_tree_workspace_size) paged_tree_workspace_size = nullptr;
   decltype(&dsqg_paged_tree) paged_tree = nullptr;
   decltype(&dsqg_tree_accept) tree_accept = nullptr;
@@ -996,6 +999,149 @@ Tensor paged_decode(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, 
   return out;
 }
 
+// ---- Attention within a window. --------------------------------------------------------------------------------------
+
+// Rows as the window's kernels read them: rows_ready's, which do not overlap and are less than 2^24 bytes apart.
+Tensor window_rows(const Tensor& t0) {
+  const Tensor t = plain_rows(t0);
+  const int64_t n = t.size(2), row = t.stride(2);
+  return t.numel() == 0 || n == 1 || (row >= t.size(3) && row * t.element_size() < (1 << 24)) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// A [B,H,N,D] tensor in token-major storage: merging the heads is a view.
+Tensor token_major(const Tensor& like) {
+  const int64_t B = like.size(0), H = like.size(1), N = like.size(2), D = like.size(3);
+  return at::empty_strided({B, H, N, D}, {N * H * D, D, H * D, 1}, like.options());
+}
+
+void set_strides(int64_t (&dst)[3], const Tensor& t) {
+  for (int i = 0; i < 3; ++i) dst[i] = t.stride(i);
+}
+
+// The checks that need no GPU, and the argument block.
+dsqg_window_shape window_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, int64_t window, int64_t sinks,
+                               std::optional<double> scale) {
+  const auto dt = q.scalar_type();
+  require(q.dim() == 4, "q must be [B,H,N,D], got ", shape_str(q.sizes()));
+  require(dt == at::kFloat || dt == at::kBFloat16 || dt == at::kHalf, "q, k, v must be float32, bfloat16 or float16, got ", dt);
+  require(k.scalar_type() == dt && v.scalar_type() == dt, "q, k, v must share a dtype, got ", dt, "/", k.scalar_type(), "/",
+          v.scalar_type());
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
+  require(k.dim() == 4 && v.sizes() == k.sizes() && k.size(0) == B && k.size(2) == N && k.size(3) == D, "k and v must be [", B, ",Hkv,", N,
+          ",", D, "], got ", shape_str(k.sizes()), " and ", shape_str(v.sizes()));
+  const int64_t Hkv = k.size(1);
+  require(Hkv > 0 ? H > 0 && H % Hkv == 0 : H == 0, "the query heads must be a positive multiple of the ", Hkv, " key/value heads, got ", H);
+  require(D > 0, "the head dim must be positive");
+  require(window >= 1, "window must be positive, got ", window);
+  require(sinks >= 0, "sinks must be 0 or more, got ", sinks);
+  require(N <= (1 << 30) && B < (1ll << 31) && H < (1ll << 31), "at most 2^30 positions, got ", shape_str(q.sizes()));
+  if (lengths.defined())
+    require(at::isIntegralType(lengths.scalar_type(), false) && lengths.sizes() == c10::IntArrayRef({B}), "lengths must be an integer [", B,
+            "] tensor, got ", lengths.scalar_type(), " ", shape_str(lengths.sizes()));
+  dsqg_window_shape s = {};
+  s.dtype = dt == at::kFloat ? DSQG_F32 : dt == at::kBFloat16 ? DSQG_BF16 : DSQG_F16;
+  s.B = (int32_t)B; s.H = (int32_t)H; s.Hkv = (int32_t)Hkv; s.N = (int32_t)N; s.D = (int32_t)D;
+  s.window = (int32_t)std::min<int64_t>(window, 1 << 30);
+  s.sinks = (int32_t)std::min<int64_t>(sinks, 1 << 30);
+  s.softmax_scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
+  return s;
+}
+
+// (out, stats); stats is undefined unless asked for.
+std::tuple<Tensor, Tensor> run_window_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& lengths0, int64_t window,
+                                          int64_t sinks, std::optional<double> scale, bool with_stats) {
+  dsqg_window_fwd_args a = {};
+  a.shape = window_shape(q0, k0, v0, lengths0, window, sinks, scale);
+  const c10::Device dev = require_gpu({&q0, &k0, &v0, &lengths0});
+  const c10::OptionalDeviceGuard guard(dev);
+  const Tensor q = window_rows(q0), k = window_rows(k0), v = window_rows(v0);
+  const Tensor lengths = lengths0.defined() ? lengths0.to(at::kLong).contiguous() : lengths0;
+  const Tensor out = token_major(q);
+  const Tensor stats = with_stats ? at::empty({q.size(0), q.size(1), q.size(2), 2}, q.options().dtype(at::kFloat)) : Tensor();
+  a.shape.lengths = static_cast<const int64_t*>(ptr(lengths));
+  a.q = ptr(q); set_strides(a.q_stride, q);
+  a.k = ptr(k); set_strides(a.k_stride, k);
+  a.v = ptr(v); set_strides(a.v_stride, v);
+  a.out = ptr(out); set_strides(a.out_stride, out);
+  a.stats = static_cast<float*>(ptr(stats));
+  check(api.window_fwd(&a, stream_of(dev)), "dsqg_window_fwd");
+  return {out, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor> run_window_bwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& lengths0,
+                                                  const Tensor& out0, const Tensor& stats, const Tensor& dout0, int64_t window,
+                                                  int64_t sinks, std::optional<double> scale) {
+  dsqg_window_bwd_args a = {};
+  a.shape = window_shape(q0, k0, v0, lengths0, window, sinks, scale);
+  const c10::Device dev = require_gpu({&q0, &k0, &v0, &lengths0, &out0, &stats, &dout0});
+  const c10::OptionalDeviceGuard guard(dev);
+  const Tensor q = window_rows(q0), k = window_rows(k0), v = window_rows(v0), out = window_rows(out0);
+  const Tensor dout = window_rows(dout0.to(q.scalar_type()));
+  const Tensor lengths = lengths0.defined() ? lengths0.to(at::kLong).contiguous() : lengths0;
+  const Tensor dq = token_major(q), dk = token_major(k), dv = token_major(v);
+  a.shape.lengths = static_cast<const int64_t*>(ptr(lengths));
+  a.q = ptr(q); set_strides(a.q_stride, q);
+  a.k = ptr(k); set_strides(a.k_stride, k);
+  a.v = ptr(v); set_strides(a.v_stride, v);
+  a.out = ptr(out); set_strides(a.out_stride, out);
+  a.dout = ptr(dout); set_strides(a.dout_stride, dout);
+  a.stats = static_cast<const float*>(ptr(stats));
+  a.dq = ptr(dq); set_strides(a.dq_stride, dq);
+  a.dk = ptr(dk); set_strides(a.dk_stride, dk);
+  a.dv = ptr(dv); set_strides(a.dv_stride, dv);
+  size_t nbytes = 0;
+  check(api.window_bwd_workspace_size(&a.shape, &nbytes), "dsqg_window_bwd_workspace_size");
+  const Tensor ws = at::empty({std::max<int64_t>((int64_t)nbytes, 1)}, q.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = nbytes;
+  check(api.window_bwd(&a, stream_of(dev)), "dsqg_window_bwd");
+  return {dq, dk, dv};
+}
+
+struct WindowFunction : torch::autograd::Function<WindowFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths, int64_t window,
+                        int64_t sinks, std::optional<double> scale) {
+    const auto [out, stats] = run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
+    ctx->save_for_backward({q, k, v, undef(lengths), out, stats});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale ? *scale : 1.0 / std::sqrt((double)q.size(3));
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (at::GradMode::is_enabled())
+      raise(PyExc_RuntimeError, "window_attention has no second derivative: call backward without create_graph");
+    const variable_list s = ctx->get_saved_variables();
+    const auto [dq, dk, dv] = run_window_bwd(s[0], s[1], s[2], s[3], s[4], s[5], g[0], ctx->saved_data["window"].toInt(),
+                                             ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor window(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths, int64_t window, int64_t sinks,
+              std::optional<double> scale) {
+  py::gil_scoped_release nogil;
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->_fw_grad(0).defined()) raise(PyExc_RuntimeError, "window_attention has no forward-mode derivative");
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return std::get<0>(run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, false));
+  window_shape(q, k, v, undef(lengths), window, sinks, scale);  // (refusals come before the graph is touched)
+  return WindowFunction::apply(q, k, v, lengths, window, sinks, scale);
+}
+
+std::tuple<Tensor, Tensor> window_fwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths, int64_t window,
+                                         int64_t sinks, std::optional<double> scale) {
+  py::gil_scoped_release nogil;
+  return run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> window_bwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths,
+                                                 const Tensor& out, const Tensor& stats, const Tensor& dout, int64_t window,
+                                                 int64_t sinks, std::optional<double> scale) {
+  py::gil_scoped_release nogil;
+  return run_window_bwd(q, k, v, undef(lengths), out, stats, dout, window, sinks, scale);
+}
+
 // ---- Drafted tokens and sampling. ----------------------------------------------------------------------------------
 
 // Integers [B,T] as the kernels read them (unit inner stride), or of one row for all (stride 0): [T].
@@ -1199,6 +1345,9 @@ void init(const py::dict& addresses, const py::object& library_error) {
   get(api.paged_read, "dsqg_paged_read");
   get(api.paged_decode_workspace_size, "dsqg_paged_decode_workspace_size");
   get(api.paged_decode, "dsqg_paged_decode");
+  get(api.window_fwd, "dsqg_window_fwd");
+  get(api.window_bwd_workspace_size, "dsqg_window_bwd_workspace_size");
+  get(api.window_bwd, "dsqg_window_bwd");
   get(api.paged_tree_workspace_size, "dsqg_paged_tree_workspace_size");
   get(api.paged_tree, "dsqg_paged_tree");
   get(api.tree_accept, "dsqg_tree_accept");
@@ -1221,6 +1370,9 @@ PYBIND11_MODULE(_dsqg_host, m) {
   m.def("paged_write", &paged_write);
   m.def("paged_read", &paged_read);
   m.def("paged_decode", &paged_decode);
+  m.def("window", &window);
+  m.def("window_fwd", &window_fwd_op);
+  m.def("window_bwd", &window_bwd_op);
   m.def("paged_tree", &paged_tree);
   m.def("tree_accept", &tree_accept);
   m.def("sample", &sample);

@@ -1,0 +1,201 @@
+// Attention within a window and its sinks, forward (gfx950).
+//
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j     over the positions j that i sees (dsqg_window.hpp)
+//
+// A workgroup takes 128 queries of a head, a wave 32 of them, and goes once over the tiles of keys and values that any of
+// them sees, with a running maximum and sum: S^T = K Q^T, weights, O^T += V^T P^T, the weights staying in registers from
+// one product to the other.  Keys and values are loaded a tile ahead and lie in LDS twice, so that a tile costs one
+// barrier.  Only tiles at the window's two ends (and the sinks') compare positions.
+//
+// Weights are rounded once to the 16-bit type before they multiply the values (2^-8 of each in bfloat16, 2^-11 in float16); float32
+// operands are not rounded.  Scores, the maximum, the sum and the output's sums are fp32.  For the backward a query's
+// reference exponent m and 1 / sum are kept apart, for m may be too large to hold the sum's logarithm.
+#include "dsqg_window.hpp"
+
+namespace dsqg {
+namespace {
+
+template <int T> constexpr int rows_of_tile() { return T == DSQG_F32 ? 32 : 64; }
+
+template <int T, int D>
+__global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
+  using X = Tile<T, D>;
+  constexpr int RT = rows_of_tile<T>(), KB = RT / 32, TB = X::bytes(RT);
+  static_assert(4 * TB >= 4 * 32 * X::RV * X::O::size, "the waves' output rows fit the tiles");
+  __shared__ __align__(16) char lds[2][2][TB];  // [which tile][keys, values]
+  __shared__ int odd[2];                        // which tile's values hold infinities or NaN, plus one
+
+  // Blocks that read the same keys, the heads of a key/value head, follow each other; the longest come first.
+  const int block = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int g = block % p.G, rest = block / p.G;
+  const int at = p.blocks - 1 - rest % p.blocks, bk = rest / p.blocks;
+  const int b = bk / p.Hkv, hk = bk - b * p.Hkv, head = hk * p.G + g;
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = l & 31, h = l >> 5;
+  const int length = window_length(p, b);
+  const int q0 = at * kCols, i0 = q0 + 32 * wave, i = i0 + c;
+  const char* const kh = p.k.at + b * p.k.b + hk * p.k.h;
+  const char* const vh = p.v.at + b * p.v.b + hk * p.v.h;
+  const WindowSpan span = q0 < length ? keys_of<RT>(p, q0, min(q0 + kCols, length) - 1) : WindowSpan{0, 0, 0};
+
+  u32x4_t q[X::KS];
+  {
+    const char* const row = p.q.at + b * p.q.b + head * p.q.h + (long long)i * p.q.n;
+#pragma unroll
+    for (int s = 0; s < X::KS; ++s) {
+      q[s] = u32x4_t{0u, 0u, 0u, 0u};
+      if (i < length) q[s] = *reinterpret_cast<const u32x4_t*>(row + (2 * X::E * s + X::E * h) * X::O::size);
+    }
+  }
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+
+  Stage<T, D, RT> sk, sv;
+  auto load = [&](int t) {
+    sk.load(kh, p.k.n, span.tile(t) * RT, length);
+    sv.load(vh, p.v.n, span.tile(t) * RT, length);
+  };
+  // Whether some of the workgroup's queries do not see some of tile t.
+  auto edge = [&](int t) {
+    const int j0 = span.tile(t) * RT;
+    return j0 + RT - 1 > q0 || (q0 + kCols - 1 - j0 >= p.window && j0 + RT > p.sinks);
+  };
+  auto store = [&](int t) {
+    sk.store(lds[t & 1][0]);
+    if (edge(t) && sv.clean()) odd[t & 1] = t + 1;
+    sv.store(lds[t & 1][1]);
+  };
+
+  Acc<T, D> o;
+#pragma unroll
+  for (int d = 0; d < X::DB; ++d) o[d] = zero_tile();
+  float m = -INFINITY, sum = 0.f;
+  bool large = false;
+  // The largest weight is 2^lift: float16 weights far below it stay clear of the type's subnormal numbers.
+  constexpr float lift = T == DSQG_F16 ? 14.f : 0.f;
+  const float far = p.scale2 < 0.f ? INFINITY : -INFINITY;  // a score that is no maximum
+
+  __syncthreads();
+  if (span.n > 0) {
+    load(0);
+    store(0);
+    if (span.n > 1) load(1);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t = 0; t < span.n; ++t) {
+    const int j0 = span.tile(t) * RT;
+    const char* const kt = lds[t & 1][0];
+    const char* const vt = lds[t & 1][1];
+    // Nothing of it is seen by the wave's queries / all of it is.
+    const bool none = j0 > i0 + 31 || (j0 + RT <= i0 - p.window + 1 && j0 >= p.sinks);
+    const bool all = j0 + RT - 1 <= i0 && (i0 + 31 - j0 < p.window || j0 + RT <= p.sinks);
+    if (!none) {
+      f32x16_t s[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        s[kb] = zero_tile();
+#pragma unroll
+        for (int e = 0; e < X::KS; ++e) s[kb] = mma<T>(row_frag<T, D>(kt + 32 * kb * X::RV * X::O::size, l, e), q[e], s[kb]);
+      }
+      auto sees = [&](int kb, int row) {  // (this lane's query)
+        const int back = i - (j0 + 32 * kb + row);
+        return back >= 0 && (back < p.window || j0 + 32 * kb + row < p.sinks);
+      };
+      uint32_t hide[KB] = {};
+      if (!all) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool gone = !sees(kb, reg_row<T>(r, h));
+            hide[kb] |= (gone ? 1u : 0u) << r;
+            s[kb][r] = gone ? far : s[kb][r];
+          }
+      }
+      float mx = s[0][0];
+      if (p.scale2 < 0.f) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fminf(mx, s[kb][r]);
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+      }
+      mx = mx == far ? -INFINITY : mx * p.scale2 - lift;  // (a scale of zero makes no NaN of what is not seen)
+      mx = xor32_pair_max(mx);
+      if (__any(mx > m)) {
+        const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        large = __any(fabsf(mn) >= kLarge && mn != -INFINITY);
+        sum *= a;
+#pragma unroll
+        for (int d = 0; d < X::DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= a;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        float w[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = exponent(s[kb][r], p.scale2, ref, large);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(w[r]);
+        if (!all) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) w[r] = (hide[kb] >> r) & 1 ? 0.f : w[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += w[r];
+        Weights<T> f;
+        pack<T>(w, f);
+        const char* const rows = vt + 32 * kb * X::RV * X::O::size;
+        contract<T, D>(o, rows, l, f);
+        if (odd[t & 1] == t + 1)
+          add_odd<T, D>(o, vh + (j0 + 32 * kb) * p.v.n, p.v.n, length - j0 - 32 * kb, l, [&](int row) { return sees(kb, row); });
+      }
+    }
+    if (t + 1 < span.n) {
+      store(t + 1);
+      if (t + 2 < span.n) load(t + 2);
+    }
+    __syncthreads();
+  }
+
+  sum = xor32_pair_sum(sum);
+  const bool live = i < length && sum != 0.f;
+  store_columns<T, D>(o, 1.f / sum, live, lds[0][0] + wave * 32 * X::RV * X::O::size,
+                      p.out.at + b * p.out.b + head * p.out.h + i0 * p.out.n, p.out.n, p.N - i0, l);
+  if (p.stats && h == 0 && i < p.N)
+    p.stats[((long long)b * p.Hkv * p.G + head) * p.N + i] = live ? make_float2(m, 1.f / sum) : make_float2(INFINITY, 0.f);
+}
+
+template <int T, int D>
+hipError_t launch(const WindowParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((window_fwd_kernel<T, D>), dim3((unsigned)((long long)p.B * p.Hkv * p.G * p.blocks)), dim3(kBlock), 0, st, p);
+  return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_dim(const WindowParams& p, hipStream_t st) {
+  switch (p.D) {
+    case 32: return launch<T, 32>(p, st);
+    case 64: return launch<T, 64>(p, st);
+    case 80: return launch<T, 80>(p, st);
+    case 96: return launch<T, 96>(p, st);
+    default: return launch<T, 128>(p, st);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_window_fwd(const WindowParams& p, int dtype, hipStream_t st) {
+  if (dtype == DSQG_F32) return launch_dim<DSQG_F32>(p, st);
+  if (dtype == DSQG_BF16) return launch_dim<DSQG_BF16>(p, st);
+  return launch_dim<DSQG_F16>(p, st);
+}
+
+}  // namespace dsqg

@@ -1,7 +1,7 @@
 """torch custom ops over the C ABI: ``dwarf::dsqg_fwd``, ``dwarf::dsqg_fwd_qkv``, ``dwarf::dsqg_bwd``,
 ``dwarf::dsqg_decode``, the interference pool ``dwarf::pool_gate_fwd`` / ``_bwd``, and the paged cache's
 ``dwarf::paged_kv_write``, ``dwarf::paged_kv_read`` and ``dwarf::paged_decode``; ``dwarf::paged_tree``,
-``dwarf::tree_accept`` and ``dwarf::sample_tokens``.
+``dwarf::window_fwd`` / ``_bwd``, ``dwarf::tree_accept`` and ``dwarf::sample_tokens``.
 
 The ops take device tensors, pass raw pointers, element strides and the current HIP stream
 to libdsqg_hip.so through ctypes, and allocate their outputs (and the backward workspace) with
@@ -717,6 +717,51 @@ def paged_decode(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], k_
 @paged_decode.register_fake
 def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, softmax_scale):
     return q.new_empty(q.shape)
+
+
+# ------------------------------------------------------------------------------------------
+# Attention within a window
+# ------------------------------------------------------------------------------------------
+
+@torch.library.custom_op("dwarf::window_fwd", mutates_args=())
+def window_fwd(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: int, sinks: int,
+               softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
+    """out [B,H,N,D] (token-major storage) and, for the backward, stats [B,H,N,2] fp32."""
+    return _lib.host().window_fwd(q, k, v, lengths, window, sinks, softmax_scale)
+
+
+@window_fwd.register_fake
+def _(q, k, v, lengths, window, sinks, softmax_scale):
+    B, H, N, D = q.shape
+    return q.new_empty((B, N, H, D)).permute(0, 2, 1, 3), q.new_empty((B, H, N, 2), dtype=torch.float32)
+
+
+@torch.library.custom_op("dwarf::window_bwd", mutates_args=())
+def window_bwd(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], out: Tensor, stats: Tensor, dout: Tensor,
+               window: int, sinks: int, softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv), token-major storage; out and stats are the forward's."""
+    return _lib.host().window_bwd(q, k, v, lengths, out, stats, dout, window, sinks, softmax_scale)
+
+
+@window_bwd.register_fake
+def _(q, k, v, lengths, out, stats, dout, window, sinks, softmax_scale):
+    return tuple(t.new_empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3])).permute(0, 2, 1, 3) for t in (q, k, v))
+
+
+def _window_setup_context(ctx, inputs, output):
+    q, k, v, lengths, ctx.window, ctx.sinks, ctx.scale = inputs
+    out, stats = output
+    ctx.save_for_backward(q, k, v, lengths, out, stats)
+    ctx.mark_non_differentiable(stats)
+
+
+def _window_backward(ctx, dout, _dstats):
+    q, k, v, lengths, out, stats = ctx.saved_tensors
+    dq, dk, dv = window_bwd(q, k, v, lengths, out, stats, dout, ctx.window, ctx.sinks, ctx.scale)
+    return dq, dk, dv, None, None, None, None
+
+
+torch.library.register_autograd("dwarf::window_fwd", _window_backward, setup_context=_window_setup_context)
 
 
 # ------------------------------------------------------------------------------------------

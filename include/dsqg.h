@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DSQG_ABI_VERSION 7
+#define DSQG_ABI_VERSION 8
 #define DSQG_MAX_OFFSETS 64
 
 /* Same type as hipStream_t; NULL is the null stream. */
@@ -415,6 +415,59 @@ typedef struct {
 
 int dsqg_paged_decode_workspace_size(const dsqg_paged_decode_args* args, size_t* bytes);
 int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
+
+/* Softmax attention within a window, with sinks (the full-attention layer of train/train_2048_condU.py:210-245 sees all
+ * earlier positions): position i of a sequence sees position j <= i if i - j < window or j < sinks.
+ *
+ *     out[b,h,i] = sum_j softmax_j(softmax_scale * q[b,h,i] . k[b,hk,j]) v[b,hk,j],    hk = h / (H / Hkv)
+ *
+ * q, out and their gradients are [B,H,N,D], k, v and theirs [B,Hkv,N,D], H a multiple of Hkv.  With lengths given, rows
+ * i >= lengths[b] are not there: nothing sees them, and their outputs and gradients are zeros.  D is one of
+ * dsqg_supported_head_dims (EUNSUPPORTED otherwise), window at least 1, sinks at least 0, N at most 2^30 and B * H * (N / 128 +
+ * 64) less than 2^31 (EUNSUPPORTED).  Every tensor has unit inner stride, strides {b, h, n} and a base that keep rows
+ * 16-byte aligned, and a row stride of at least D elements and less than 2^24 bytes.
+ *
+ * stats [B,H,N,2] (float, contiguous, 8-byte aligned; the forward's may be NULL) holds, for the backward, each query's
+ * reference exponent and the inverse of its weights' sum.  Scores and sums are fp32, in an order that does not change
+ * between calls; the weights and, in the backward, their gradients are rounded once to a 16-bit dtype before they multiply
+ * rows.  A row that a query does not see does not reach its output, whatever it holds, nor a row of a query that does not
+ * see a key that key's gradients. */
+typedef struct {
+    int32_t dtype;             /* DSQG_F32, DSQG_BF16 or DSQG_F16 */
+    int32_t B, H, Hkv, N, D;
+    int32_t window, sinks;
+    float softmax_scale;
+    const int64_t* lengths;    /* [B] or NULL */
+} dsqg_window_shape;
+
+typedef struct {
+    dsqg_window_shape shape;
+    const void* q;  int64_t q_stride[3];
+    const void* k;  int64_t k_stride[3];
+    const void* v;  int64_t v_stride[3];
+    void* out;      int64_t out_stride[3];
+    float* stats;
+} dsqg_window_fwd_args;
+
+int dsqg_window_fwd(const dsqg_window_fwd_args* args, dsqg_stream_t stream);
+
+typedef struct {
+    dsqg_window_shape shape;
+    const void* q;     int64_t q_stride[3];
+    const void* k;     int64_t k_stride[3];
+    const void* v;     int64_t v_stride[3];
+    const void* out;   int64_t out_stride[3];
+    const void* dout;  int64_t dout_stride[3];
+    const float* stats;
+    void* dq;  int64_t dq_stride[3];
+    void* dk;  int64_t dk_stride[3];
+    void* dv;  int64_t dv_stride[3];
+    void* workspace;           /* 256-byte aligned */
+    size_t workspace_bytes;
+} dsqg_window_bwd_args;
+
+int dsqg_window_bwd_workspace_size(const dsqg_window_shape* shape, size_t* bytes);
+int dsqg_window_bwd(const dsqg_window_bwd_args* args, dsqg_stream_t stream);
 
 /* The accepted path of a tree of drafted tokens (no counterpart in the reference).  Node i of sequence b has
  * the token tokens[b,i] and hangs on the node parents[b,i] (parents_stride 0: one tree for all); picks[b,i] is the
