@@ -449,8 +449,15 @@ class PagedKVCache:
                        self.page_table, pos, counts=counts, **self._state())
         return counts
 
-    def step(self, q: Tensor, k_new: Tensor, v_new: Tensor, softmax_scale: Optional[float] = None) -> Tensor:
-        """Output [B,H*G,D] of one new token per sequence at its position, which advances."""
+    def step(self, q: Tensor, k_new: Tensor, v_new: Tensor, softmax_scale: Optional[float] = None,
+             window: Optional[int] = None, sinks: int = 0) -> Tensor:
+        """Output [B,H*G,D] of one new token per sequence at its position, which advances.  With a window it sees the
+        last ``window`` positions, its own among them, and those below ``sinks``."""
+        if window is not None:
+            out = self.tree_step(q.unsqueeze(2), k_new.unsqueeze(2), v_new.unsqueeze(2), window=window, sinks=sinks,
+                                 softmax_scale=softmax_scale)[:, :, 0]
+            self.pos += self.pos >= 0
+            return out
         dt = self.dtype
         out = paged_decode_step(q.detach().to(dt), k_new.detach().to(dt), v_new.detach().to(dt), self.k_pages,
                                 self.v_pages, self.page_table, self.pos, softmax_scale=softmax_scale,

@@ -19,7 +19,8 @@ temperature-scaled nucleus (top-p) sampling.
 
 The full-attention layer's cache is a flat tensor that every step attends whole, in torch, or, asked for
 with ``paged=True`` or an 8-bit ``kv_dtype``, a ``PagedKVCache``: the step then reads the rows in use only,
-in one HIP kernel, and the cache may be 8 bits wide.
+in one HIP kernel, and the cache may be 8 bits wide.  The layer may see a window and a few first tokens alone
+(``full_attn_window``), and tokens may be drawn from given random numbers with top-k and min-p (``generate``).
 """
 
 from __future__ import annotations
@@ -30,17 +31,27 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
-from .api import PagedKVCache
+from . import _lib
+from .api import PagedKVCache, sample_tokens, window_attention
 from .modules import FFN, DSQGBlock, Linear
 
 
 class FullCausalAttention(nn.Module):
     """train/train_2048_condU.py:210-245: softmax attention over all earlier tokens, with the
     DSQG layers' output gate.  ``prefill`` / ``step`` keep its K/V rows in a preallocated
-    cache for generation."""
+    cache for generation.  With a ``window`` (no counterpart in the reference) a token sees the last
+    ``window`` tokens and the first ``sinks``, on the HIP kernels (``window_attention``: head dims 32, 64, 80, 96
+    and 128), and dropout is on the layer's output alone, as in the DSQG layers."""
 
-    def __init__(self, embedding_dim: int, num_heads: int, dropout: float = 0.1):
+    def __init__(self, embedding_dim: int, num_heads: int, dropout: float = 0.1,
+                 window: Optional[int] = None, sinks: int = 0):
         super().__init__()
+        assert window is None or window >= 1, f"window must be positive (or None), got {window}"
+        assert sinks >= 0, f"sinks must be 0 or more, got {sinks}"
+        assert window is None or embedding_dim // num_heads in _lib.supported_head_dims(), \
+            f"head dim {embedding_dim // num_heads} is none of {_lib.supported_head_dims()}"
+        self.window = window
+        self.sinks = sinks
         self.embedding_dim = embedding_dim
         self.num_heads = num_heads
         self.head_dim = embedding_dim // num_heads
@@ -68,6 +79,9 @@ class FullCausalAttention(nn.Module):
             cache.k[:, :, :N] = k
             cache.v[:, :, :N] = v
             cache.pos.fill_(N)
+        if self.window is not None:
+            out = window_attention(q, k, v, self.window, self.sinks)
+            return self._finish(out.permute(0, 2, 1, 3).reshape(B, N, E), x)
         # 16-bit inputs are attended in fp32: it keeps 16-bit batched products with transposed
         # operands (the math path of scaled_dot_product_attention) out of the layer.
         up = (lambda t: t.float()) if q.dtype in (torch.float16, torch.bfloat16) else (lambda t: t)
@@ -84,13 +98,17 @@ class FullCausalAttention(nn.Module):
         B, E = x_t.shape
         q, k, v = self._heads(self.qkv_proj(x_t).unsqueeze(1), B, 1)
         if isinstance(cache, PagedKVCache):
-            out = cache.step(q[:, :, 0], k[:, :, 0], v[:, :, 0])
+            out = cache.step(q[:, :, 0], k[:, :, 0], v[:, :, 0], window=self.window, sinks=self.sinks)
             return self._finish(out.reshape(B, E), x_t)
         slot = cache.pos[:1]
         cache.k.index_copy_(2, slot, k)
         cache.v.index_copy_(2, slot, v)
         T = cache.k.shape[2]
-        mask = (torch.arange(T, device=x_t.device) <= slot).view(1, 1, 1, T)
+        at = torch.arange(T, device=x_t.device)
+        mask = at <= slot
+        if self.window is not None:
+            mask = mask & ((at > slot - self.window) | (at < self.sinks))
+        mask = mask.view(1, 1, 1, T)
         out = F.scaled_dot_product_attention(q.float(), cache.k.float(), cache.v.float(),
                                              attn_mask=mask)
         cache.pos += 1
@@ -113,11 +131,12 @@ KVCache = Union[_KVCache, PagedKVCache]
 class FullAttentionBlock(nn.Module):
     """train/train_2048_condU.py:304-315: pre-norm block around FullCausalAttention + FFN."""
 
-    def __init__(self, embedding_dim: int, num_heads: int, ffn_dim: int, dropout: float = 0.1):
+    def __init__(self, embedding_dim: int, num_heads: int, ffn_dim: int, dropout: float = 0.1,
+                 window: Optional[int] = None, sinks: int = 0):
         super().__init__()
         self.norm1 = nn.LayerNorm(embedding_dim)
         self.norm2 = nn.LayerNorm(embedding_dim)
-        self.attn = FullCausalAttention(embedding_dim, num_heads, dropout)
+        self.attn = FullCausalAttention(embedding_dim, num_heads, dropout, window, sinks)
         self.ffn = FFN(embedding_dim, ffn_dim, dropout)
 
     def forward(self, x: Tensor, cache: Optional[KVCache] = None) -> Tensor:
@@ -146,12 +165,14 @@ class FullAttentionBlock(nn.Module):
 
 class CondMTransformer(nn.Module):
     """train/train_2048_condU.py:320-365 with the DSQG blocks on the HIP kernels.  ``offsets``
-    (default: the 44-offset table) selects the DSQG layers' offset table."""
+    (default: the 44-offset table) selects the DSQG layers' offset table; ``full_attn_window`` and ``full_attn_sinks``
+    narrow the full-attention layer (``FullCausalAttention``)."""
 
     def __init__(self, vocab_size: int, embedding_dim: int, num_layers: int, num_heads: int,
                  ffn_dim: int, seq_len: int, full_attn_layer: int = 5,
                  interference_interval: int = 3, dropout: float = 0.1,
-                 offsets: Optional[Sequence[int]] = None):
+                 offsets: Optional[Sequence[int]] = None, full_attn_window: Optional[int] = None,
+                 full_attn_sinks: int = 0):
         super().__init__()
         self.seq_len = seq_len
         self.embedding = nn.Embedding(vocab_size, embedding_dim)
@@ -161,7 +182,8 @@ class CondMTransformer(nn.Module):
         blocks = []
         for i in range(num_layers):
             if i == full_attn_layer:
-                blocks.append(FullAttentionBlock(embedding_dim, num_heads, ffn_dim, dropout))
+                blocks.append(FullAttentionBlock(embedding_dim, num_heads, ffn_dim, dropout,
+                                                 full_attn_window, full_attn_sinks))
             else:
                 blocks.append(DSQGBlock(
                     embedding_dim, num_heads, ffn_dim, seq_len, dropout=dropout,
@@ -242,13 +264,23 @@ class CondMTransformer(nn.Module):
     @torch.no_grad()
     def generate(self, idx: Tensor, max_new: int, temperature: float = 1.0, top_p: float = 0.9,
                  generator: Optional[torch.Generator] = None, use_graph: bool = True,
-                 paged: bool = False, kv_dtype: Optional[torch.dtype] = None) -> Tensor:
+                 paged: bool = False, kv_dtype: Optional[torch.dtype] = None, top_k: int = 0,
+                 min_p: float = 0.0, uniforms: Optional[Tensor] = None) -> Tensor:
         """Append ``max_new`` sampled tokens to idx [B, N]; returns [B, N + max_new].
 
         After the prefill, the first step runs eagerly and the next ones replay it from a HIP
         graph (``use_graph``); sampling stays outside the graph.  ``paged`` and ``kv_dtype`` choose the
         full-attention layer's cache (``new_cache``; a paged one refuses head dims without kernels).
+        With ``top_k``, ``min_p`` or ``uniforms`` [B, max_new] (numbers from [0, 1), one for each token; drawn
+        from ``generator`` where they are not given) tokens come from ``sample_tokens``, one kernel, else from the
+        reference's softmax, sort and multinomial.
         """
+        kernel = uniforms is not None or top_k > 0 or min_p > 0
+        if kernel and uniforms is None:
+            uniforms = torch.rand((idx.shape[0], max_new), generator=generator, device=idx.device)
+        if uniforms is not None:
+            assert tuple(uniforms.shape) == (idx.shape[0], max_new), \
+                f"uniforms must be {(idx.shape[0], max_new)}, got {tuple(uniforms.shape)}"
         was_training = self.training
         self.eval()
         ids = idx
@@ -256,7 +288,7 @@ class CondMTransformer(nn.Module):
         logits = None
         graph = side = None
         tok_in = logits_out = None
-        for _ in range(max_new):
+        for i in range(max_new):
             n = ids.shape[1]
             if n <= self.seq_len:
                 if cache is None:
@@ -265,7 +297,10 @@ class CondMTransformer(nn.Module):
                 # else: the last token's logits came from the previous step
             else:  # past the position table: the reference's sliding-window recomputation
                 logits = self.forward(ids[:, -self.seq_len:])[:, -1]
-            nxt = _sample(logits.float(), temperature, top_p, generator)
+            if kernel:
+                nxt = sample_tokens(logits, uniforms[:, i], temperature if temperature > 0.01 else 0.0, top_k, top_p, min_p)
+            else:
+                nxt = _sample(logits.float(), temperature, top_p, generator)
             ids = torch.cat([ids, nxt.unsqueeze(1)], dim=1)
             if ids.shape[1] > self.seq_len:
                 continue
