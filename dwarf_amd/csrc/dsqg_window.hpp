@@ -39,13 +39,20 @@ struct WindowParams {
   WindowRows q, k, v, out, dout, dq, dk, dv;
   float2* stats;               // [B, H, N]: the weights' reference exponent and 1 / sum (forward: or null)
   float* delta;                // [B, H, N]: dout . out
-  int blocks;                  // column blocks (of kCols) of a head
-  // dk/dv: key blocks below `split` hold sinks whose far queries are other workgroups': `far` of them for each.
-  int split, far;
-  float* part;                 // [B, Hkv, split, 1 + far, 2, kCols, D]
+  int waves, blocks;           // waves of a workgroup, 32 queries each; query blocks of a head
+  // dk/dv: keys of a block, and blocks; those below `split` hold sinks whose far queries are other workgroups': `far` of
+  // them for each.
+  int kcols, kblocks, split, far;
+  float* part;                 // [B, Hkv, split, 1 + far, 2, kcols, D]
 };
 
-constexpr int kCols = 128;  // of a workgroup: 32 a wave
+// Whether a query workgroup may have eight waves rather than four: the rows' loads and stores to LDS are shared by twice the
+// queries, the barriers by twice the waves.  Rows of 16 bits above 64 elements gain (D = 128 at B1 H16 Hkv4 N16384 window 1024:
+// dq 364 us to 426, forward 262 to 268), shorter ones lose (D = 32 at B8 H8 N2048 window 256: 39.5 to 35.2 and 39.1 to 32.5).
+constexpr bool may_be_wide(int T, int D) { return T != DSQG_F32 && D > 64; }
+
+// Pairs of waves of a dk/dv workgroup, of 32 keys each: four, whose tiles and operands fit LDS but at 128 elements of float32.
+constexpr int key_pairs(int T, int D) { return T == DSQG_F32 && D > 96 ? 2 : 4; }
 
 __device__ __forceinline__ int window_length(const WindowParams& p, int b) {
   return p.lengths ? (int)max(0ll, min((long long)p.N, p.lengths[b])) : p.N;
@@ -77,17 +84,29 @@ __device__ __forceinline__ f32x16_t zero_tile() {
   return z;
 }
 
+// A tile's rows in LDS.  16 bits: 16-byte pieces in rows of a power of two of them, piece i of row r in slot i ^ f(r), so that
+// neither reads of one piece of sixteen rows (row_frag) nor of four pieces of four rows (col_frag) meet in a bank: with rows
+// padded by a piece instead the latter took four times their cycles, half of all of LDS's.  float32, which the matrix
+// instructions bound by far: rows padded by a piece.
 template <int T, int D>
 struct Tile {
   using O = Op<T>;
   static constexpr int E = O::E;
-  static constexpr int RV = D + E;               // LDS row stride in elements (a row and 16 bytes)
+  static constexpr int SLOTS = D <= 32 ? 4 : D <= 64 ? 8 : 16;
+  static constexpr int RB = T == DSQG_F32 ? (D + E) * 4 : SLOTS * 16;  // bytes of a row
   static constexpr int KS = D / (2 * E);         // fragments of a row
   static constexpr int DB = (D + 31) / 32;       // 32-wide blocks of a row
   static constexpr int C = 16 / E;               // fragments of a block of 32 rows as an operand
   static constexpr int PPR = D * O::size / 16;   // 16-byte pieces of a row
-  // Bytes of `rows` staged rows (the transposed reads of the last block may run past a row of D = 80).
-  static constexpr int bytes(int rows) { return rows * RV * O::size + (D % 32 ? 64 : 0); }
+  // Bytes of `rows` staged rows (float32: the reads of the last block may run past a row of D = 80).
+  static constexpr int bytes(int rows) { return rows * RB + (T == DSQG_F32 && D % 32 ? 64 : 0); }
+  // Which slots a row's pieces are in: f(row).
+  static __device__ __forceinline__ int flip(int row) {
+    if constexpr (T == DSQG_F32) return 0;
+    else if constexpr (SLOTS == 4) return (row >> 2) & 3;
+    else if constexpr (SLOTS == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return ((row & 3) << 2) | ((row >> 2) & 3);
+  }
 };
 
 template <int T, int D> using Acc = f32x16_t[Tile<T, D>::DB];  // a wave's [D x 32] sums
@@ -101,26 +120,31 @@ __device__ __forceinline__ int operand_row(int l) {
   else return (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1);
 }
 
-// Fragment s of the A operand whose rows begin at `rows` (LDS, row-major).
+// Fragment s of the A operand whose rows, 32 from a multiple of 32 on, begin at `rows` (LDS).
 template <int T, int D>
 __device__ __forceinline__ u32x4_t row_frag(const char* rows, int l, int s) {
   using X = Tile<T, D>;
-  return *reinterpret_cast<const u32x4_t*>(rows + (operand_row<T>(l) * X::RV + s * 2 * X::E + X::E * (l >> 5)) * X::O::size);
+  const int row = operand_row<T>(l);
+  return *reinterpret_cast<const u32x4_t*>(rows + row * X::RB + ((2 * s) ^ ((l >> 5) ^ X::flip(row))) * 16);
 }
 
-// Fragment c of the A operand whose rows are the elements 32 d + l % 32 and whose contraction runs over the tile's rows.
+// Fragment c of the A operand whose rows are the elements 32 d + l % 32 and whose contraction runs over those rows.
 template <int T, int D>
 __device__ __forceinline__ u32x4_t col_frag(const char* rows, int l, int c, int d) {
   using X = Tile<T, D>;
   if constexpr (T == DSQG_F32) {
-    const float* t = reinterpret_cast<const float*>(rows) + (8 * c + 4 * (l >> 5)) * X::RV + 32 * d + (l & 31);
+    const float* t = reinterpret_cast<const float*>(rows + (8 * c + 4 * (l >> 5)) * X::RB) + 32 * d + (l & 31);
     u32x4_t f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint(t[e * X::RV]);
+    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint(t[e * (X::RB / 4)]);
     return f;
   } else {
-    const bf16_t* t = reinterpret_cast<const bf16_t*>(rows) + (16 * c + 8 * (l >> 5) + ((l & 15) >> 2)) * X::RV + 32 * d + (l & 16) + 4 * (l & 3);
-    const uint2 a = __builtin_bit_cast(uint2, lds_read_tr16(t)), b = __builtin_bit_cast(uint2, lds_read_tr16(t + 4 * X::RV));
+    const int row = 8 * (l >> 5) + ((l & 15) >> 2), piece = ((l & 16) >> 3) | ((l & 3) >> 1);
+    auto at = [&](int q) {
+      return reinterpret_cast<const bf16_t*>(rows + (row + 4 * q) * X::RB + ((4 * d) ^ (piece ^ X::flip(row + 4 * q))) * 16 + 8 * (l & 1) +
+                                             16 * c * X::RB);
+    };
+    const uint2 a = __builtin_bit_cast(uint2, lds_read_tr16(at(0))), b = __builtin_bit_cast(uint2, lds_read_tr16(at(1)));
     return u32x4_t{a.x, a.y, b.x, b.y};
   }
 }
@@ -147,11 +171,11 @@ __device__ __forceinline__ constexpr int reg_row(int r, int h) {
   return 2 * E * (r / E) + E * h + r % E;
 }
 
-// Rows of a tile on their way from memory to LDS: every thread of the workgroup has the same pieces of each tile.
-template <int T, int D, int RT>
+// Rows of a tile on their way from memory to LDS: every one of the workgroup's NT threads has the same pieces of each tile.
+template <int T, int D, int RT, int NT = kBlock>
 struct Stage {
   using X = Tile<T, D>;
-  static constexpr int U = (RT * X::PPR + kBlock - 1) / kBlock;
+  static constexpr int U = (RT * X::PPR + NT - 1) / NT;
   u32x4_t x[U];
   // Rows `row0` on of a head's rows; those from `length` on are zeros.  (Row strides are below 2^24 bytes.)
   __device__ __forceinline__ void load(const char* head, long long stride, int row0, int length) {
@@ -160,16 +184,16 @@ struct Stage {
                                                                        n > 0 ? (n - 1) * (int)stride + D * X::O::size : 0, 0x00020000);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = threadIdx.x + u * kBlock, row = e / X::PPR;
+      const int e = threadIdx.x + u * NT, row = e / X::PPR;
       x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, row * (int)stride + (e - row * X::PPR) * 16, 0, 0);
     }
   }
   __device__ __forceinline__ void store(char* rows) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = threadIdx.x + u * kBlock, row = e / X::PPR;
-      if (RT * X::PPR % kBlock == 0 || row < RT)
-        *reinterpret_cast<u32x4_t*>(rows + row * X::RV * X::O::size + (e - row * X::PPR) * 16) = x[u];
+      const int e = threadIdx.x + u * NT, row = e / X::PPR;
+      if (RT * X::PPR % NT == 0 || row < RT)
+        *reinterpret_cast<u32x4_t*>(rows + row * X::RB + ((e - row * X::PPR) ^ X::flip(row)) * 16) = x[u];
     }
   }
   // Puts zeros in the place of infinities and NaN, which times the weight of a column that does not see them would be no
@@ -192,17 +216,41 @@ struct Stage {
   }
 };
 
-// acc[d] += A^T w over the 32 rows at `rows`.
+// acc[d] += A^T w over the 32 rows at `rows`: each block's fragments are on their way while the one before is multiplied.
 template <int T, int D>
 __device__ __forceinline__ void contract(Acc<T, D>& acc, const char* rows, int l, const Weights<T>& w) {
   using X = Tile<T, D>;
+  u32x4_t f[2][X::C];
 #pragma unroll
-  for (int d = 0; d < X::DB; ++d)
+  for (int c = 0; c < X::C; ++c) f[0][c] = col_frag<T, D>(rows, l, c, 0);
 #pragma unroll
-    for (int c = 0; c < X::C; ++c) {
-      acc[d] = mma<T>(col_frag<T, D>(rows, l, c, d), w[c], acc[d]);
-      if (c == X::C - 1) __builtin_amdgcn_sched_barrier(0);
+  for (int d = 0; d < X::DB; ++d) {
+    if (d + 1 < X::DB) {
+#pragma unroll
+      for (int c = 0; c < X::C; ++c) f[(d + 1) & 1][c] = col_frag<T, D>(rows, l, c, d + 1);
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < X::C; ++c) acc[d] = mma<T>(f[d & 1][c], w[c], acc[d]);
+  }
+}
+
+// The scores of the 32 rows at `rows` with the columns in b.
+template <int T, int D>
+__device__ __forceinline__ f32x16_t scores(const char* rows, int l, const u32x4_t (&b)[Tile<T, D>::KS]) {
+  using X = Tile<T, D>;
+  constexpr int AHEAD = T == DSQG_F32 ? 4 : X::KS;  // (all of a row's fragments, 32 registers at most, before the first product)
+  u32x4_t a[AHEAD];
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e) a[e] = row_frag<T, D>(rows, l, e);
+  __builtin_amdgcn_sched_barrier(0);
+  f32x16_t s = zero_tile();
+#pragma unroll
+  for (int e = 0; e < X::KS; ++e) {
+    s = mma<T>(a[e % AHEAD], b[e], s);
+    if (e + AHEAD < X::KS) a[e % AHEAD] = row_frag<T, D>(rows, l, e + AHEAD);
+  }
+  return s;
 }
 
 // Adds what Stage::clean left out of 32 rows, where the lane's column sees it: the rows as they are in memory, of which
@@ -240,14 +288,54 @@ __device__ __forceinline__ void add_odd(Acc<T, D>& acc, const char* rows, long l
 // before m, the rounded largest of them, is taken from them.
 constexpr float kLarge = 65536.f;
 
-__device__ __forceinline__ float exponent(float s, float c, float m, bool large) {
+__device__ __forceinline__ float large_exponent(float s, float c, float m) {
 #pragma clang fp contract(off)
-  if (large) return s * c - m;
-  return __builtin_fmaf(s, c, -m);
+  return s * c - m;
 }
 
-// A wave's 32 columns [D x 32] to rows of an output, times f (of each column), through the wave's LDS block of 32 rows;
-// columns from `last` on are not stored, those from `live` on are zeros.
+// s to exponents; m(r) of each value.
+template <typename F>
+__device__ __forceinline__ void exponents(float (&s)[16], float c, bool large, F&& m) {
+  if (__builtin_expect(large, 0)) {
+    asm volatile("");  // (a branch: as a choice it costs three more instructions for each value)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = large_exponent(s[r], c, m(r));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, -m(r));
+  }
+}
+
+// Which of a tile's 32 rows a column sees: those `lo` .. `hi`, and the first `sinks`.  (Bounds in 32 bits: positions and
+// windows are 2^30 at most.)
+struct Seen {
+  int lo, hi, sinks;
+  __device__ __forceinline__ bool operator()(int row) const { return row <= hi && (row >= lo || row < sinks); }
+};
+
+// Puts x in the place of the values of rows that the column does not see.  Most tiles hold no sinks: one comparison then.
+template <int T, int N>
+__device__ __forceinline__ void hide(float x, const Seen& seen, bool sinks, int h, float (&a)[16], float (&b)[N]) {
+  auto put = [&](int r, bool see) {
+    a[r] = see ? a[r] : x;
+    if constexpr (N == 16) b[r] = see ? b[r] : x;
+  };
+  if (sinks) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) put(r, seen(reg_row<T>(r, h)));
+  } else {
+    const unsigned n = (unsigned)max(0, seen.hi - max(seen.lo, -64) + 1);  // (no row is below -64)
+    const int lo = max(seen.lo, -64) - Op<T>::E * h;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) put(r, (unsigned)(reg_row<T>(r, 0) - lo) < n);
+  }
+}
+
+// A wave's 32 columns [D x 32] to rows of an output, times f (of each column), through the wave's LDS block (out_block bytes);
+// n rows are stored, of columns that are not live zeros.
+template <int T, int D>
+constexpr int out_block() { return 32 * (D * Op<T>::size + 16); }
+
 template <int T, int D>
 __device__ __forceinline__ void store_columns(const Acc<T, D>& acc, float f, bool live, char* block, char* out,
                                               long long stride, int n, int l) {
@@ -262,7 +350,7 @@ __device__ __forceinline__ void store_columns(const Acc<T, D>& acc, float f, boo
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = live ? acc[d][4 * g + e] * f : 0.f;
-      char* to = block + (c * X::RV + at) * X::O::size;
+      char* to = block + c * (out_block<T, D>() / 32) + at * X::O::size;
       if constexpr (T == DSQG_F32) {
         *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
       } else {
@@ -281,7 +369,7 @@ __device__ __forceinline__ void store_columns(const Acc<T, D>& acc, float f, boo
   for (int u = 0; u < 32 * X::PPR / 64; ++u) {
     const int e = l + 64 * u, row = e / X::PPR, piece = e - row * X::PPR;
     if (row < n)
-      __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(block + row * X::RV * X::O::size + piece * 16),
+      __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(block + row * (out_block<T, D>() / 32) + piece * 16),
                                   reinterpret_cast<u32x4_t*>(out + row * stride + piece * 16));
   }
 }

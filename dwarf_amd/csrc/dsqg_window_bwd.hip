@@ -14,14 +14,16 @@
 //
 // p and dS enter the products rounded to the 16-bit type (2^-8 of each in bfloat16, 2^-11 in float16); float32 operands are not
 // rounded.  Everything else is fp32.
+//
+// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, dq 365 us, dk/dv 485 us, 565 TFLOP/s of the seven products; B8 H8
+// Hkv1 N2048 D32 window 256 with 4 sinks, dq 30 us, dk/dv 43 us, their parts' sum 4.6 us.  Vector instructions bound both: a
+// pair's exponent, weight, dS and masks cost as much at D = 32 as at D = 128.
 #include <algorithm>
 
 #include "dsqg_window.hpp"
 
 namespace dsqg {
 namespace {
-
-template <int T, int D> constexpr int rows_of_tile() { return T == DSQG_F32 || D > 64 ? 32 : 64; }
 
 __device__ __forceinline__ u32x4_t frag_or_zero(const char* at, bool there) {
   u32x4_t x = {0u, 0u, 0u, 0u};
@@ -49,11 +51,13 @@ __device__ __forceinline__ float dot_frag(u32x4_t a, u32x4_t b, float s) {
   return s;
 }
 
-template <int T, int D>
-__global__ __launch_bounds__(kBlock, 2) void window_dq_kernel(WindowParams p) {
+template <int T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(WindowParams p) {
   using X = Tile<T, D>;
-  constexpr int RT = rows_of_tile<T, D>(), KB = RT / 32, TB = X::bytes(RT);
-  __shared__ __align__(16) char lds[2][2][TB];
+  constexpr int RT = T == DSQG_F32 || D > 64 ? 32 : 64, KB = RT / 32, TB = X::bytes(RT), kCols = 32 * NW;
+  constexpr int BYTES = 4 * TB > NW * out_block<T, D>() ? 4 * TB : NW * out_block<T, D>();
+  __shared__ __align__(16) char bytes[BYTES];
+  auto lds = reinterpret_cast<char(*)[2][TB]>(bytes);  // [which tile][keys, values]
   __shared__ int odd[2];  // which tile's keys hold infinities or NaN, plus one
 
   const int block = xcd_logical_block(blockIdx.x, gridDim.x);
@@ -90,7 +94,7 @@ __global__ __launch_bounds__(kBlock, 2) void window_dq_kernel(WindowParams p) {
   if (h == 0 && i < p.N) p.delta[stat] = delta;
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
 
-  Stage<T, D, RT> sk, sv;
+  Stage<T, D, RT, 64 * NW> sk, sv;
   auto load = [&](int t) {
     sk.load(kh, p.k.n, span.tile(t) * RT, length);
     sv.load(vh, p.v.n, span.tile(t) * RT, length);
@@ -125,30 +129,24 @@ __global__ __launch_bounds__(kBlock, 2) void window_dq_kernel(WindowParams p) {
       const bool none = k0 > i0 + 31 || (k0 + 32 <= i0 - p.window + 1 && k0 >= p.sinks);
       const bool all = k0 + 31 <= i0 && (i0 + 31 - k0 < p.window || k0 + 32 <= p.sinks);
       if (none) continue;
-      const char* const kt = lds[t & 1][0] + 32 * kb * X::RV * X::O::size;
-      const char* const vt = lds[t & 1][1] + 32 * kb * X::RV * X::O::size;
-      f32x16_t s = zero_tile(), dp = zero_tile();
-#pragma unroll
-      for (int e = 0; e < X::KS; ++e) s = mma<T>(row_frag<T, D>(kt, l, e), q[e], s);
-#pragma unroll
-      for (int e = 0; e < X::KS; ++e) dp = mma<T>(row_frag<T, D>(vt, l, e), dout[e], dp);
-      auto sees = [&](int row) {
-        const int back = i - (k0 + row);
-        return back >= 0 && (back < p.window || k0 + row < p.sinks);
-      };
+      const char* const kt = lds[t & 1][0] + 32 * kb * X::RB;
+      const char* const vt = lds[t & 1][1] + 32 * kb * X::RB;
+      const f32x16_t s = scores<T, D>(kt, l, q), dp = scores<T, D>(vt, l, dout);
+      const Seen seen = {i - p.window + 1 - k0, i - k0, p.sinks - k0};
       float w[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) w[r] = exponent(s[r], p.scale2, st.x, large);
+      for (int r = 0; r < 16; ++r) w[r] = s[r];
+      exponents(w, p.scale2, large, [&](int) { return st.x; });
 #pragma unroll
       for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(w[r]) * st.y * (dp[r] - delta);
       if (!all) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] = sees(reg_row<T>(r, h)) ? w[r] : 0.f;
+        float no[1];
+        hide<T>(0.f, seen, k0 < p.sinks, h, w, no);
       }
       Weights<T> f;
       pack<T>(w, f);
       contract<T, D>(acc, kt, l, f);
-      if (odd[t & 1] == t + 1) add_odd<T, D>(acc, kh + k0 * p.k.n, p.k.n, length - k0, l, sees);
+      if (odd[t & 1] == t + 1) add_odd<T, D>(acc, kh + k0 * p.k.n, p.k.n, length - k0, l, seen);
     }
     if (t + 1 < span.n) {
       store(t + 1);
@@ -156,42 +154,70 @@ __global__ __launch_bounds__(kBlock, 2) void window_dq_kernel(WindowParams p) {
     }
     __syncthreads();
   }
-  store_columns<T, D>(acc, p.scale, i < length, lds[0][0] + wave * 32 * X::RV * X::O::size,
+  store_columns<T, D>(acc, p.scale, i < length, bytes + wave * out_block<T, D>(),
                       p.dq.at + b * p.dq.b + head * p.dq.h + i0 * p.dq.n, p.dq.n, p.N - i0, l);
 }
 
-template <int T, int D>
-__global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
-  using X = Tile<T, D>;
-  constexpr int RT = rows_of_tile<T, D>(), RB = RT / 32, TB = X::bytes(RT);
-  __shared__ __align__(16) char lds[2][2][TB];         // [which tile][queries, dout]
-  __shared__ __align__(16) float rows[2][3][RT];       // ... [reference exponent, 1 / sum, D]
-  __shared__ int odd[2][3];                            // ... queries, dout hold infinities or NaN; exponents are large
-
-  const int roles = p.blocks + p.split * p.far;  // of a key/value head; those of the sinks' far queries first
-  const int block = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int bk = block / roles, role = block - bk * roles;
-  const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
-  const int at = role < p.split * p.far ? role / p.far : role - p.split * p.far;
-  const int part = role < p.split * p.far ? 1 + role % p.far : 0;
-  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = l & 31, h = l >> 5;
-  const int length = window_length(p, b);
-  const int k0 = at * kCols, j0 = k0 + 32 * wave, j = j0 + c;
-
-  // Tiles of queries: of each head the same.
-  int first = k0 / RT, tiles = 0;
-  if (k0 < length) {
+// What a dk/dv workgroup takes: a key block (part 0), those of a head on one XCD, or, behind all of them, a share of the far
+// queries of one that holds sinks.
+struct KeyBlock {
+  int bk, at, part;
+  __device__ __forceinline__ explicit KeyBlock(const WindowParams& p) {
+    const int heads = p.B * p.Hkv, whole = heads * p.kblocks;
+    if ((int)blockIdx.x < whole) {
+      const int block = xcd_logical_block(blockIdx.x, whole);
+      bk = block / p.kblocks;
+      at = block - bk * p.kblocks;
+      part = 0;
+    } else {
+      const int block = blockIdx.x - whole, rest = block / heads;
+      bk = block - rest * heads;
+      at = rest / p.far;
+      part = 1 + rest - at * p.far;
+    }
+  }
+  // The tiles of RT queries that it goes over, of each head the same; its keys are `kc`.
+  __device__ __forceinline__ void queries(const WindowParams& p, int RT, int kc, int length, int& first, int& tiles) const {
+    const int k0 = at * kc;
+    first = k0 / RT;
+    tiles = 0;
+    if (k0 >= length) return;
     const int last = (length - 1) / RT;
-    const int near = min((long long)last, ((long long)k0 + kCols - 2 + p.window) / RT);  // of the window
-    if (at >= p.split) tiles = (k0 < p.sinks ? last : near) + 1 - first;
-    else if (part == 0) tiles = near + 1 - first;
-    else {
+    const int near = (int)min((long long)last, ((long long)k0 + kc - 2 + p.window) / RT);  // of the window
+    if (at >= p.split) {
+      tiles = (k0 < p.sinks ? last : near) + 1 - first;
+    } else if (part == 0) {
+      tiles = near + 1 - first;
+    } else {
       const int n = last - near, lo = (int)((long long)n * (part - 1) / p.far), hi = (int)((long long)n * part / p.far);
       first = near + 1 + lo;
       tiles = hi - lo;
     }
   }
+};
+
+// Up to `kSingle` elements a wave has the scores, weights and sums of its 32 keys to itself.
+constexpr int kSingle = 64;
+
+template <int T, int D>
+__global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void window_dkdv_kernel(WindowParams p) {
+  using X = Tile<T, D>;
+  constexpr int RT = T == DSQG_F32 ? 32 : 64, RB = RT / 32, TB = X::bytes(RT), KC = kBlock / 2;
+  static_assert(4 * TB >= 4 * out_block<T, D>(), "the waves' output rows fit the tiles");
+  __shared__ __align__(16) char lds[2][2][TB];         // [which tile][queries, dout]
+  __shared__ __align__(16) float rows[2][3][RT];       // ... [reference exponent, 1 / sum, D]
+  __shared__ int odd[2][3];                            // ... queries, dout hold infinities or NaN; exponents are large
+
+  const KeyBlock block(p);
+  const int bk = block.bk, at = block.at, part = block.part;
+  const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = l & 31, h = l >> 5;
+  const int length = window_length(p, b);
+  const int k0 = at * KC, j0 = k0 + 32 * wave, j = j0 + c;
+
+  int first, tiles;
+  block.queries(p, RT, KC, length, first, tiles);
   const int steps = tiles * p.G;
 
   u32x4_t k[X::KS], v[X::KS];
@@ -225,7 +251,7 @@ __global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
   };
   auto edge = [&](int t) {
     const int i0 = row0(t);
-    return i0 < k0 + kCols - 1 || (i0 + RT - 1 - k0 >= p.window && k0 + kCols > p.sinks);
+    return i0 < k0 + KC - 1 || (i0 + RT - 1 - k0 >= p.window && k0 + KC > p.sinks);
   };
   auto store = [&](int t) {
     if (edge(t)) {
@@ -261,39 +287,35 @@ __global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
       const bool none = i0 + 31 < j0 || (i0 - (j0 + 31) >= p.window && j0 >= p.sinks);
       const bool all = i0 >= j0 + 31 && (i0 + 31 - j0 < p.window || j0 + 32 <= p.sinks);
       if (none) continue;
-      const char* const qt = lds[t & 1][0] + 32 * rb * X::RV * X::O::size;
-      const char* const dt = lds[t & 1][1] + 32 * rb * X::RV * X::O::size;
-      auto sees = [&](int row) {
-        const int back = i0 + row - j;
-        return back >= 0 && (back < p.window || j < p.sinks);
-      };
-      f32x16_t s = zero_tile(), dp = zero_tile();
-#pragma unroll
-      for (int e = 0; e < X::KS; ++e) s = mma<T>(row_frag<T, D>(qt, l, e), k[e], s);
-#pragma unroll
-      for (int e = 0; e < X::KS; ++e) dp = mma<T>(row_frag<T, D>(dt, l, e), v[e], dp);
+      const char* const qt = lds[t & 1][0] + 32 * rb * X::RB;
+      const char* const dt = lds[t & 1][1] + 32 * rb * X::RB;
+      // (Rows are queries here: a sink is seen by all from itself on.)
+      const Seen seen = {j - i0, j < p.sinks ? 64 : min(64, j - i0 + p.window - 1), 0};
+      const f32x16_t s = scores<T, D>(qt, l, k), dp = scores<T, D>(dt, l, v);
       const bool large = odd[t & 1][2] == t + 1;
-      float w[16], x[16];
+      float w[16], x[16], m[16];
+#pragma unroll
+      for (int r4 = 0; r4 < 16; r4 += 4) {
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&rows[t & 1][0][32 * rb + reg_row<T>(r4, h)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[r4 + e] = s[r4 + e];
+          m[r4 + e] = y[e];
+        }
+      }
+      exponents(w, p.scale2, large, [&](int r) { return m[r]; });
 #pragma unroll
       for (int r4 = 0; r4 < 16; r4 += 4) {
         const int row = 32 * rb + reg_row<T>(r4, h);
-        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&rows[t & 1][0][row]);
         const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&rows[t & 1][1][row]);
         const f32x4_t d = *reinterpret_cast<const f32x4_t*>(&rows[t & 1][2][row]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[r4 + e] = __builtin_amdgcn_exp2f(exponent(s[r4 + e], p.scale2, m[e], large)) * y[e];
+          w[r4 + e] = __builtin_amdgcn_exp2f(w[r4 + e]) * y[e];
           x[r4 + e] = w[r4 + e] * (dp[r4 + e] - d[e]);
         }
       }
-      if (!all) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool seen = sees(reg_row<T>(r, h));
-          w[r] = seen ? w[r] : 0.f;
-          x[r] = seen ? x[r] : 0.f;
-        }
-      }
+      if (!all) hide<T>(0.f, seen, false, h, w, x);
       Weights<T> f;
       pack<T>(w, f);
       contract<T, D>(dv, dt, l, f);
@@ -301,9 +323,9 @@ __global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
       contract<T, D>(dk, qt, l, f);
       const int head = hk * p.G + t / tiles;
       if (odd[t & 1][0] == t + 1)
-        add_odd<T, D>(dk, p.q.at + b * p.q.b + head * p.q.h + i0 * p.q.n, p.q.n, length - i0, l, sees);
+        add_odd<T, D>(dk, p.q.at + b * p.q.b + head * p.q.h + i0 * p.q.n, p.q.n, length - i0, l, seen);
       if (odd[t & 1][1] == t + 1)
-        add_odd<T, D>(dv, p.dout.at + b * p.dout.b + head * p.dout.h + i0 * p.dout.n, p.dout.n, length - i0, l, sees);
+        add_odd<T, D>(dv, p.dout.at + b * p.dout.b + head * p.dout.h + i0 * p.dout.n, p.dout.n, length - i0, l, seen);
     }
     if (t + 1 < steps) {
       store(t + 1);
@@ -313,7 +335,7 @@ __global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
   }
 
   if (at < p.split) {
-    float* const to = p.part + ((((long long)bk * p.split + at) * (1 + p.far) + part) * 2 * kCols + 32 * wave + c) * D;
+    float* const to = p.part + ((((long long)bk * p.split + at) * (1 + p.far) + part) * 2 * KC + 32 * wave + c) * D;
 #pragma unroll
     for (int d = 0; d < X::DB; ++d)
 #pragma unroll
@@ -321,29 +343,238 @@ __global__ __launch_bounds__(kBlock) void window_dkdv_kernel(WindowParams p) {
         const int e = 32 * d + 8 * g + 4 * h;
         if (D % 32 != 0 && e >= D) continue;
         *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
-        *reinterpret_cast<f32x4_t*>(to + kCols * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
       }
     return;
   }
-  char* const mine = lds[0][0] + wave * 32 * X::RV * X::O::size;
+  char* const mine = lds[0][0] + wave * out_block<T, D>();
   store_columns<T, D>(dk, p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
   store_columns<T, D>(dv, 1.f, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
 }
 
-// Sums of the sinks' key blocks over their parts.  Grid: [B * Hkv * split * kCols / 8, 2], a thread four elements.
+// Eight waves for 128 keys: a key's scores and weights take registers for its own key and value, its sums for two rows of
+// D more, and one wave with both leaves no place for a second one on its SIMD (D = 128: 978 us at B1 H16 Hkv4 N16384 window 1024).
+// So waves 0-3 make p and dS of 32 keys each, and waves 4-7, a step of 32 queries behind, multiply them with the rows: the
+// operands go through LDS lane by lane, 64 bytes each way, and a SIMD has one of each kind, whose vector and matrix work overlap.
+constexpr int kSteps = 3;  // tiles in LDS: one used by each kind, one arriving
+template <int T, int D> constexpr int dkdv_threads() { return 2 * 64 * key_pairs(T, D); }
+
+template <int T, int D>
+__global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 1) void window_dkdv_pairs_kernel(WindowParams p) {
+  using X = Tile<T, D>;
+  constexpr int RT = 32, TB = X::bytes(RT), kPairs = key_pairs(T, D), KC = 32 * kPairs;
+  __shared__ __align__(16) char lds[kSteps][2][TB];       // [which tile][queries, dout]
+  __shared__ __align__(16) u32x4_t ops[2][kPairs][2 * X::C][64];  // p and dS of a step
+  __shared__ __align__(16) float rows[kSteps][3][RT];     // ... [reference exponent, 1 / sum, D]
+  __shared__ int odd[kSteps][3];                          // ... queries, dout hold infinities or NaN; exponents are large
+  static_assert(kSteps * 2 * TB >= kPairs * out_block<T, D>(), "the waves' output rows fit the tiles");
+
+  const KeyBlock block(p);
+  const int bk = block.bk, at = block.at, part = block.part;
+  const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = wave % kPairs;
+  const bool maker = wave < kPairs;
+  const int c = l & 31, h = l >> 5;
+  const int length = window_length(p, b);
+  const int k0 = at * KC, j0 = k0 + 32 * pair, j = j0 + c;
+
+  int first, tiles;
+  block.queries(p, RT, KC, length, first, tiles);
+  const int steps = tiles * p.G;
+  if (threadIdx.x < 3 * kSteps) odd[threadIdx.x / 3][threadIdx.x % 3] = 0;
+
+  Stage<T, D, RT, 2 * 64 * kPairs> sq, sd;
+  float2 st;
+  float de;
+  int lh = 0, li = 0;  // the next tile to load: its head and number
+  auto load = [&] {
+    const int head = hk * p.G + lh, i0 = (first + li) * RT;
+    sq.load(p.q.at + b * p.q.b + head * p.q.h, p.q.n, i0, length);
+    sd.load(p.dout.at + b * p.dout.b + head * p.dout.h, p.dout.n, i0, length);
+    st = make_float2(INFINITY, 0.f);
+    de = 0.f;
+    if (threadIdx.x < RT && i0 + (int)threadIdx.x < length) {
+      const long long s = ((long long)b * p.Hkv * p.G + head) * p.N + i0 + threadIdx.x;
+      st = p.stats[s];
+      de = p.delta[s];
+    }
+    if (++li == tiles) {
+      li = 0;
+      ++lh;
+    }
+  };
+  auto store = [&](int t, int at, int i0) {  // step t's tile, whose first query is i0, to place `at`
+    if (i0 < k0 + KC - 1 || (i0 + RT - 1 - k0 >= p.window && k0 + KC > p.sinks)) {  // some keys are not seen
+      if (sq.clean()) odd[at][0] = t + 1;
+      if (sd.clean()) odd[at][1] = t + 1;
+    }
+    sq.store(lds[at][0]);
+    sd.store(lds[at][1]);
+    if (threadIdx.x < RT) {
+      rows[at][0][threadIdx.x] = st.x;
+      rows[at][1][threadIdx.x] = st.y;
+      rows[at][2][threadIdx.x] = de;
+      if (fabsf(st.x) >= kLarge && st.x != INFINITY) odd[at][2] = t + 1;
+    }
+  };
+  auto next = [&](int x) { return x == kSteps - 1 ? 0 : x + 1; };
+  // Nothing of the tile from query i0 on sees the wave's keys.
+  auto none = [&](int i0) { return i0 + 31 < j0 || (i0 - (j0 + 31) >= p.window && j0 >= p.sinks); };
+  auto seen_of = [&](int i0) {  // (Rows are queries here: a sink is seen by all from itself on.)
+    return Seen{j - i0, j < p.sinks ? 64 : min(64, j - i0 + p.window - 1), 0};
+  };
+
+  __syncthreads();
+  if (steps > 0) {
+    load();
+    store(0, 0, first * RT);
+    if (steps > 1) load();
+  }
+  __syncthreads();
+
+  if (maker) {
+    u32x4_t k[X::KS], v[X::KS];
+    {
+      const char* const rk = p.k.at + b * p.k.b + hk * p.k.h + (long long)j * p.k.n;
+      const char* const rv = p.v.at + b * p.v.b + hk * p.v.h + (long long)j * p.v.n;
+#pragma unroll
+      for (int s = 0; s < X::KS; ++s) {
+        const int e = (2 * X::E * s + X::E * h) * X::O::size;
+        k[s] = frag_or_zero(rk + e, j < length);
+        v[s] = frag_or_zero(rv + e, j < length);
+      }
+    }
+    int place = 0, tile = 0;
+#pragma unroll 1
+    for (int t = 0; t <= steps; ++t) {
+      const int i0 = (first + tile) * RT;
+      if (t < steps && !none(i0)) {
+        const char* const qt = lds[place][0];
+        const char* const dt = lds[place][1];
+        const f32x16_t s = scores<T, D>(qt, l, k), dp = scores<T, D>(dt, l, v);
+        const bool large = odd[place][2] == t + 1;
+        float w[16], x[16], m[16];
+#pragma unroll
+        for (int r4 = 0; r4 < 16; r4 += 4) {
+          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&rows[place][0][reg_row<T>(r4, h)]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[r4 + e] = s[r4 + e];
+            m[r4 + e] = y[e];
+          }
+        }
+        exponents(w, p.scale2, large, [&](int r) { return m[r]; });
+#pragma unroll
+        for (int r4 = 0; r4 < 16; r4 += 4) {
+          const int row = reg_row<T>(r4, h);
+          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(&rows[place][1][row]);
+          const f32x4_t d = *reinterpret_cast<const f32x4_t*>(&rows[place][2][row]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[r4 + e] = __builtin_amdgcn_exp2f(w[r4 + e]) * y[e];
+            x[r4 + e] = w[r4 + e] * (dp[r4 + e] - d[e]);
+          }
+        }
+        const bool all = i0 >= j0 + 31 && (i0 + 31 - j0 < p.window || j0 + 32 <= p.sinks);
+        if (!all) hide<T>(0.f, seen_of(i0), false, h, w, x);
+        Weights<T> f;
+        pack<T>(w, f);
+#pragma unroll
+        for (int e = 0; e < X::C; ++e) ops[t & 1][pair][e][l] = f[e];
+        pack<T>(x, f);
+#pragma unroll
+        for (int e = 0; e < X::C; ++e) ops[t & 1][pair][X::C + e][l] = f[e];
+      }
+      place = next(place);
+      if (++tile == tiles) tile = 0;
+      if (t + 1 < steps) {
+        store(t + 1, place, (first + tile) * RT);
+        if (t + 2 < steps) load();
+      }
+      __syncthreads();
+    }
+    return;
+  }
+
+  Acc<T, D> dk, dv;
+#pragma unroll
+  for (int d = 0; d < X::DB; ++d) dk[d] = dv[d] = zero_tile();
+  int place = 0, last = 0, tile = 0, was = 0, head = hk * p.G;  // of step t, and of the step before
+#pragma unroll 1
+  for (int t = 0; t <= steps; ++t) {
+    const int i0 = (first + was) * RT;
+    if (t > 0 && !none(i0)) {
+      const char* const qt = lds[last][0];
+      const char* const dt = lds[last][1];
+      Weights<T> f;
+#pragma unroll
+      for (int e = 0; e < X::C; ++e) f[e] = ops[(t - 1) & 1][pair][e][l];
+      contract<T, D>(dv, dt, l, f);
+#pragma unroll
+      for (int e = 0; e < X::C; ++e) f[e] = ops[(t - 1) & 1][pair][X::C + e][l];
+      contract<T, D>(dk, qt, l, f);
+      if (odd[last][0] == t)
+        add_odd<T, D>(dk, p.q.at + b * p.q.b + head * p.q.h + i0 * p.q.n, p.q.n, length - i0, l, seen_of(i0));
+      if (odd[last][1] == t)
+        add_odd<T, D>(dv, p.dout.at + b * p.dout.b + head * p.dout.h + i0 * p.dout.n, p.dout.n, length - i0, l, seen_of(i0));
+    }
+    if (t > 0 && was == tiles - 1) ++head;
+    was = tile;
+    last = place;
+    place = next(place);
+    if (++tile == tiles) tile = 0;
+    if (t + 1 < steps) {
+      store(t + 1, place, (first + tile) * RT);
+      if (t + 2 < steps) load();
+    }
+    __syncthreads();
+  }
+
+  if (at < p.split) {
+    float* const to = p.part + ((((long long)bk * p.split + at) * (1 + p.far) + part) * 2 * KC + 32 * pair + c) * D;
+#pragma unroll
+    for (int d = 0; d < X::DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int e = 32 * d + 8 * g + 4 * h;
+        if (D % 32 != 0 && e >= D) continue;
+        *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+      }
+    return;
+  }
+  char* const mine = lds[0][0] + pair * out_block<T, D>();
+  store_columns<T, D>(dk, p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
+  store_columns<T, D>(dv, 1.f, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
+}
+
+// Sums of the sinks' key blocks over their parts.  Grid: [B * Hkv * split * kcols / 8, 2], a thread four elements.
 template <int T, int D>
 __global__ __launch_bounds__(kBlock) void window_sinks_kernel(WindowParams p) {
   constexpr int L = D / 4;  // lanes of a row
   const int which = blockIdx.y;
   for (int e = threadIdx.x; e < 8 * L; e += kBlock) {
     const long long row = (long long)blockIdx.x * 8 + e / L;
-    const int col = (int)(row % kCols), d = e % L * 4;
-    const long long block = row / kCols;
-    const int at = (int)(block % p.split), bk = (int)(block / p.split), b = bk / p.Hkv, hk = bk - b * p.Hkv, j = at * kCols + col;
+    const int col = (int)(row % p.kcols), d = e % L * 4;
+    const long long block = row / p.kcols;
+    const int at = (int)(block % p.split), bk = (int)(block / p.split), b = bk / p.Hkv, hk = bk - b * p.Hkv, j = at * p.kcols + col;
     if (j >= p.N) continue;
     f32x4_t x = zero4();
-    const float* from = p.part + ((block * (1 + p.far) * 2 + which) * kCols + col) * D + d;
-    for (int i = 0; i <= p.far; ++i) x += *reinterpret_cast<const f32x4_t*>(from + (long long)i * 2 * kCols * D);
+    const float* from = p.part + ((block * (1 + p.far) * 2 + which) * p.kcols + col) * D + d;
+    const int parts = j < p.sinks ? p.far : 0;  // (others' keys are not seen from afar)
+    // (Sixteen parts' loads at once: 4.6 us at D = 32 with 18 far parts, 5.6 at D = 128 with 53;
+    // one after the other 7.9 and 15.7.)
+    constexpr int kAtOnce = 16;
+    for (int i = 0; i <= parts; i += kAtOnce) {
+      f32x4_t y[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        y[u] = *reinterpret_cast<const f32x4_t*>(from + (long long)min(i + u, parts) * 2 * p.kcols * D);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (i + u <= parts) x += y[u];
+    }
     const bool live = j < window_length(p, b);
     const float f = which == 0 ? p.scale : 1.f;
 #pragma unroll
@@ -363,11 +594,18 @@ __global__ __launch_bounds__(kBlock) void window_sinks_kernel(WindowParams p) {
 
 template <int T, int D>
 hipError_t launch(const WindowParams& p, hipStream_t st) {
-  const unsigned heads = (unsigned)(p.B * p.Hkv);
-  hipLaunchKernelGGL((window_dq_kernel<T, D>), dim3(heads * (unsigned)(p.G * p.blocks)), dim3(kBlock), 0, st, p);
-  hipLaunchKernelGGL((window_dkdv_kernel<T, D>), dim3(heads * (unsigned)(p.blocks + p.split * p.far)), dim3(kBlock), 0, st, p);
+  const unsigned heads = (unsigned)(p.B * p.Hkv), blocks = heads * (unsigned)(p.G * p.blocks);
+  bool wide = false;
+  if constexpr (may_be_wide(T, D)) {
+    wide = p.waves == 8;
+    if (wide) hipLaunchKernelGGL((window_dq_kernel<T, D, 8>), dim3(blocks), dim3(512), 0, st, p);
+  }
+  if (!wide) hipLaunchKernelGGL((window_dq_kernel<T, D, 4>), dim3(blocks), dim3(256), 0, st, p);
+  const dim3 grid(heads * (unsigned)(p.kblocks + p.split * p.far));
+  if constexpr (D > kSingle) hipLaunchKernelGGL((window_dkdv_pairs_kernel<T, D>), grid, dim3(dkdv_threads<T, D>()), 0, st, p);
+  else hipLaunchKernelGGL((window_dkdv_kernel<T, D>), grid, dim3(kBlock), 0, st, p);
   if (p.split)
-    hipLaunchKernelGGL((window_sinks_kernel<T, D>), dim3(heads * (unsigned)(p.split * kCols / 8), 2), dim3(kBlock), 0, st, p);
+    hipLaunchKernelGGL((window_sinks_kernel<T, D>), dim3(heads * (unsigned)(p.split * p.kcols / 8), 2), dim3(kBlock), 0, st, p);
   return hipGetLastError();
 }
 
@@ -405,23 +643,30 @@ int check_window(const dsqg_window_shape& s, WindowParams* p) {
   p->window = std::min(s.window, 1 << 30);
   p->sinks = std::min(s.sinks, 1 << 30);
   p->scale = s.softmax_scale;
-  p->scale2 = s.softmax_scale * 1.4426950408889634f;
+  // (No scale gives equal weights to all scores up to 2^100, and a score of -infinity none.)
+  p->scale2 = s.softmax_scale == 0.f ? 0x1p-126f : s.softmax_scale * 1.4426950408889634f;
   p->lengths = reinterpret_cast<const long long*>(s.lengths);
-  p->blocks = (s.N + kCols - 1) / kCols;
+  // Eight waves of 32 queries share a tile where that leaves two workgroups for each CU, else four (may_be_wide).
+  p->waves = may_be_wide(s.dtype, s.D) && (long long)s.B * s.H * ((s.N + 255ll) / 256) >= 512 ? 8 : 4;
+  p->blocks = (s.N + 32 * p->waves - 1) / (32 * p->waves);
   // The grids, and positions plus a window in 32 bits.
-  if (s.N > (1 << 30) || (long long)s.B * s.H * (p->blocks + 64) >= (1ll << 31)) return DSQG_EUNSUPPORTED;
-  // The sinks' far queries: shares of about as many queries as the other blocks see, 64 of them at most.
-  const long long beyond = (long long)s.N - kCols - p->window;
+  if (s.N > (1 << 30) || (long long)s.B * s.H * (s.N / 64ll + 64) >= (1ll << 31)) return DSQG_EUNSUPPORTED;
+  // The sinks' far queries: shares of a quarter of the queries that other blocks see, which fill the places that those leave
+  // free at the end; 64 of them at most.
+  const int kc = p->kcols = 32 * key_pairs(s.dtype, s.D);
+  p->kblocks = (s.N + kc - 1) / kc;
+  const long long beyond = (long long)s.N - kc - p->window;
   if (p->sinks > 0 && beyond > 0) {
-    p->split = (std::min(p->sinks, s.N) + kCols - 1) / kCols;
-    p->far = (int)std::min((beyond + p->window + kCols - 1) / (p->window + kCols), std::max(1ll, 64ll / p->split));
+    p->split = (std::min(p->sinks, s.N) + kc - 1) / kc;
+    const long long share = std::max(64, (p->window + kc) / 4);
+    p->far = (int)std::min((beyond + share - 1) / share, std::max(1ll, 64ll / p->split));
   }
   return DSQG_OK;
 }
 
 size_t delta_bytes(const dsqg_window_shape& s) { return ((size_t)s.B * s.H * s.N * sizeof(float) + 255) / 256 * 256; }
 size_t part_bytes(const WindowParams& p) {
-  return (size_t)p.B * p.Hkv * p.split * (1 + p.far) * 2 * kCols * p.D * sizeof(float);
+  return (size_t)p.B * p.Hkv * p.split * (1 + p.far) * 2 * p.kcols * p.D * sizeof(float);
 }
 
 // Rows: a base and strides {b, h, n} that keep every row 16-byte aligned, and rows that do not overlap, within 2^24 bytes.

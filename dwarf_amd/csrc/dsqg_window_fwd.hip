@@ -2,7 +2,7 @@
 //
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j     over the positions j that i sees (dsqg_window.hpp)
 //
-// A workgroup takes 128 queries of a head, a wave 32 of them, and goes once over the tiles of keys and values that any of
+// A workgroup takes 128 or 256 queries of a head, a wave 32 of them, and goes once over the tiles of keys and values that any of
 // them sees, with a running maximum and sum: S^T = K Q^T, weights, O^T += V^T P^T, the weights staying in registers from
 // one product to the other.  Keys and values are loaded a tile ahead and lie in LDS twice, so that a tile costs one
 // barrier.  Only tiles at the window's two ends (and the sinks') compare positions.
@@ -10,19 +10,22 @@
 // Weights are rounded once to the 16-bit type before they multiply the values (2^-8 of each in bfloat16, 2^-11 in float16); float32
 // operands are not rounded.  Scores, the maximum, the sum and the output's sums are fp32.  For the backward a query's
 // reference exponent m and 1 / sum are kept apart, for m may be too large to hold the sum's logarithm.
+//
+// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, 262 us, 525 TFLOP/s of the two products; B8 H8 Hkv1 N2048 D32 window
+// 256 with 4 sinks, 24 us, 190 TFLOP/s.  Vector instructions and latency bound it: at D = 128 half of the cycles issue
+// vector work and a fifth matrix work, at D = 32 a score costs as many vector instructions for a quarter of the products.
 #include "dsqg_window.hpp"
 
 namespace dsqg {
 namespace {
 
-template <int T> constexpr int rows_of_tile() { return T == DSQG_F32 ? 32 : 64; }
-
-template <int T, int D>
-__global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
+template <int T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(WindowParams p) {
   using X = Tile<T, D>;
-  constexpr int RT = rows_of_tile<T>(), KB = RT / 32, TB = X::bytes(RT);
-  static_assert(4 * TB >= 4 * 32 * X::RV * X::O::size, "the waves' output rows fit the tiles");
-  __shared__ __align__(16) char lds[2][2][TB];  // [which tile][keys, values]
+  constexpr int RT = T == DSQG_F32 || (D > 64 && NW == 4) ? 32 : 64, KB = RT / 32, TB = X::bytes(RT), kCols = 32 * NW;
+  constexpr int BYTES = 4 * TB > NW * out_block<T, D>() ? 4 * TB : NW * out_block<T, D>();
+  __shared__ __align__(16) char bytes[BYTES];          // the tiles, in the end the waves' output rows
+  auto lds = reinterpret_cast<char(*)[2][TB]>(bytes);  // [which tile][keys, values]
   __shared__ int odd[2];                        // which tile's values hold infinities or NaN, plus one
 
   // Blocks that read the same keys, the heads of a key/value head, follow each other; the longest come first.
@@ -49,7 +52,7 @@ __global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
   }
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
 
-  Stage<T, D, RT> sk, sv;
+  Stage<T, D, RT, 64 * NW> sk, sv;
   auto load = [&](int t) {
     sk.load(kh, p.k.n, span.tile(t) * RT, length);
     sv.load(vh, p.v.n, span.tile(t) * RT, length);
@@ -72,7 +75,7 @@ __global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
   bool large = false;
   // The largest weight is 2^lift: float16 weights far below it stay clear of the type's subnormal numbers.
   constexpr float lift = T == DSQG_F16 ? 14.f : 0.f;
-  const float far = p.scale2 < 0.f ? INFINITY : -INFINITY;  // a score that is no maximum
+  const float far = p.scale2 < 0.f ? INFINITY : -INFINITY;  // a score of weight zero (scale2 is never zero)
 
   __syncthreads();
   if (span.n > 0) {
@@ -86,46 +89,38 @@ __global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
     const int j0 = span.tile(t) * RT;
     const char* const kt = lds[t & 1][0];
     const char* const vt = lds[t & 1][1];
-    // Nothing of it is seen by the wave's queries / all of it is.
-    const bool none = j0 > i0 + 31 || (j0 + RT <= i0 - p.window + 1 && j0 >= p.sinks);
-    const bool all = j0 + RT - 1 <= i0 && (i0 + 31 - j0 < p.window || j0 + RT <= p.sinks);
-    if (!none) {
-      f32x16_t s[KB];
+    // Of a block of 32 keys the wave's queries see nothing / all.
+    auto none = [&](int k0) { return k0 > i0 + 31 || (k0 + 32 <= i0 - p.window + 1 && k0 >= p.sinks); };
+    auto all = [&](int k0) { return k0 + 31 <= i0 && (i0 + 31 - k0 < p.window || k0 + 32 <= p.sinks); };
+    // All blocks' scores first: the matrix instructions work on the second while the first is weighed.  (Not at D = 32, where
+    // four workgroups a CU do that, with 128 registers a wave.)
+    constexpr bool FIRST = D > 32;
+    f32x16_t x[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        s[kb] = zero_tile();
+    for (int kb = 0; kb < KB; ++kb)
+      if (FIRST && !none(j0 + 32 * kb)) x[kb] = scores<T, D>(kt + 32 * kb * X::RB, l, q);
 #pragma unroll
-        for (int e = 0; e < X::KS; ++e) s[kb] = mma<T>(row_frag<T, D>(kt + 32 * kb * X::RV * X::O::size, l, e), q[e], s[kb]);
+    for (int kb = 0; kb < KB; ++kb) {
+      const int k0 = j0 + 32 * kb;
+      if (none(k0)) continue;
+      if (!FIRST) x[kb] = scores<T, D>(kt + 32 * kb * X::RB, l, q);
+      float s[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = x[kb][r];
+      const Seen seen = {i - p.window + 1 - k0, i - k0, p.sinks - k0};
+      if (!all(k0)) {
+        float no[1];
+        hide<T>(far, seen, k0 < p.sinks, h, s, no);
       }
-      auto sees = [&](int kb, int row) {  // (this lane's query)
-        const int back = i - (j0 + 32 * kb + row);
-        return back >= 0 && (back < p.window || j0 + 32 * kb + row < p.sinks);
-      };
-      uint32_t hide[KB] = {};
-      if (!all) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool gone = !sees(kb, reg_row<T>(r, h));
-            hide[kb] |= (gone ? 1u : 0u) << r;
-            s[kb][r] = gone ? far : s[kb][r];
-          }
-      }
-      float mx = s[0][0];
+      float mx = s[0];
       if (p.scale2 < 0.f) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fminf(mx, s[kb][r]);
+        for (int r = 1; r < 16; ++r) mx = fminf(mx, s[r]);
       } else {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
       }
-      mx = mx == far ? -INFINITY : mx * p.scale2 - lift;  // (a scale of zero makes no NaN of what is not seen)
-      mx = xor32_pair_max(mx);
+      mx = xor32_pair_max(mx * p.scale2 - lift);
       if (__any(mx > m)) {
         const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
@@ -137,26 +132,15 @@ __global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
           for (int r = 0; r < 16; ++r) o[d][r] *= a;
       }
       const float ref = m == -INFINITY ? 0.f : m;
+      exponents(s, p.scale2, large, [&](int) { return ref; });
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        float w[16];
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] = exponent(s[kb][r], p.scale2, ref, large);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(w[r]);
-        if (!all) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) w[r] = (hide[kb] >> r) & 1 ? 0.f : w[r];
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum += w[r];
-        Weights<T> f;
-        pack<T>(w, f);
-        const char* const rows = vt + 32 * kb * X::RV * X::O::size;
-        contract<T, D>(o, rows, l, f);
-        if (odd[t & 1] == t + 1)
-          add_odd<T, D>(o, vh + (j0 + 32 * kb) * p.v.n, p.v.n, length - j0 - 32 * kb, l, [&](int row) { return sees(kb, row); });
-      }
+      for (int r = 0; r < 16; ++r) sum += s[r];
+      Weights<T> f;
+      pack<T>(s, f);
+      contract<T, D>(o, vt + 32 * kb * X::RB, l, f);
+      if (odd[t & 1] == t + 1) add_odd<T, D>(o, vh + k0 * p.v.n, p.v.n, length - k0, l, seen);
     }
     if (t + 1 < span.n) {
       store(t + 1);
@@ -167,16 +151,23 @@ __global__ __launch_bounds__(kBlock, 2) void window_fwd_kernel(WindowParams p) {
 
   sum = xor32_pair_sum(sum);
   const bool live = i < length && sum != 0.f;
-  store_columns<T, D>(o, 1.f / sum, live, lds[0][0] + wave * 32 * X::RV * X::O::size,
+  store_columns<T, D>(o, 1.f / sum, live, bytes + wave * out_block<T, D>(),
                       p.out.at + b * p.out.b + head * p.out.h + i0 * p.out.n, p.out.n, p.N - i0, l);
   if (p.stats && h == 0 && i < p.N)
     p.stats[((long long)b * p.Hkv * p.G + head) * p.N + i] = live ? make_float2(m, 1.f / sum) : make_float2(INFINITY, 0.f);
 }
 
+template <int T, int D, int NW>
+hipError_t launch_waves(const WindowParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((window_fwd_kernel<T, D, NW>), dim3((unsigned)((long long)p.B * p.Hkv * p.G * p.blocks)), dim3(64 * NW), 0, st, p);
+  return hipGetLastError();
+}
+
 template <int T, int D>
 hipError_t launch(const WindowParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((window_fwd_kernel<T, D>), dim3((unsigned)((long long)p.B * p.Hkv * p.G * p.blocks)), dim3(kBlock), 0, st, p);
-  return hipGetLastError();
+  if constexpr (may_be_wide(T, D))
+    if (p.waves == 8) return launch_waves<T, D, 8>(p, st);
+  return launch_waves<T, D, 4>(p, st);
 }
 
 template <int T>

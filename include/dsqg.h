@@ -423,7 +423,7 @@ int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
  *
  * q, out and their gradients are [B,H,N,D], k, v and theirs [B,Hkv,N,D], H a multiple of Hkv.  With lengths given, rows
  * i >= lengths[b] are not there: nothing sees them, and their outputs and gradients are zeros.  D is one of
- * dsqg_supported_head_dims (EUNSUPPORTED otherwise), window at least 1, sinks at least 0, N at most 2^30 and B * H * (N / 128 +
+ * dsqg_supported_head_dims (EUNSUPPORTED otherwise), window at least 1, sinks at least 0, N at most 2^30 and B * H * (N / 64 +
  * 64) less than 2^31 (EUNSUPPORTED).  Every tensor has unit inner stride, strides {b, h, n} and a base that keep rows
  * 16-byte aligned, and a row stride of at least D elements and less than 2^24 bytes.
  *
