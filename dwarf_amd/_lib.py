@@ -190,7 +190,7 @@ class SampleArgs(ctypes.Structure):
                 ("logits", _vp), ("logits_stride", ctypes.c_int64), ("u", _vp),
                 ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double),
                 ("top_k", ctypes.c_int64), ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp),
-                ("tokens", _vp), ("logprobs", _vp)]
+                ("tokens", _vp), ("logprobs", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
 # Every symbol include/dsqg.h declares, with its ctypes signature.
@@ -232,6 +232,7 @@ SIGNATURES = {
     "dsqg_paged_tree_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs),
                                                       ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_paged_tree": (ctypes.c_int, [ctypes.POINTER(PagedTreeArgs), _vp]),
+    "dsqg_sample_workspace_size": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
     "dsqg_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
 }
 

@@ -51,6 +51,7 @@ struct Api {
   decltype(&dsqg_paged_tree) paged_tree = nullptr;
   decltype(&dsqg_tree_accept) tree_accept = nullptr;
   decltype(&dsqg_sample) sample = nullptr;
+  decltype(&dsqg_sample_workspace_size) sample_workspace_size = nullptr;
   PyObject* library_error = nullptr;  // dwarf_amd._lib.DSQGLibraryError
 } api;
 
@@ -1321,6 +1322,9 @@ std::tuple<Tensor, OptTensor> sample(const Tensor& logits0, const Tensor& u0, do
   a.min_ps = static_cast<const float*>(ptr(min_ps));
   a.tokens = static_cast<int64_t*>(ptr(tokens));
   a.logprobs = static_cast<float*>(ptr(logp));
+  check(api.sample_workspace_size(a.B, a.V, a.dtype, &a.workspace_bytes), "dsqg_sample_workspace_size");
+  const Tensor work = a.workspace_bytes ? at::empty({(int64_t)a.workspace_bytes}, x.options().dtype(at::kByte)) : Tensor();
+  a.workspace = ptr(work);
   check(api.sample(&a, stream_of(dev)), "dsqg_sample");
   return {tokens, opt(logp)};
 }
@@ -1352,6 +1356,7 @@ void init(const py::dict& addresses, const py::object& library_error) {
   get(api.paged_tree, "dsqg_paged_tree");
   get(api.tree_accept, "dsqg_tree_accept");
   get(api.sample, "dsqg_sample");
+  get(api.sample_workspace_size, "dsqg_sample_workspace_size");
   api.library_error = library_error.inc_ref().ptr();  // lives as long as the process
 }
 

@@ -563,8 +563,11 @@ typedef struct {
     const float* min_ps;
     int64_t* tokens;           /* [B] */
     float* logprobs;           /* [B] or NULL */
+    void* workspace;           /* 256-byte aligned; may be NULL where its size is 0 */
+    size_t workspace_bytes;
 } dsqg_sample_args;
 
+int dsqg_sample_workspace_size(int32_t B, int32_t V, int32_t dtype, size_t* bytes);
 int dsqg_sample(const dsqg_sample_args* args, dsqg_stream_t stream);
 
 #ifdef __cplusplus

@@ -275,3 +275,49 @@ def test_write_rows(gpu_device, kv):
     paged_kv_write(k[:, :, :0], v[:, :, :0], c[0], c[1], table, pos, rows=rows, **c[2])
     paged_kv_write(k, v, c[0], c[1], table, pos, rows=rows[:, :0], **c[2])
     assert not c[0].view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("V,dtype", [(8192, F32), (9001, BF), (40001, F16), (40000, F32)])
+def test_split_rows(gpu_device, V, dtype):
+    """A few long rows, which several workgroups share: every way that the limits take, row by row and together."""
+    x, u = rows(5, V + 3, V, dtype)
+    x[1, :] = 0.25                          # equal logits, whose limits end inside a group
+    x[2, torch.arange(V + 3) % 997 != 5] = -math.inf  # a masked vocabulary
+    x[3, 100:V:50] = math.nan
+    x = x[:, 3:]                            # (rows that begin anywhere)
+    for kw in (dict(), dict(top_k=1), dict(top_k=50, top_p=0.8), dict(top_k=1000, min_p=0.01), dict(top_k=1500, top_p=0.9),
+               dict(top_p=0.9), dict(top_p=0.99999), dict(min_p=0.05), dict(temperature=0.0)):
+        check(x, u, **{"temperature": 0.8, **kw})
+    k, p = torch.tensor([0, 7, 3, 2000, V]), torch.tensor([0.7, 1.0, 0.5, 0.9, 1.0])
+    t = torch.tensor([0.9, 1.1, 0.0, 0.7, math.inf])
+    check(x, u, t, k, p, torch.tensor([0.0, 0.0, 0.1, 0.002, 0.0]))
+    y = x.clone()
+    y[0, V // 2] = y[0, V - 1] = math.inf   # infinities share their row
+    y[4] = -math.inf                        # no candidate
+    check(y, u, 0.9, top_p=0.95)
+    check(y, u, 0.9, top_k=11)
+
+
+def test_split_rows_in_two_graphs(gpu_device):
+    """Graphs that are replayed in turn, each with scratch memory of its own."""
+    x, u = rows(2, 50000, 3)
+    x, u = x.cuda(), u.cuda()
+    y, v = x.flip(1).contiguous(), 1 - u
+    calls = [lambda: sample_tokens(x, u, 0.9, top_p=0.9, return_logprobs=True), lambda: sample_tokens(y, v, 1.1, top_k=30, return_logprobs=True)]
+    graphs, outs = [], []
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    for i in range(4):
+        x.copy_(torch.randn(2, 50000, generator=torch.Generator().manual_seed(50 + i)) * 2)
+        y.copy_(x.flip(1))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for call, out in zip(calls, outs):
+            for a, b in zip(call(), out):
+                assert torch.equal(a, b)
