@@ -18,6 +18,11 @@
 // Weights of groups of 16 columns enter the second product as two 16-bit terms (dsqg_paged_mfma.hip: 2^-16 of the weight),
 // those of larger groups, which arithmetic bounds, as one: a rounding of up to 2^-8 (bfloat16) or 2^-11 (float16) of each
 // weight, of the size of the output's own.  Scores, statistics and sums are fp32.
+//
+// Measured: 16 sequences of up to 8192, 8 key/value heads of 4, 64 nodes, D = 128 over e4m3, 326 us, 266 TFLOP/s: vector
+// instructions (a weight's and the codes', of which 32 columns share each) and the latency of two waves a SIMD bound it.
+// 32 sequences of up to 2048, 12 heads, 26 nodes, D = 64 in bfloat16, 42 us, 3.2 TB/s; one node within a window of 1024 of
+// 8191, 25 us, 3.9 TB/s: reads of pages, each wave a tile ahead.  One sequence of 77 in float32, 8 us: a launch's latency.
 #include <algorithm>
 
 #include "dsqg_launch.hpp"
@@ -103,8 +108,13 @@ __device__ __forceinline__ bool odd_values(uint4 v) {
   return odd;
 }
 
+// Whether a group's queries are read from LDS for each tile, where they would take 32 registers of a wave or more.
+constexpr bool queries_in_lds(int QT, int CT, int D, int NQ) {
+  return QT != DSQG_F32 && !(QT == DSQG_F16 && narrow(CT)) && NQ * ((D + 31) / 32) >= 8;
+}
+
 template <int QT, int CT, int D, int NQ>
-__global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
+__global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_kernel(PagedTree p) {
   using S = Steps<CT, D>;
   using V = ValueMap<CT, D>;
   constexpr bool FP32 = QT == DSQG_F32;
@@ -112,10 +122,14 @@ __global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
   constexpr bool QLO = QT == DSQG_F16 && narrow(CT);  // queries in two terms
   constexpr bool PLO = !FP32 && NQ == 1;              // weights in two terms
   constexpr int ES = elem_size(CT), KS = S::count, DB = D / 16;
-  constexpr int RV = FP32 ? D + 4 : Geo<D>::RV;       // row stride of staged values, in elements
+  // Row stride of staged values, in elements: of 16 bits an odd multiple of eight banks, so that the transposed reads, of four
+  // pieces of sixteen rows, meet in none.
+  constexpr int RV = FP32 ? D + 4 : D % 32 == 0 ? D + 16 : D;
   typedef typename std::conditional<FP32, float, bf16_t>::type val_t;
   __shared__ __align__(16) val_t sV[kWaves][kTile * RV];
   __shared__ float wm[kWaves][16], wl[kWaves][16];
+  constexpr bool QLDS = queries_in_lds(QT, CT, D, NQ);
+  __shared__ uint4 sQ[QLDS ? NQ * KS : 1][QLDS ? 64 : 1];  // a lane's fragments
 
   const int groups = p.cols / (16 * NQ);
   const int unit = blockIdx.x;  // (grid.x is rounded up, so that a unit's groups run on one XCD)
@@ -225,9 +239,19 @@ __global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
   // Tiles from all_from on that end before the draft have no masks; rows below any_from that are no sinks are seen by nobody.
   const int all_from = p.window ? max(0, pos + nodes - p.window) : 0, any_from = p.window ? max(0, pos - p.window + 1) : 0;
 
-  Frag<FP32> qh[NQ][KS], ql[NQ][QLO ? KS : 1];
+  Frag<FP32> qh[QLDS ? 1 : NQ][KS], ql[NQ][QLO ? KS : 1];
+  if constexpr (QLDS) {
+    for (int e = wave; e < NQ * KS; e += kWaves) {
+      const int n = e / KS, m = c0 + 16 * n + i, t = m / p.G, d = S::at(e - n * KS, g);
+      Raw8<QT> r;
+      raw_zero<QT>(r);
+      if (m < M && d < D) r = raw_load<QT>(p.q + b * p.qb + (hk * p.G + m - t * p.G) * p.qh + t * p.qt + d * elem_size(QT));
+      sQ[e][l] = r.a;
+    }
+    __syncthreads();
+  }
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+  for (int n = 0; n < (QLDS ? 0 : NQ); ++n) {
     const int m = c0 + 16 * n + i, t = m / p.G;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -405,17 +429,32 @@ __global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
     f32x4_t s[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = zero4();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    if constexpr (QLDS) {
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
-        Frag<FP32> a;
-        if constexpr (FP32) raw_floats<CT>(kr[h][e], a.x);
-        else a.x = operand<CT>(kr[h][e]);
+        Frag<FP32> a[2], q;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[h].x = operand<CT>(kr[h][e]);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-          s[n][h] = mma<FP32, F16>(a, qh[n][e], s[n][h]);
-          if constexpr (QLO) s[n][h] = mma<FP32, F16>(a, ql[n][e], s[n][h]);
+          q.x = sQ[n * KS + e][l];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[n][h] = mma<FP32, F16>(a[h], q, s[n][h]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+          Frag<FP32> a;
+          if constexpr (FP32) raw_floats<CT>(kr[h][e], a.x);
+          else a.x = operand<CT>(kr[h][e]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            s[n][h] = mma<FP32, F16>(a, qh[n][e], s[n][h]);
+            if constexpr (QLO) s[n][h] = mma<FP32, F16>(a, ql[n][e], s[n][h]);
+          }
         }
       }
     }
@@ -440,13 +479,15 @@ __global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
         x[e] = s[n][e / 4][e % 4] * p.scale;
         if constexpr (narrow(CT)) x[e] = __builtin_amdgcn_ldexpf(x[e], (int)((ek[e / 4] >> (8 * (e % 4))) & 255) - 127);
       }
-      if (odd | no[0] | no[1]) {
+      if (__builtin_expect(odd | no[0] | no[1], 0)) {
+        asm volatile("");  // (a branch)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (no[e / 4] || (narrow(CT) && ((ek[e / 4] >> (8 * (e % 4))) & 255) == 255)) x[e] = nan;
       }
       uint32_t hide = 0;
       if (masks) {
+        asm volatile("");
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const bool hidden = !seen_by(tile + 16 * (e / 4) + 4 * g + e % 4, sees[n], lo[n]);
@@ -471,12 +512,14 @@ __global__ __launch_bounds__(kBlock) void paged_tree_kernel(PagedTree p) {
       for (int e = 0; e < 8; ++e) lsum[n] += w[e];
       if constexpr (narrow(CT)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int byte = (int)((ev[e / 4] >> (8 * (e % 4))) & 255);
-          w[e] = __builtin_amdgcn_ldexpf(w[e], byte - 127);
-          // (A scale of a row that is not seen is no number of this column.)
-          if (odd && byte == 255) w[e] = nan;
-          if (masks && ((hide >> e) & 1)) w[e] = 0.f;
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_ldexpf(w[e], (int)((ev[e / 4] >> (8 * (e % 4))) & 255) - 127);
+        if (__builtin_expect(odd, 0)) {
+          asm volatile("");
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (((ev[e / 4] >> (8 * (e % 4))) & 255) == 255) w[e] = nan;
+            if ((hide >> e) & 1) w[e] = 0.f;  // (a scale of a row that is not seen is no number of this column)
+          }
         }
       }
       if constexpr (FP32) {
@@ -653,27 +696,36 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PagedTree p) {
   }
 }
 
-// Columns of a workgroup: 16 for each tile of the products.  Larger groups read the cache less often, and take
-// more registers: four tiles of 16-bit operands, two where queries have two terms or are float32.
-int group_tiles(int M, int dtype, int cache_dtype) {
-  if (M <= 16) return 1;
-  return M <= 32 || dtype == DSQG_F32 || (dtype == DSQG_F16 && narrow(cache_dtype)) ? 2 : 4;
+// Columns of a workgroup: 16 for each tile of the products.  Larger groups read the cache less often, and take more
+// registers: four tiles where a wave's rows on their way and its sums leave room, those of 8-bit caches of up to 96 elements,
+// else two, and two where queries have two terms or are float32.  (16 sequences of up to 8192, 8 key/value heads, 256 columns,
+// e4m3: four 193 us and two 206 at D = 64, 221 and 269 at 96, 364 and 331 at 128; bfloat16 at 64 either 120.)
+constexpr bool four_tiles(int dtype, int cache_dtype, int D) { return dtype == DSQG_BF16 && narrow(cache_dtype) && D <= 96; }
+
+int group_tiles(int M, int dtype, int cache_dtype, int D) {
+  return M <= 16 ? 1 : M <= 32 || !four_tiles(dtype, cache_dtype, D) ? 2 : 4;
 }
 
 long long units_of(const PagedTree& p) { return (long long)p.c.B * p.c.Hkv; }
 
 // Chooses the columns' groups and the split; returns the parts that may have to be joined.
-long long plan(PagedTree& p, int dtype, int cache_dtype) {
-  const int M = p.T * p.G, wide = 16 * group_tiles(M, dtype, cache_dtype);
+long long plan(PagedTree& p, int dtype, int cache_dtype, int D) {
+  const int M = p.T * p.G, wide = 16 * group_tiles(M, dtype, cache_dtype, D);
   p.cols = (M + wide - 1) / wide * wide;
   const long long units = units_of(p), groups = p.cols / wide;
   // The most tiles that a sequence of this table can have.
   long long rows = ((long long)p.c.M << p.c.shift) + p.T;
   if (p.window) rows = std::min(rows, (long long)p.window + p.T + 64 + (p.sinks + 31ll) / 32 * 32);
   const long long tiles = (rows + kTile - 1) / kTile;
-  long long chunk = 4;
-  while (chunk < tiles && chunk * 512 < tiles * units * groups) chunk *= 2;
+  // Parts of two rounds of the waves at least, and as many as give each CU one: the join of more costs what their balance
+  // gives (32 sequences of up to 2048, 12 heads, 26 nodes: 384 parts 42.5 us, 768 and their join 48; 77 tokens: 1 part 8.3 us, 2
+  // and theirs 11).
+  long long chunk = 8;
+  while (chunk < tiles && chunk * 256 < tiles * units * groups) chunk *= 2;
   while ((tiles + chunk - 1) / chunk * groups > 65535) chunk *= 2;  // (the grid's limit)
+  // Parts alike, of whole rounds of the waves.
+  const long long parts = (tiles + chunk - 1) / chunk;
+  chunk = ((tiles + parts - 1) / parts + kWaves - 1) / kWaves * kWaves;
   p.chunk = (int)chunk;
   p.splits = (int)((tiles + chunk - 1) / chunk);
   return p.splits > 1 ? units * p.splits * p.cols : 0;
@@ -687,10 +739,9 @@ void launch(const PagedTree& p, hipStream_t st) {
 
 template <int QT, int CT, int D>
 void launch_groups(const PagedTree& p, int ct, hipStream_t st) {
-  constexpr bool two = QT == DSQG_F32 || (QT == DSQG_F16 && narrow(CT));
-  const int nq = group_tiles(p.T * p.G, QT, ct);
+  const int nq = group_tiles(p.T * p.G, QT, ct, D);
   if (nq == 1) return launch<QT, CT, D, 1>(p, st);
-  if constexpr (!two)
+  if constexpr (four_tiles(QT, CT, D))
     if (nq == 4) return launch<QT, CT, D, 4>(p, st);
   launch<QT, CT, D, 2>(p, st);
 }
@@ -736,7 +787,7 @@ int check_tree(const dsqg_paged_tree_args* a, PagedTree* p, long long* parts) {
   // (No place is 2^30 positions from another, as none is that far from the first.)
   p->window = std::min(a->window, 1 << 30);
   p->sinks = p->window ? std::min(a->sinks, 1 << 30) : 0;
-  *parts = plan(*p, c.dtype, c.cache_dtype);
+  *parts = plan(*p, c.dtype, c.cache_dtype, c.D);
   return *parts < (1ll << 31) ? DSQG_OK : DSQG_EUNSUPPORTED;
 }
 
@@ -798,7 +849,7 @@ extern "C" int dsqg_paged_tree(const dsqg_paged_tree_args* a, dsqg_stream_t stre
   p.words = narrow(c.cache_dtype) && p.c.ksn == 1 && p.c.vsn == 1 && odd % 4 == 0;
   // (As the single-token step's: pools larger than a third of the Infinity Cache.  Groups of columns find each other's
   // rows in L2 only if they stay there.)
-  p.stream = p.cols == 16 * group_tiles(p.T * p.G, c.dtype, c.cache_dtype) &&
+  p.stream = p.cols == 16 * group_tiles(p.T * p.G, c.dtype, c.cache_dtype, c.D) &&
              2ll * c.P * c.Hkv * c.page * c.D * elem_size(c.cache_dtype) > (85ll << 20);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (c.dtype == DSQG_F32) launch_dim<DSQG_F32>(p, c.cache_dtype, c.D, st);
