@@ -17,7 +17,8 @@
 //
 // Weights of groups of 16 columns enter the second product as two 16-bit terms (dsqg_paged_mfma.hip: 2^-16 of the weight),
 // those of larger groups, which arithmetic bounds, as one: a rounding of up to 2^-8 (bfloat16) or 2^-11 (float16) of each
-// weight, of the size of the output's own.  Scores, statistics and sums are fp32.
+// weight, of the size of the output's own.  (float16 queries over 8-bit rows, whose operands are bfloat16: two again, for
+// 2^-8 is more than their output's rounding.)  Scores, statistics and sums are fp32.
 //
 // Measured: 16 sequences of up to 8192, 8 key/value heads of 4, 64 nodes, D = 128 over e4m3, 326 us, 266 TFLOP/s: vector
 // instructions (a weight's and the codes', of which 32 columns share each) and the latency of two waves a SIMD bound it.
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
   constexpr bool FP32 = QT == DSQG_F32;
   constexpr bool F16 = CT == DSQG_F16;                // operands in float16 (else bf16, where they are 16 bits)
   constexpr bool QLO = QT == DSQG_F16 && narrow(CT);  // queries in two terms
-  constexpr bool PLO = !FP32 && NQ == 1;              // weights in two terms
+  constexpr bool PLO = !FP32 && (NQ == 1 || QLO);     // weights in two terms
   constexpr int ES = elem_size(CT), KS = S::count, DB = D / 16;
   // Row stride of staged values, in elements: of 16 bits an odd multiple of eight banks, so that the transposed reads, of four
   // pieces of sixteen rows, meet in none.
