@@ -298,8 +298,8 @@ def paged_tree_step(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor],
     With k_new = v_new = None nothing is written and the draft's rows are attended as the pages hold them.  A
     sequence with pos[b] < 0 gets zeros and writes nothing, a node that sees a position without a page NaN.  A row that a
     node does not see does not reach it, whatever it holds.  The range of values is ``paged_decode_step``'s.  Weights of
-    T * G > 16 tokens and heads are rounded once, to the cache's 16-bit type (8 bits: bfloat16), before they multiply
-    the values.  The step has no gradient.  ``draft_tree_accept`` says which rows to keep.
+    T * G > 16 tokens and heads are rounded once, to the cache's 16-bit type (8 bits: bfloat16; not with float16
+    queries, which keep two terms), before they multiply the values.  The step has no gradient.  ``draft_tree_accept`` says which rows to keep.
     """
     if ops.traced(q, k_pages, v_pages):
         return ops.paged_tree(q, k_new, v_new, k_pages, v_pages, page_table, pos, parents, counts, window, sinks, k_scale,

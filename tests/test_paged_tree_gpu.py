@@ -406,3 +406,22 @@ def test_other_streams_and_traced(gpu_device):
     version = c.k._version
     paged_tree_step(q, None, None, c.k, c.v, c.table, pos, pt)
     assert c.k._version == version
+
+
+@pytest.mark.parametrize("kv", [E4, I8])
+@pytest.mark.parametrize("D", [32, 128])
+def test_float16_over_8_bits(gpu_device, kv, D):
+    """Float16 queries over 8-bit rows: 20 nodes give what 16 of them give, whose weights are two bfloat16 terms.  Both are
+    within 2^-16 of the weights' mass, at most the largest value, and half a step of the output (2^-11 of it) of the exact
+    result, so within 2^-15 max|v| and 2^-10 |x| of each other.  (One term would be off by up to 2^-9 of the mass.)"""
+    pos, G = [300, 45], 1
+    outs = []
+    for T in (20, 16):
+        c = Cache(gpu_device, 2, 2, D, 16, 24, F16, kv, [p + 20 for p in pos])
+        junk(c, pos)
+        g = torch.Generator().manual_seed(9)
+        q, k, v = (torch.randn(2, 2 * n, 20, D, generator=g).to(gpu_device, F16)[:, :, :T] for n in (G, 1, 1))
+        outs.append(paged_tree_step(q, k, v, c.k, c.v, c.table, torch.tensor(pos, device=gpu_device), **c.state).double().cpu()[:, :, :16])
+        largest = max(torch.nan_to_num(c.rows("v", b, pos[b] + 16)).abs().max().item() for b in range(2))
+    x, y = outs
+    assert torch.isfinite(x).all() and ((x - y).abs() <= 2.0 ** -10 * y.abs() + 2.0 ** -15 * largest).all()

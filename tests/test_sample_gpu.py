@@ -321,3 +321,12 @@ def test_split_rows_in_two_graphs(gpu_device):
         for call, out in zip(calls, outs):
             for a, b in zip(call(), out):
                 assert torch.equal(a, b)
+
+
+def test_many_of_few(gpu_device):
+    """A top-k of most of a row that the list holds, and rows a little longer than it."""
+    for V, k in ((3000, 2000), (4096, 1025), (4097, 1024), (6000, 1024)):
+        for dtype in (F32, BF):
+            x, u = rows(6, V, V + k, dtype)
+            check(x, u, 0.9, top_k=k)
+            check(x, u, 0.6, top_k=k, top_p=0.97, min_p=1e-4)
