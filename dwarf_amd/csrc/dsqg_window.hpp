@@ -293,6 +293,16 @@ __device__ __forceinline__ float large_exponent(float s, float c, float m) {
   return s * c - m;
 }
 
+// The reference exponent of a largest score s, whose weight becomes 2^lift.  The score is rounded first, as large_exponent
+// rounds it (in one multiply-add a huge product could end a step below the rounded score, and its weight be 2^128), and float16's
+// lift is left out where that step is so large that less than 2^16 of it could become more: its largest weight is 1 there.
+template <int T>
+__device__ __forceinline__ float reference_exponent(float s, float c, float lift) {
+#pragma clang fp contract(off)
+  const float m = s * c;
+  return T == DSQG_F16 && fabsf(m) >= kLarge ? m : m - lift;
+}
+
 // s to exponents; m(r) of each value.
 template <typename F>
 __device__ __forceinline__ void exponents(float (&s)[16], float c, bool large, F&& m) {

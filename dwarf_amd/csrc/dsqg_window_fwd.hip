@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(Wi
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
       }
-      mx = xor32_pair_max(mx * p.scale2 - lift);
+      mx = xor32_pair_max(reference_exponent<T>(mx, p.scale2, lift));
       if (__any(mx > m)) {
         const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
