@@ -499,7 +499,10 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
       float mx = x[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-      mx = lifted<F16>(col_max(mx));
+      mx = col_max(mx);
+      // (Where a score's step is 8 and more the lift may come out as 16, and a weight as 2^16, which is no single float16 number:
+      // huge scores have no lift.)
+      mx = F16 && !PLO && fabsf(mx) >= 65536.f ? mx : lifted<F16>(mx);
       if (__any(mx > m[n])) {
         const float mn = fmaxf(m[n], mx), a = weight(m[n], mn);
         m[n] = mn;
