@@ -196,6 +196,21 @@ struct Stage {
         *reinterpret_cast<u32x4_t*>(rows + row * X::RB + ((e - row * X::PPR) ^ X::flip(row)) * 16) = x[u];
     }
   }
+  // Times 2^-30.
+  __device__ __forceinline__ void shrink() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = x[u][e];
+        if constexpr (T == DSQG_F32)
+          x[u][e] = __float_as_uint(__uint_as_float(w) * 0x1p-30f);
+        else
+          x[u][e] = (__float_as_uint(__uint_as_float(w & 0xffff0000u) * 0x1p-30f) & 0xffff0000u) |
+                    (__float_as_uint(__uint_as_float(w << 16) * 0x1p-30f) >> 16);
+      }
+    }
+  }
   // Puts zeros in the place of infinities and NaN, which times the weight of a column that does not see them would be no
   // zero (add_odd); says whether this thread's pieces held any.
   __device__ __forceinline__ bool clean() {

@@ -19,21 +19,24 @@
 namespace dsqg {
 namespace {
 
+// One pass of workgroup `workgroup`, with values times 2^-30 where `small`; says whether one of its sums was no number, with
+// nothing written.
 template <int T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(WindowParams p) {
+__device__ __forceinline__ bool window_fwd_pass(const WindowParams& p, int workgroup, int thread, bool small) {
   using X = Tile<T, D>;
   constexpr int RT = T == DSQG_F32 || (D > 64 && NW == 4) ? 32 : 64, KB = RT / 32, TB = X::bytes(RT), kCols = 32 * NW;
   constexpr int BYTES = 4 * TB > NW * out_block<T, D>() ? 4 * TB : NW * out_block<T, D>();
   __shared__ __align__(16) char bytes[BYTES];          // the tiles, in the end the waves' output rows
   auto lds = reinterpret_cast<char(*)[2][TB]>(bytes);  // [which tile][keys, values]
   __shared__ int odd[2];                        // which tile's values hold infinities or NaN, plus one
+  __shared__ int over;                          // whether a sum is no number
 
   // Blocks that read the same keys, the heads of a key/value head, follow each other; the longest come first.
-  const int block = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int block = xcd_logical_block(workgroup, gridDim.x);
   const int g = block % p.G, rest = block / p.G;
   const int at = p.blocks - 1 - rest % p.blocks, bk = rest / p.blocks;
   const int b = bk / p.Hkv, hk = bk - b * p.Hkv, head = hk * p.G + g;
-  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int c = l & 31, h = l >> 5;
   const int length = window_length(p, b);
   const int q0 = at * kCols, i0 = q0 + 32 * wave, i = i0 + c;
@@ -50,7 +53,8 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(Wi
       if (i < length) q[s] = *reinterpret_cast<const u32x4_t*>(row + (2 * X::E * s + X::E * h) * X::O::size);
     }
   }
-  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  if (thread < 2) odd[thread] = 0;
+  if (thread == 0) over = 0;
 
   Stage<T, D, RT, 64 * NW> sk, sv;
   auto load = [&](int t) {
@@ -64,6 +68,7 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(Wi
   };
   auto store = [&](int t) {
     sk.store(lds[t & 1][0]);
+    if (T != DSQG_F16 && small) sv.shrink();
     if (edge(t) && sv.clean()) odd[t & 1] = t + 1;
     sv.store(lds[t & 1][1]);
   };
@@ -149,12 +154,40 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(Wi
     __syncthreads();
   }
 
+  if (T != DSQG_F16 && !small) {
+    float any = 0.f;
+#pragma unroll
+    for (int d = 0; d < X::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (D % 32 == 0 || 32 * d + 8 * (r / 4) < D) any = __builtin_fmaf(o[d][r], 0.f, any);
+    if (any != any) over = 1;
+    __syncthreads();
+    if (over) return true;
+  }
   sum = xor32_pair_sum(sum);
   const bool live = i < length && sum != 0.f;
-  store_columns<T, D>(o, 1.f / sum, live, bytes + wave * out_block<T, D>(),
+  store_columns<T, D>(o, (small ? 0x1p30f : 1.f) / sum, live, bytes + wave * out_block<T, D>(),
                       p.out.at + b * p.out.b + head * p.out.h + i0 * p.out.n, p.out.n, p.N - i0, l);
   if (p.stats && h == 0 && i < p.N)
     p.stats[((long long)b * p.Hkv * p.G + head) * p.N + i] = live ? make_float2(m, 1.f / sum) : make_float2(INFINITY, 0.f);
+  return false;
+}
+
+// Sums of values near the type's largest may pass it where their mean does not.  A workgroup with such a sum (or one that sees an
+// infinity) goes over its tiles once more with values times 2^-30, so that sums of 2^30 rows are finite.
+template <int T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_fwd_kernel(WindowParams p) {
+  if constexpr (T == DSQG_F16) {  // (2^30 of its largest, times 2^14, are far from float32's)
+    window_fwd_pass<T, D, NW>(p, blockIdx.x, threadIdx.x, false);
+    return;
+  }
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int workgroup = blockIdx.x;
+    asm volatile("" : "+s"(workgroup));  // (a second pass finds its places anew: kept, they would take registers)
+    if (!window_fwd_pass<T, D, NW>(p, workgroup, threadIdx.x, pass == 1)) break;
+  }
 }
 
 template <int T, int D, int NW>

@@ -431,7 +431,11 @@ int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
  * reference exponent and the inverse of its weights' sum.  Scores and sums are fp32, in an order that does not change
  * between calls; the weights and, in the backward, their gradients are rounded once to a 16-bit dtype before they multiply
  * rows.  A row that a query does not see does not reach its output, whatever it holds, nor a row of a query that does not
- * see a key that key's gradients. */
+ * see a key that key's gradients.
+ *
+ * Outputs are finite where the values are, up to 2^-7 below the type's largest.  Weights are kept relative to the largest: a row
+ * that weighs less than 2^-96 of the heaviest (2^-38 in float16) weighs nothing, and gives an infinity or NaN where its value is
+ * infinite. */
 typedef struct {
     int32_t dtype;             /* DSQG_F32, DSQG_BF16 or DSQG_F16 */
     int32_t B, H, Hkv, N, D;

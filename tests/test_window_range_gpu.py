@@ -1,10 +1,10 @@
-"""Attention within a window on the GPU at the ends of its range: huge scores."""
+"""Attention within a window on the GPU at the ends of its range: huge scores, the largest values."""
 
 import pytest
 import torch
 
 from oracle import window_oracle as wo
-from tests.test_window_gpu import BF, F16, F32, inputs, run
+from tests.test_window_gpu import BF, F16, F32, check, inputs, run
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,18 @@ def test_huge_scores(gpu_device, dtype, power):
     out = got["out"][0, 0].cpu()
     assert sure.sum() > 200 and torch.equal(out[sure], v[0, 0][s.argmax(-1)][sure])
     assert all(torch.isfinite(x).all() for x in got.values())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("D", [32, 80, 128])
+@pytest.mark.parametrize("flat", [True, False])
+def test_largest_values(gpu_device, dtype, D, flat):
+    """Values of half the type's largest to 0.95 of it, of one sign in each element: their means are as large, and finite."""
+    q, k, v, dout = inputs(2, 2, 1, 300, D, dtype)
+    sign = torch.where(torch.arange(D) % 3 == 0, -1.0, 1.0)
+    v = (sign * (1.0 + 0.9 * torch.rand(2, 1, 300, D, generator=torch.Generator().manual_seed(D)))).to(dtype)
+    v = v * 2.0 ** (15 if dtype == F16 else 127)
+    # (Gradients pass by products of dout with those, which are to be numbers too.)
+    got = check(q * (0.0 if flat else 1.0), k, v, dout * 2.0 ** (-10 if dtype == F16 else -20), 200, 3, lengths=[300, 77])
+    assert all(torch.isfinite(x).all() for x in got.values())
+    assert got["out"][0].float().abs().amin() >= (2.0 ** 15 if dtype == F16 else 2.0 ** 127) * (1 - 2.0 ** -7)
