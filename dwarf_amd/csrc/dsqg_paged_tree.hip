@@ -13,7 +13,8 @@
 // Masks are needed in few tiles: those that hold rows of the draft and, with a window, those where it begins and the sinks'.
 // There a node's ancestors are one 64-bit word, found by doubling pointers over the wave (lane j: node j).  A value
 // that some columns of such a tile do not see must not reach them, not even as 0 times an infinity: where a tile with
-// masks holds infinities or NaN, its second product runs a column at a time, the other's values taken out.
+// masks holds infinities or NaN, its second product runs a column at a time, the other's values taken out.  8 bits have the NaN
+// of e4m3 alone (which no writer here makes): a zero takes its place in the product, and the sums that see it are NaN in the end.
 //
 // Weights of groups of 16 columns enter the second product as two 16-bit terms (dsqg_paged_mfma.hip: 2^-16 of the weight),
 // those of larger groups, which arithmetic bounds, as one: a rounding of up to 2^-8 (bfloat16) or 2^-11 (float16) of each
@@ -109,6 +110,9 @@ __device__ __forceinline__ bool odd_values(uint4 v) {
   return odd;
 }
 
+// NaN among four e4m3 codes (0x7f with either sign): a byte's top bit is set where its other seven are, as one added to them carries.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Whether a group's queries are read from LDS for each tile, where they would take 32 registers of a wave or more.
 constexpr bool queries_in_lds(int QT, int CT, int D, int NQ) {
   return QT != DSQG_F32 && !(QT == DSQG_F16 && narrow(CT)) && NQ * ((D + 31) / 32) >= 8;
@@ -129,6 +133,9 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
   typedef typename std::conditional<FP32, float, bf16_t>::type val_t;
   __shared__ __align__(16) val_t sV[kWaves][kTile * RV];
   __shared__ float wm[kWaves][16], wl[kWaves][16];
+  // e4m3: which elements of a lane's sums see a NaN in a tile with masks.
+  __shared__ uint32_t sees_nan[CT == DSQG_E4M3 ? kWaves : 1][NQ][64];
+  static_assert(4 * DB <= 32, "a bit for each");
   constexpr bool QLDS = queries_in_lds(QT, CT, D, NQ);
   __shared__ uint4 sQ[QLDS ? NQ * KS : 1][QLDS ? 64 : 1];  // a lane's fragments
 
@@ -372,10 +379,53 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
     return j < 0 ? t >= from || t < p.sinks : j < 64 && ((mask >> j) & 1);
   };
 
+  // e4m3: zeros in the place of the NaN among the tile's value rows, and marks for the sums that see them.
+  auto take_nan = [&](int tile) {
+    asm volatile("");  // (a branch)
+    uint32_t odd = 0;
+#pragma unroll
+    for (int u = 0; u < V::passes; ++u)
+#pragma unroll
+      for (int w = 0; w < V::per_lane; ++w) odd |= nan_codes(vr[u][w].x) | nan_codes(vr[u][w].y) | nan_codes(vr[u][w].z) | nan_codes(vr[u][w].w);
+    if (!__any(odd != 0)) return;
+#pragma unroll
+    for (int u = 0; u < V::passes; ++u) {
+#pragma unroll
+      for (int w = 0; w < V::per_lane; ++w) {
+        const int row = u * V::rows + l / V::lanes, piece = l % V::lanes + V::lanes * w;
+        uint32_t x[4] = {vr[u][w].x, vr[u][w].y, vr[u][w].z, vr[u][w].w}, gone = 0;  // a bit for each of the piece's codes
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t at = nan_codes(x[q]) >> 7;
+          x[q] &= ~(at * 255u);
+          gone |= ((at & 1u) | (at >> 7 & 2u) | (at >> 14 & 4u) | (at >> 21 & 8u)) << (4 * q);
+        }
+        vr[u][w] = make_uint4(x[0], x[1], x[2], x[3]);
+        if (piece >= V::pieces) gone = 0;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll 1
+          for (int c = 0; c < 16; ++c) {
+            const u64 mask = __shfl(sees[n], c, 64);
+            const int from = __shfl(lo[n], c, 64);
+            // Element 16 d + 4 g + e of column c is the sum o[n][d][e] of lane 16 g + c.
+            if (seen_by(tile + row, mask, from))
+              for (uint32_t rest = gone; rest; rest &= rest - 1) {
+                const int b = __builtin_ctz(rest);
+                atomicOr(&sees_nan[wave][n][16 * (b >> 2) + c], 1u << (4 * piece + (b & 3)));
+              }
+          }
+        }
+      }
+    }
+  };
+
   // The tile's value rows to LDS as operand values, zeros in the place of those that nobody sees; says whether an
   // infinity or NaN is among the others of a tile with masks.
   auto stage = [&](int tile, bool masks) {
     bool odd = false;
+    if constexpr (CT == DSQG_E4M3)
+      if (masks) take_nan(tile);
 #pragma unroll
     for (int u = 0; u < V::passes; ++u) {
       const int row = u * V::rows + l / V::lanes;
@@ -421,6 +471,10 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
     for (int d = 0; d < DB; ++d) o[n][d] = zero4();
   }
   const float nan = __uint_as_float(0x7fc00000u);
+  if constexpr (CT == DSQG_E4M3) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) sees_nan[wave][n][l] = 0;
+  }
 
   if (first < v1) load(0);
 #pragma unroll 1
@@ -560,7 +614,7 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
       }
       return f;
     };
-    if (!odd_rows) {
+    if (narrow(CT) || !odd_rows) {
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         const Frag<FP32> x = values(d);
@@ -597,6 +651,18 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
           }
         }
       }
+    }
+  }
+
+  if constexpr (CT == DSQG_E4M3) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const uint32_t in = sees_nan[wave][n][l];
+      if (!__any(in != 0)) continue;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] += (in >> (4 * d + e)) & 1 ? nan : 0.f;
     }
   }
 

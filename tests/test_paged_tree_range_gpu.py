@@ -1,4 +1,4 @@
-"""Drafted-token steps on the GPU at the ends of their range: huge scores."""
+"""Drafted-token steps on the GPU at the ends of their range: huge scores, NaN codes of 8-bit pages."""
 
 import pytest
 import torch
@@ -41,3 +41,43 @@ def test_huge_scores(gpu_device, dtype, kv, T, power):
                 want = vv[sees[int(s.argmax())]]
                 assert ((out[b, 0, i] - want).abs() <= want.abs() * (2.0 ** -16 + torch.finfo(dtype).eps / 2)).all(), (b, i)
     assert sure > 3 * T
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("T,G", [(12, 1), (30, 1), (50, 2)])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_nan_codes_stay_with_who_sees_them(gpu_device, dtype, D, T, G, code):
+    """Pages from elsewhere may hold e4m3's NaN under an ordinary scale: the nodes that see its row get NaN in that element, and
+    everything else is what it was, bit by bit (a hidden row's weight is 0 and its value no part of the sums)."""
+    n, parents = 75, tree(T, 4)
+    nodes = po.tree_rows(parents, T)
+    c = Cache(gpu_device, 1, 2, D, 16, 9, dtype, E4, [n + T])
+    q = torch.randn(1, 2 * G, T, D, generator=torch.Generator().manual_seed(1)).to(dtype).to(gpu_device)
+    pt, pos = torch.tensor(parents, device=gpu_device), torch.tensor([n], device=gpu_device)
+
+    def call(**kw):
+        return paged_tree_step(q, None, None, c.k, c.v, c.table, pos, pt, **kw, **c.state).cpu()
+
+    for at, kw in ((n + 3, {}), (n + T - 1, {}), (n - 9, dict(window=12, sinks=2)), (3, dict(window=40, sinks=5)), (n + 2, dict(window=3))):
+        hit = torch.tensor([at in po.tree_sees(node, nodes, n, kw.get("window"), kw.get("sinks", 0)) for node in nodes])
+        want = call(**kw)
+        assert torch.isfinite(want).all()
+        cell = c.v.view(torch.uint8)[int(c.table[0, at // 16]), 1, at % 16]
+        old = cell.clone()
+        cell[7] = cell[D - 1] = code
+        got = call(**kw)
+        cell.copy_(old)
+        want[:, G:, hit, 7] = want[:, G:, hit, D - 1] = torch.nan
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), (at, kw)
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0)), (at, kw)
+        assert not hit.all() or at == 3
+        # A key's scores are NaN, and so all of such a node's output.
+        cell = c.k.view(torch.uint8)[int(c.table[0, at // 16]), 1, at % 16]
+        old = cell.clone()
+        cell[5] = code
+        got = call(**kw)
+        cell.copy_(old)
+        want[:, G:, hit] = torch.nan
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), (at, kw)
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0)), (at, kw)
