@@ -1151,6 +1151,15 @@ Tensor node_table(const Tensor& t, at::ScalarType dt) {
   return x.numel() == 0 || x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous();
 }
 
+// Parents, of any integer type: numbers past the nodes' are brought to one that is no node, before 32 bits make another of them.
+Tensor parent_table(const Tensor& t) {
+  const auto dt = t.scalar_type();
+  if (dt != at::kLong && dt != at::kUInt32 && dt != at::kUInt64) return node_table(t, at::kInt);
+  Tensor x = t.to(at::kLong);
+  if (dt == at::kUInt64) x = x.masked_fill(x < 0, DSQG_MAX_TREE);
+  return node_table(x.clamp(-2, DSQG_MAX_TREE), at::kInt);
+}
+
 // Shapes of a tree: parents [T] or [B,T], counts [B] or none.
 void check_tree(const Tensor& parents, const OptTensor& counts, int64_t B, int64_t T) {
   require(at::isIntegralType(parents.scalar_type(), false) &&
@@ -1177,7 +1186,7 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& tokens0, const Tens
   const c10::Device dev = require_gpu({&tokens0, &parents0, &picks0});
   if (counts0) require_gpu({&tokens0, &*counts0});
   const c10::OptionalDeviceGuard guard(dev);
-  const Tensor tokens = node_table(tokens0, at::kLong), parents = node_table(parents0, at::kInt), picks = node_table(picks0, at::kLong);
+  const Tensor tokens = node_table(tokens0, at::kLong), parents = parent_table(parents0), picks = node_table(picks0, at::kLong);
   const Tensor counts = counts0 ? counts0->to(at::kLong).contiguous() : Tensor();
   const auto o = tokens.options().dtype(at::kLong);
   const Tensor path = at::empty({B, T}, o), n = at::empty({B}, o), next = at::empty({B}, o);
@@ -1230,7 +1239,7 @@ Tensor paged_tree(const Tensor& q0, const OptTensor& k0, const OptTensor& v0, co
   if (parents0) require_gpu({&kp, &*parents0});
   const c10::OptionalDeviceGuard guard(c.dev);
   const Tensor q = plain_rows(q0), pos = c.index(pos0, "pos");
-  const Tensor parents = parents0 ? node_table(*parents0, at::kInt) : Tensor();
+  const Tensor parents = parents0 ? parent_table(*parents0) : Tensor();
   const Tensor counts = counts0 ? c.index(*counts0, "counts") : Tensor();
   const Tensor k = kn.defined() ? plain_rows(kn) : kn, v = vn.defined() ? plain_rows(vn) : vn;
   // Token-major storage: the callers' head merge is a view.

@@ -1,9 +1,9 @@
-"""Drafted-token steps on the GPU at the ends of their range: huge scores, NaN codes of 8-bit pages."""
+"""Drafted-token steps on the GPU at the ends of their range: huge scores, NaN codes of 8-bit pages, parents past 32 bits."""
 
 import pytest
 import torch
 
-from dwarf_amd import paged_tree_step
+from dwarf_amd import draft_tree_accept, paged_tree_step
 from oracle import paged_oracle as po
 from tests.test_paged_gpu import Cache
 from tests.test_paged_tree_gpu import BF, E4, F16, F32, tree
@@ -81,3 +81,36 @@ def test_nan_codes_stay_with_who_sees_them(gpu_device, dtype, D, T, G, code):
         want[:, G:, hit] = torch.nan
         assert torch.equal(torch.isnan(got), torch.isnan(want)), (at, kw)
         assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0)), (at, kw)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_parents_past_32_bits(gpu_device, shared):
+    """64-bit parents that 32 bits would make a node of: such nodes, and those below them, are none."""
+    T, wrong = 12, [2 ** 32, 2 ** 32 - 1, -2 ** 32 - 1, 2 ** 40 + 1, -2 ** 63, 2 ** 63 - 1]
+    parents = tree(T, 2)
+    for i, w in zip((1, 3, 5, 6, 8, 11), wrong):
+        parents[i] = w
+    small = [p if -1 <= p < T else -2 for p in parents]
+    assert sum(x is None for x in po.tree_rows(parents, T)) >= 6
+    c = Cache(gpu_device, 2, 1, 64, 16, 6, BF, lengths=[40 + T, 5 + T])
+    q, k, v = (torch.randn(2, 1, T, 64, generator=torch.Generator().manual_seed(i)).to(BF).to(gpu_device) for i in range(3))
+    pos = torch.tensor([40, 5], device=gpu_device)
+    tokens = torch.zeros(2, T, dtype=torch.int64, device=gpu_device)
+
+    def table(p, dtype):
+        return torch.tensor(p if shared else [p, p], dtype=dtype).to(gpu_device)
+
+    want = paged_tree_step(q, k, v, c.k, c.v, c.table, pos, table(small, torch.int32))
+    for i, node in enumerate(po.tree_rows(parents, T)):
+        assert (want[:, :, i] == 0).all() == (node is None)
+    assert torch.equal(paged_tree_step(q, k, v, c.k, c.v, c.table, pos, table(parents, torch.int64)), want)
+    for a, b in zip(draft_tree_accept(tokens, table(parents, torch.int64), tokens), draft_tree_accept(tokens, table(small, torch.int32), tokens)):
+        assert torch.equal(a, b)
+    # Unsigned ones: -1 is their largest number, no node.
+    line = [0, 0, 1, 2 ** 32 - 1, 2, 2 ** 32 - 2]
+    for dtype, more in ((torch.uint32, 0), (torch.uint64, 2 ** 64 - 2 ** 32)):
+        big = [x + more if x > 99 else x for x in line]
+        p = table(big + [0] * (T - 6), torch.uint64).to(dtype)
+        path, n, _ = draft_tree_accept(tokens, p, tokens)
+        assert path[:, :4].tolist() == [[0, 1, 2, 4]] * 2 and n.tolist() == [4, 4]
+        assert (paged_tree_step(q, k, v, c.k, c.v, c.table, pos, p) == 0).all()
