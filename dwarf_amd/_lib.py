@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DSQG_HIP_LIB", PKG_DIR / "libdsqg_hip.so"))
 
 MAX_OFFSETS = 64
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 DSQG_OK, DSQG_EINVAL, DSQG_EUNSUPPORTED, DSQG_EHIP, DSQG_EWORKSPACE = 0, 1, 2, 3, 4
 DSQG_ETOOLARGE = 5
@@ -156,13 +156,14 @@ class WindowShape(ctypes.Structure):
 
 class WindowFwdArgs(ctypes.Structure):
     _fields_ = [("shape", WindowShape), ("q", _vp), ("q_stride", _i64x3), ("k", _vp), ("k_stride", _i64x3),
-                ("v", _vp), ("v_stride", _i64x3), ("out", _vp), ("out_stride", _i64x3), ("stats", _vp)]
+                ("v", _vp), ("v_stride", _i64x3), ("out", _vp), ("out_stride", _i64x3), ("stats", _vp),
+                ("low", _vp), ("low_stride", _i64x3)]
 
 
 class WindowBwdArgs(ctypes.Structure):
     _fields_ = [("shape", WindowShape), ("q", _vp), ("q_stride", _i64x3), ("k", _vp), ("k_stride", _i64x3),
                 ("v", _vp), ("v_stride", _i64x3), ("out", _vp), ("out_stride", _i64x3),
-                ("dout", _vp), ("dout_stride", _i64x3), ("stats", _vp),
+                ("dout", _vp), ("dout_stride", _i64x3), ("stats", _vp), ("low", _vp), ("low_stride", _i64x3),
                 ("dq", _vp), ("dq_stride", _i64x3), ("dk", _vp), ("dk_stride", _i64x3),
                 ("dv", _vp), ("dv_stride", _i64x3), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 

@@ -1048,8 +1048,8 @@ dsqg_window_shape window_shape(const Tensor& q, const Tensor& k, const Tensor& v
   return s;
 }
 
-// (out, stats); stats is undefined unless asked for.
-std::tuple<Tensor, Tensor> run_window_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& lengths0, int64_t window,
+// (out, stats, low); stats and low, what out's rounding to 16 bits took off, are undefined unless asked for.
+std::tuple<Tensor, Tensor, Tensor> run_window_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& lengths0, int64_t window,
                                           int64_t sinks, std::optional<double> scale, bool with_stats) {
   dsqg_window_fwd_args a = {};
   a.shape = window_shape(q0, k0, v0, lengths0, window, sinks, scale);
@@ -1065,19 +1065,25 @@ std::tuple<Tensor, Tensor> run_window_fwd(const Tensor& q0, const Tensor& k0, co
   a.v = ptr(v); set_strides(a.v_stride, v);
   a.out = ptr(out); set_strides(a.out_stride, out);
   a.stats = static_cast<float*>(ptr(stats));
+  const Tensor low = with_stats && a.shape.dtype != DSQG_F32 ? token_major(q) : Tensor();
+  if (low.defined()) {
+    a.low = ptr(low);
+    set_strides(a.low_stride, low);
+  }
   check(api.window_fwd(&a, stream_of(dev)), "dsqg_window_fwd");
-  return {out, stats};
+  return {out, stats, low};
 }
 
 std::tuple<Tensor, Tensor, Tensor> run_window_bwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& lengths0,
-                                                  const Tensor& out0, const Tensor& stats, const Tensor& dout0, int64_t window,
-                                                  int64_t sinks, std::optional<double> scale) {
+                                                  const Tensor& out0, const Tensor& stats, const Tensor& low0, const Tensor& dout0,
+                                                  int64_t window, int64_t sinks, std::optional<double> scale) {
   dsqg_window_bwd_args a = {};
   a.shape = window_shape(q0, k0, v0, lengths0, window, sinks, scale);
-  const c10::Device dev = require_gpu({&q0, &k0, &v0, &lengths0, &out0, &stats, &dout0});
+  const c10::Device dev = require_gpu({&q0, &k0, &v0, &lengths0, &out0, &stats, &low0, &dout0});
   const c10::OptionalDeviceGuard guard(dev);
   const Tensor q = window_rows(q0), k = window_rows(k0), v = window_rows(v0), out = window_rows(out0);
   const Tensor dout = window_rows(dout0.to(q.scalar_type()));
+  const Tensor low = low0.defined() ? window_rows(low0) : low0;
   const Tensor lengths = lengths0.defined() ? lengths0.to(at::kLong).contiguous() : lengths0;
   const Tensor dq = token_major(q), dk = token_major(k), dv = token_major(v);
   a.shape.lengths = static_cast<const int64_t*>(ptr(lengths));
@@ -1087,6 +1093,10 @@ std::tuple<Tensor, Tensor, Tensor> run_window_bwd(const Tensor& q0, const Tensor
   a.out = ptr(out); set_strides(a.out_stride, out);
   a.dout = ptr(dout); set_strides(a.dout_stride, dout);
   a.stats = static_cast<const float*>(ptr(stats));
+  if (low.defined()) {
+    a.low = ptr(low);
+    set_strides(a.low_stride, low);
+  }
   a.dq = ptr(dq); set_strides(a.dq_stride, dq);
   a.dk = ptr(dk); set_strides(a.dk_stride, dk);
   a.dv = ptr(dv); set_strides(a.dv_stride, dv);
@@ -1102,8 +1112,8 @@ std::tuple<Tensor, Tensor, Tensor> run_window_bwd(const Tensor& q0, const Tensor
 struct WindowFunction : torch::autograd::Function<WindowFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths, int64_t window,
                         int64_t sinks, std::optional<double> scale) {
-    const auto [out, stats] = run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
-    ctx->save_for_backward({q, k, v, undef(lengths), out, stats});
+    const auto [out, stats, low] = run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
+    ctx->save_for_backward({q, k, v, undef(lengths), out, stats, low});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale ? *scale : 1.0 / std::sqrt((double)q.size(3));
@@ -1113,7 +1123,7 @@ struct WindowFunction : torch::autograd::Function<WindowFunction> {
     if (at::GradMode::is_enabled())
       raise(PyExc_RuntimeError, "window_attention has no second derivative: call backward without create_graph");
     const variable_list s = ctx->get_saved_variables();
-    const auto [dq, dk, dv] = run_window_bwd(s[0], s[1], s[2], s[3], s[4], s[5], g[0], ctx->saved_data["window"].toInt(),
+    const auto [dq, dk, dv] = run_window_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], g[0], ctx->saved_data["window"].toInt(),
                                              ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -1130,17 +1140,18 @@ Tensor window(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor
   return WindowFunction::apply(q, k, v, lengths, window, sinks, scale);
 }
 
-std::tuple<Tensor, Tensor> window_fwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths, int64_t window,
-                                         int64_t sinks, std::optional<double> scale) {
+std::tuple<Tensor, Tensor, Tensor> window_fwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths,
+                                                 int64_t window, int64_t sinks, std::optional<double> scale) {
   py::gil_scoped_release nogil;
-  return run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
+  const auto [out, stats, low] = run_window_fwd(q, k, v, undef(lengths), window, sinks, scale, true);
+  return {out, stats, low.defined() ? low : at::empty({0}, out.options())};
 }
 
 std::tuple<Tensor, Tensor, Tensor> window_bwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths,
-                                                 const Tensor& out, const Tensor& stats, const Tensor& dout, int64_t window,
-                                                 int64_t sinks, std::optional<double> scale) {
+                                                 const Tensor& out, const Tensor& stats, const OptTensor& low, const Tensor& dout,
+                                                 int64_t window, int64_t sinks, std::optional<double> scale) {
   py::gil_scoped_release nogil;
-  return run_window_bwd(q, k, v, undef(lengths), out, stats, dout, window, sinks, scale);
+  return run_window_bwd(q, k, v, undef(lengths), out, stats, undef(low), dout, window, sinks, scale);
 }
 
 // ---- Drafted tokens and sampling. ----------------------------------------------------------------------------------

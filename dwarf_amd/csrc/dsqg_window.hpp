@@ -37,6 +37,7 @@ struct WindowParams {
   float scale, scale2;         // softmax_scale, and times log2(e)
   const long long* lengths;    // or null: N
   WindowRows q, k, v, out, dout, dq, dk, dv;
+  WindowRows low;              // what out's rounding took off (low_part), or null
   float2* stats;               // [B, H, N]: the weights' reference exponent and 1 / sum (forward: or null)
   float* delta;                // [B, H, N]: dout . out
   int waves, blocks;           // waves of a workgroup, 32 queries each; query blocks of a head
@@ -356,12 +357,23 @@ __device__ __forceinline__ void hide(float x, const Seen& seen, bool sinks, int 
   }
 }
 
+// What the rounding of x to 16 bits takes off, in float16 times 2^11, which keeps it as far from the subnormal numbers as x is.
+// (None where the result is no number.)
+template <int T> constexpr float low_scale() { return T == DSQG_F16 ? 2048.f : 1.f; }
+template <int T>
+__device__ __forceinline__ float low_part(float x) {
+  float low;
+  if constexpr (T == DSQG_F16) low = (x - (float)(_Float16)x) * low_scale<T>();
+  else low = x - __uint_as_float(cvt_pk_bf16(x, 0.f) << 16);
+  return fabsf(low) < INFINITY ? low : 0.f;
+}
+
 // A wave's 32 columns [D x 32] to rows of an output, times f (of each column), through the wave's LDS block (out_block bytes);
-// n rows are stored, of columns that are not live zeros.
+// n rows are stored, of columns that are not live zeros.  LOW: what their rounding takes off, in their place.
 template <int T, int D>
 constexpr int out_block() { return 32 * (D * Op<T>::size + 16); }
 
-template <int T, int D>
+template <int T, int D, bool LOW = false>
 __device__ __forceinline__ void store_columns(const Acc<T, D>& acc, float f, bool live, char* block, char* out,
                                               long long stride, int n, int l) {
   using X = Tile<T, D>;
@@ -374,7 +386,10 @@ __device__ __forceinline__ void store_columns(const Acc<T, D>& acc, float f, boo
       if (D % 32 != 0 && at >= D) continue;
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = live ? acc[d][4 * g + e] * f : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = live ? acc[d][4 * g + e] * f : 0.f;
+        if constexpr (LOW) x[e] = low_part<T>(x[e]);
+      }
       char* to = block + c * (out_block<T, D>() / 32) + at * X::O::size;
       if constexpr (T == DSQG_F32) {
         *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};

@@ -1,6 +1,11 @@
 // Attention within a window and its sinks, backward (gfx950).
 //
 //   p_ij = 2^(scale2 q_i.k_j - m_i) / sum_i,   D_i = dout_i . out_i,   dS_ij = p_ij (dout_i . v_j - D_i)
+//
+// (out as the forward summed it: its 16-bit value and what the rounding took off.  From the 16-bit value alone D_i is off by more
+// than all of dS_ij where a query has nearly all its weight on one key: dq and dk by 0.0055 of their norm with a window of 2 in
+// bfloat16, against 0.0023 so and the 0.0017 that the results' own rounding is.)
+//
 //   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i p_ij dout_i
 //
 // Two launches, neither of which needs an atomic: dq with a wave's 32 queries as columns, over the tiles of keys and values
@@ -74,18 +79,21 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(Win
   const long long stat = ((long long)b * p.Hkv * p.G + head) * p.N + i;
 
   u32x4_t q[X::KS], dout[X::KS];
-  float delta = 0.f;
+  float delta = 0.f, lost = 0.f;
   {
     const char* const rq = p.q.at + b * p.q.b + head * p.q.h + (long long)i * p.q.n;
     const char* const rd = p.dout.at + b * p.dout.b + head * p.dout.h + (long long)i * p.dout.n;
     const char* const ro = p.out.at + b * p.out.b + head * p.out.h + (long long)i * p.out.n;
+    const char* const rl = p.low.at + b * p.low.b + head * p.low.h + (long long)i * p.low.n;
 #pragma unroll
     for (int s = 0; s < X::KS; ++s) {
       const int e = (2 * X::E * s + X::E * h) * X::O::size;
       q[s] = frag_or_zero(rq + e, i < length);
       dout[s] = frag_or_zero(rd + e, i < length);
       delta = dot_frag<T>(dout[s], frag_or_zero(ro + e, i < length), delta);
+      if (T != DSQG_F32) lost = dot_frag<T>(dout[s], frag_or_zero(rl + e, i < length && p.low.at), lost);
     }
+    if (T != DSQG_F32) delta += lost * (1.f / low_scale<T>());
     delta = xor32_pair_sum(delta);
   }
   float2 st = make_float2(INFINITY, 0.f);
@@ -697,6 +705,7 @@ extern "C" int dsqg_window_fwd(const dsqg_window_fwd_args* a, dsqg_stream_t stre
       !rows(a->out, a->out_stride, &p.out) || (reinterpret_cast<uintptr_t>(a->stats) & 7u) != 0)
     return DSQG_EINVAL;
   p.stats = reinterpret_cast<float2*>(a->stats);
+  if (a->low && (s.dtype == DSQG_F32 || !rows(a->low, a->low_stride, &p.low))) return DSQG_EINVAL;
   return launch_window_fwd(p, s.dtype, reinterpret_cast<hipStream_t>(stream)) == hipSuccess ? DSQG_OK : DSQG_EHIP;
 }
 
@@ -720,6 +729,7 @@ extern "C" int dsqg_window_bwd(const dsqg_window_bwd_args* a, dsqg_stream_t stre
       !rows(a->dk, a->dk_stride, &p.dk) || !rows(a->dv, a->dv_stride, &p.dv) || !a->stats ||
       (reinterpret_cast<uintptr_t>(a->stats) & 7u) != 0)
     return DSQG_EINVAL;
+  if (a->low && (s.dtype == DSQG_F32 || !rows(a->low, a->low_stride, &p.low))) return DSQG_EINVAL;
   if (!a->workspace || a->workspace_bytes < delta_bytes(s) + part_bytes(p)) return DSQG_EWORKSPACE;
   if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return DSQG_EINVAL;
   p.stats = reinterpret_cast<float2*>(const_cast<float*>(a->stats));

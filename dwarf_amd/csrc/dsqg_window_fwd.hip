@@ -169,6 +169,10 @@ __device__ __forceinline__ bool window_fwd_pass(const WindowParams& p, int workg
   const bool live = i < length && sum != 0.f;
   store_columns<T, D>(o, (small ? 0x1p30f : 1.f) / sum, live, bytes + wave * out_block<T, D>(),
                       p.out.at + b * p.out.b + head * p.out.h + i0 * p.out.n, p.out.n, p.N - i0, l);
+  if constexpr (T != DSQG_F32)
+    if (p.low.at)
+      store_columns<T, D, true>(o, (small ? 0x1p30f : 1.f) / sum, live, bytes + wave * out_block<T, D>(),
+                                p.low.at + b * p.low.b + head * p.low.h + i0 * p.low.n, p.low.n, p.N - i0, l);
   if (p.stats && h == 0 && i < p.N)
     p.stats[((long long)b * p.Hkv * p.G + head) * p.N + i] = live ? make_float2(m, 1.f / sum) : make_float2(INFINITY, 0.f);
   return false;

@@ -725,39 +725,42 @@ def _(q, k_new, v_new, k_pages, v_pages, page_table, pos, k_scale, v_scale, soft
 
 @torch.library.custom_op("dwarf::window_fwd", mutates_args=())
 def window_fwd(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: int, sinks: int,
-               softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
-    """out [B,H,N,D] (token-major storage) and, for the backward, stats [B,H,N,2] fp32."""
+               softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
+    """out [B,H,N,D] (token-major storage) and, for the backward, stats [B,H,N,2] fp32 and low, what out's rounding to 16
+    bits took off (as out; float32: empty)."""
     return _lib.host().window_fwd(q, k, v, lengths, window, sinks, softmax_scale)
 
 
 @window_fwd.register_fake
 def _(q, k, v, lengths, window, sinks, softmax_scale):
     B, H, N, D = q.shape
-    return q.new_empty((B, N, H, D)).permute(0, 2, 1, 3), q.new_empty((B, H, N, 2), dtype=torch.float32)
+    out = q.new_empty((B, N, H, D)).permute(0, 2, 1, 3)
+    return out, q.new_empty((B, H, N, 2), dtype=torch.float32), q.new_empty((0,)) if q.dtype == torch.float32 else torch.empty_like(out)
 
 
 @torch.library.custom_op("dwarf::window_bwd", mutates_args=())
 def window_bwd(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], out: Tensor, stats: Tensor, dout: Tensor,
-               window: int, sinks: int, softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
-    """(dq, dk, dv), token-major storage; out and stats are the forward's."""
-    return _lib.host().window_bwd(q, k, v, lengths, out, stats, dout, window, sinks, softmax_scale)
+               window: int, sinks: int, softmax_scale: Optional[float],
+               low: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv), token-major storage; out, stats and low are the forward's."""
+    return _lib.host().window_bwd(q, k, v, lengths, out, stats, low, dout, window, sinks, softmax_scale)
 
 
 @window_bwd.register_fake
-def _(q, k, v, lengths, out, stats, dout, window, sinks, softmax_scale):
+def _(q, k, v, lengths, out, stats, dout, window, sinks, softmax_scale, low=None):
     return tuple(t.new_empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3])).permute(0, 2, 1, 3) for t in (q, k, v))
 
 
 def _window_setup_context(ctx, inputs, output):
     q, k, v, lengths, ctx.window, ctx.sinks, ctx.scale = inputs
-    out, stats = output
-    ctx.save_for_backward(q, k, v, lengths, out, stats)
-    ctx.mark_non_differentiable(stats)
+    out, stats, low = output
+    ctx.save_for_backward(q, k, v, lengths, out, stats, low)
+    ctx.mark_non_differentiable(stats, low)
 
 
-def _window_backward(ctx, dout, _dstats):
-    q, k, v, lengths, out, stats = ctx.saved_tensors
-    dq, dk, dv = window_bwd(q, k, v, lengths, out, stats, dout, ctx.window, ctx.sinks, ctx.scale)
+def _window_backward(ctx, dout, _dstats, _dlow):
+    q, k, v, lengths, out, stats, low = ctx.saved_tensors
+    dq, dk, dv = window_bwd(q, k, v, lengths, out, stats, dout, ctx.window, ctx.sinks, ctx.scale, low if low.numel() else None)
     return dq, dk, dv, None, None, None, None
 
 

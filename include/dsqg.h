@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DSQG_ABI_VERSION 8
+#define DSQG_ABI_VERSION 9
 #define DSQG_MAX_OFFSETS 64
 
 /* Same type as hipStream_t; NULL is the null stream. */
@@ -428,7 +428,9 @@ int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
  * 16-byte aligned, and a row stride of at least D elements and less than 2^24 bytes.
  *
  * stats [B,H,N,2] (float, contiguous, 8-byte aligned; the forward's may be NULL) holds, for the backward, each query's
- * reference exponent and the inverse of its weights' sum.  Scores and sums are fp32, in an order that does not change
+ * reference exponent and the inverse of its weights' sum, and low [B,H,N,D], of the inputs' 16-bit dtype, what out's rounding
+ * took off (float16: times 2^11).  The backward takes dout . out from both; where low is NULL, from out alone, whose rounding
+ * then shows in dq and dk: 3.5 times the error where a query sees few keys.  Scores and sums are fp32, in an order that does not change
  * between calls; the weights and, in the backward, their gradients are rounded once to a 16-bit dtype before they multiply
  * rows.  A row that a query does not see does not reach its output, whatever it holds, nor a row of a query that does not
  * see a key that key's gradients.
@@ -451,6 +453,7 @@ typedef struct {
     const void* v;  int64_t v_stride[3];
     void* out;      int64_t out_stride[3];
     float* stats;
+    void* low;      int64_t low_stride[3];     /* 16-bit dtypes, or NULL */
 } dsqg_window_fwd_args;
 
 int dsqg_window_fwd(const dsqg_window_fwd_args* args, dsqg_stream_t stream);
@@ -463,6 +466,7 @@ typedef struct {
     const void* out;   int64_t out_stride[3];
     const void* dout;  int64_t dout_stride[3];
     const float* stats;
+    const void* low;   int64_t low_stride[3];  /* 16-bit dtypes, or NULL */
     void* dq;  int64_t dq_stride[3];
     void* dk;  int64_t dk_stride[3];
     void* dv;  int64_t dv_stride[3];

@@ -40,3 +40,22 @@ def test_largest_values(gpu_device, dtype, D, flat):
     got = check(q * (0.0 if flat else 1.0), k, v, dout * 2.0 ** (-10 if dtype == F16 else -20), 200, 3, lengths=[300, 77])
     assert all(torch.isfinite(x).all() for x in got.values())
     assert got["out"][0].float().abs().amin() >= (2.0 ** 15 if dtype == F16 else 2.0 ** 127) * (1 - 2.0 ** -7)
+
+
+def far_off(got, ref):
+    """|got - ref| over |ref|, 2-norms."""
+    return ((got.double().cpu() - ref).norm() / ref.norm()).item()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("D", [32, 80, 128])
+@pytest.mark.parametrize("window,sinks", [(1, 1), (2, 0), (3, 0), (8, 1)])
+def test_gradients_of_few_keys(gpu_device, dtype, D, window, sinks):
+    """Three roundings make dq and dk, of at most half a step e each: the result's, dS's, and the weights' behind dout . out.
+    Even ones from -e to e are e / sqrt(3) in the mean, and three of them e.  (Were dout . out taken from the rounded output, its
+    error of e |dout||out| / sqrt(D) would be larger than the dS of queries with nearly all their weight on one key.)"""
+    q, k, v, dout = inputs(1, 2, 1, 600, D, dtype)
+    got = run(q, k, v, dout, window, sinks)
+    ref, _ = wo.forward_backward(q, k, v, dout, window, sinks)
+    for n in ("dq", "dk", "dv"):
+        assert far_off(got[n], ref[n]) <= torch.finfo(dtype).eps / 2, n
