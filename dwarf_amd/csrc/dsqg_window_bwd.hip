@@ -17,8 +17,8 @@
 // where the others take a window.  Its queries beyond the window are split over further workgroups, and a third
 // launch adds the parts.
 //
-// p and dS enter the products rounded to the 16-bit type (2^-8 of each in bfloat16, 2^-11 in float16); float32 operands are not
-// rounded.  Everything else is fp32.
+// p and dS enter the products rounded to the 16-bit type (2^-8 of each in bfloat16, 2^-11 in float16, where factors keep them in
+// its range); float32 operands are not rounded.  Everything else is fp32.
 //
 // Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, dq 365 us, dk/dv 485 us, 565 TFLOP/s of the seven products; B8 H8
 // Hkv1 N2048 D32 window 256 with 4 sinks, dq 30 us, dk/dv 43 us, their parts' sum 4.6 us.  Vector instructions bound both: a
@@ -55,6 +55,47 @@ __device__ __forceinline__ float dot_frag(u32x4_t a, u32x4_t b, float s) {
   }
   return s;
 }
+
+// float16 operands end at 65504 and lose bits below 2^-14, where loss scales and long windows bring dS past either: it is packed
+// times a power of two of its column, which its largest so far chooses (2^13 to 2^15 then) as the forward's running maximum
+// does, and the column's sum is taken back by it.  p, at most 1, is packed times 2^14.
+constexpr float kNoFactor = 0x1p120f;  // before the first
+template <int T> constexpr float weight_factor() { return T == DSQG_F16 ? 0x1p14f : 1.f; }
+
+// The column's factor for sixteen more values a lane.
+__device__ __forceinline__ float next_factor(const float (&x)[16], float c) {
+  float mx = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(x[r]));
+  mx = xor32_pair_max(mx);
+  if (__any(mx * c > 0x1p15f)) {
+    const uint32_t e = max(__float_as_uint(mx) >> 23, 27u);  // (2^-100 at least)
+    const float next = __uint_as_float((267u - e) << 23);    // 2^13 over mx's power of two
+    c = mx * c > 0x1p15f ? next : c;
+  }
+  return c;
+}
+
+// next / c of two powers of two, next the smaller.
+__device__ __forceinline__ float factor_ratio(float next, float c) {
+  const int e = (int)(__float_as_uint(next) >> 23) - (int)(__float_as_uint(c) >> 23) + 127;
+  return e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.f;
+}
+
+template <int N>
+__device__ __forceinline__ void refactor(f32x16_t (&acc)[N], float& c, float next) {
+  if (__any(next != c)) {
+    const float f = factor_ratio(next, c);
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+    c = next;
+  }
+}
+
+// 1 / c, and what else a sum is multiplied by in the end.
+__device__ __forceinline__ float unfactor(float c, float f) { return __uint_as_float((254u << 23) - __float_as_uint(c)) * f; }
 
 template <int T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(WindowParams p) {
@@ -120,6 +161,7 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(Win
   Acc<T, D> acc;
 #pragma unroll
   for (int d = 0; d < X::DB; ++d) acc[d] = zero_tile();
+  float factor = T == DSQG_F16 ? kNoFactor : 1.f;
 
   __syncthreads();
   if (span.n > 0) {
@@ -151,6 +193,11 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(Win
         float no[1];
         hide<T>(0.f, seen, k0 < p.sinks, h, w, no);
       }
+      if constexpr (T == DSQG_F16) {
+        refactor(acc, factor, next_factor(w, factor));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] *= factor;
+      }
       Weights<T> f;
       pack<T>(w, f);
       contract<T, D>(acc, kt, l, f);
@@ -162,7 +209,7 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(Win
     }
     __syncthreads();
   }
-  store_columns<T, D>(acc, p.scale, i < length, bytes + wave * out_block<T, D>(),
+  store_columns<T, D>(acc, unfactor(factor, p.scale), i < length, bytes + wave * out_block<T, D>(),
                       p.dq.at + b * p.dq.b + head * p.dq.h + i0 * p.dq.n, p.dq.n, p.N - i0, l);
 }
 
@@ -270,7 +317,7 @@ __global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void wind
     sd.store(lds[t & 1][1]);
     if (threadIdx.x < RT) {
       rows[t & 1][0][threadIdx.x] = st.x;
-      rows[t & 1][1][threadIdx.x] = st.y;
+      rows[t & 1][1][threadIdx.x] = st.y * weight_factor<T>();
       rows[t & 1][2][threadIdx.x] = de;
       if (fabsf(st.x) >= kLarge && st.x != INFINITY) odd[t & 1][2] = t + 1;
     }
@@ -279,6 +326,7 @@ __global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void wind
   Acc<T, D> dk, dv;
 #pragma unroll
   for (int d = 0; d < X::DB; ++d) dk[d] = dv[d] = zero_tile();
+  float factor = T == DSQG_F16 ? kNoFactor : 1.f;
 
   __syncthreads();
   if (steps > 0) {
@@ -327,6 +375,11 @@ __global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void wind
       Weights<T> f;
       pack<T>(w, f);
       contract<T, D>(dv, dt, l, f);
+      if constexpr (T == DSQG_F16) {
+        refactor(dk, factor, next_factor(x, factor));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= factor;
+      }
       pack<T>(x, f);
       contract<T, D>(dk, qt, l, f);
       const int head = hk * p.G + t / tiles;
@@ -342,6 +395,7 @@ __global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void wind
     __syncthreads();
   }
 
+  const float fk = unfactor(factor, 1.f / weight_factor<T>()), fv = 1.f / weight_factor<T>();
   if (at < p.split) {
     float* const to = p.part + ((((long long)bk * p.split + at) * (1 + p.far) + part) * 2 * KC + 32 * wave + c) * D;
 #pragma unroll
@@ -350,14 +404,14 @@ __global__ __launch_bounds__(kBlock, D <= 32 && T != DSQG_F32 ? 3 : 2) void wind
       for (int g = 0; g < 4; ++g) {
         const int e = 32 * d + 8 * g + 4 * h;
         if (D % 32 != 0 && e >= D) continue;
-        *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
-        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+        *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]} * fk;
+        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]} * fv;
       }
     return;
   }
   char* const mine = lds[0][0] + wave * out_block<T, D>();
-  store_columns<T, D>(dk, p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
-  store_columns<T, D>(dv, 1.f, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
+  store_columns<T, D>(dk, fk * p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
+  store_columns<T, D>(dv, fv, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
 }
 
 // Eight waves for 128 keys: a key's scores and weights take registers for its own key and value, its sums for two rows of
@@ -373,6 +427,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
   constexpr int RT = 32, TB = X::bytes(RT), kPairs = key_pairs(T, D), KC = 32 * kPairs;
   __shared__ __align__(16) char lds[kSteps][2][TB];       // [which tile][queries, dout]
   __shared__ __align__(16) u32x4_t ops[2][kPairs][2 * X::C][64];  // p and dS of a step
+  __shared__ float factors[2][kPairs][T == DSQG_F16 ? 64 : 1];    // ... dS's columns' factors
   __shared__ __align__(16) float rows[kSteps][3][RT];     // ... [reference exponent, 1 / sum, D]
   __shared__ int odd[kSteps][3];                          // ... queries, dout hold infinities or NaN; exponents are large
   static_assert(kSteps * 2 * TB >= kPairs * out_block<T, D>(), "the waves' output rows fit the tiles");
@@ -421,7 +476,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
     sd.store(lds[at][1]);
     if (threadIdx.x < RT) {
       rows[at][0][threadIdx.x] = st.x;
-      rows[at][1][threadIdx.x] = st.y;
+      rows[at][1][threadIdx.x] = st.y * weight_factor<T>();
       rows[at][2][threadIdx.x] = de;
       if (fabsf(st.x) >= kLarge && st.x != INFINITY) odd[at][2] = t + 1;
     }
@@ -454,6 +509,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
       }
     }
     int place = 0, tile = 0;
+    float factor = T == DSQG_F16 ? kNoFactor : 1.f;
 #pragma unroll 1
     for (int t = 0; t <= steps; ++t) {
       const int i0 = (first + tile) * RT;
@@ -490,6 +546,12 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
         pack<T>(w, f);
 #pragma unroll
         for (int e = 0; e < X::C; ++e) ops[t & 1][pair][e][l] = f[e];
+        if constexpr (T == DSQG_F16) {
+          factor = next_factor(x, factor);
+          factors[t & 1][pair][l] = factor;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] *= factor;
+        }
         pack<T>(x, f);
 #pragma unroll
         for (int e = 0; e < X::C; ++e) ops[t & 1][pair][X::C + e][l] = f[e];
@@ -508,6 +570,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
   Acc<T, D> dk, dv;
 #pragma unroll
   for (int d = 0; d < X::DB; ++d) dk[d] = dv[d] = zero_tile();
+  float factor = T == DSQG_F16 ? kNoFactor : 1.f;
   int place = 0, last = 0, tile = 0, was = 0, head = hk * p.G;  // of step t, and of the step before
 #pragma unroll 1
   for (int t = 0; t <= steps; ++t) {
@@ -521,6 +584,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
       contract<T, D>(dv, dt, l, f);
 #pragma unroll
       for (int e = 0; e < X::C; ++e) f[e] = ops[(t - 1) & 1][pair][X::C + e][l];
+      if constexpr (T == DSQG_F16) refactor(dk, factor, factors[(t - 1) & 1][pair][l]);
       contract<T, D>(dk, qt, l, f);
       if (odd[last][0] == t)
         add_odd<T, D>(dk, p.q.at + b * p.q.b + head * p.q.h + i0 * p.q.n, p.q.n, length - i0, l, seen_of(i0));
@@ -539,6 +603,7 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
     __syncthreads();
   }
 
+  const float fk = unfactor(factor, 1.f / weight_factor<T>()), fv = 1.f / weight_factor<T>();
   if (at < p.split) {
     float* const to = p.part + ((((long long)bk * p.split + at) * (1 + p.far) + part) * 2 * KC + 32 * pair + c) * D;
 #pragma unroll
@@ -547,14 +612,14 @@ __global__ __launch_bounds__((dkdv_threads<T, D>()), key_pairs(T, D) == 4 ? 2 : 
       for (int g = 0; g < 4; ++g) {
         const int e = 32 * d + 8 * g + 4 * h;
         if (D % 32 != 0 && e >= D) continue;
-        *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
-        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+        *reinterpret_cast<f32x4_t*>(to + e) = f32x4_t{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]} * fk;
+        *reinterpret_cast<f32x4_t*>(to + KC * D + e) = f32x4_t{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]} * fv;
       }
     return;
   }
   char* const mine = lds[0][0] + pair * out_block<T, D>();
-  store_columns<T, D>(dk, p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
-  store_columns<T, D>(dv, 1.f, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
+  store_columns<T, D>(dk, fk * p.scale, j < length, mine, p.dk.at + b * p.dk.b + hk * p.dk.h + j0 * p.dk.n, p.dk.n, p.N - j0, l);
+  store_columns<T, D>(dv, fv, j < length, mine, p.dv.at + b * p.dv.b + hk * p.dv.h + j0 * p.dv.n, p.dv.n, p.N - j0, l);
 }
 
 // Sums of the sinks' key blocks over their parts.  Grid: [B * Hkv * split * kcols / 8, 2], a thread four elements.

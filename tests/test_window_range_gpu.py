@@ -59,3 +59,39 @@ def test_gradients_of_few_keys(gpu_device, dtype, D, window, sinks):
     ref, _ = wo.forward_backward(q, k, v, dout, window, sinks)
     for n in ("dq", "dk", "dv"):
         assert far_off(got[n], ref[n]) <= torch.finfo(dtype).eps / 2, n
+
+
+@pytest.mark.parametrize("size", [1e-4, 1.0, 1e3])
+@pytest.mark.parametrize("D,G", [(32, 1), (64, 2), (80, 1), (128, 2)])
+@pytest.mark.parametrize("sinks", [0, 4])
+def test_float16_gradients_of_any_size(gpu_device, size, D, G, sinks):
+    """A long window's weights and small gradients lie far below float16's normal numbers: both are brought up before they are
+    rounded, so that the errors are those of ``test_gradients_of_few_keys``, and for dv those of two roundings."""
+    q, k, v, dout = inputs(1, G, 1, 1500, D, F16)
+    dout = (dout.float() * size).half()
+    got = run(q, k, v, dout, 1024, sinks)
+    ref, _ = wo.forward_backward(q, k, v, dout, 1024, sinks)
+    # (Results below 2^-14 are off by half their smallest step, 2^-25, each.)
+    for n in ("dq", "dk", "dv"):
+        assert far_off(got[n], ref[n]) <= torch.finfo(F16).eps / 2 + 2.0 ** -25 * ref[n].numel() ** 0.5 / ref[n].norm(), n
+
+
+@pytest.mark.parametrize("D", [32, 80, 128])
+def test_float16_gradients_past_the_largest_on_the_way(gpu_device, D):
+    """Score gradients above 65504 in front of small keys and queries: the results fit."""
+    q, k, v, dout = inputs(1, 2, 1, 400, D, F16)
+    q, k, v, dout = (x.float() * f for x, f in ((q, 2.0 ** -6), (k, 2.0 ** -6), (v, 16.0), (dout, 2e3)))
+    dout[:, :, 200:] *= 2.0 ** -12  # and others that are small, before and behind them
+    dout[:, :, :100] *= 2.0 ** -20
+    q, k, v, dout = (x.half() for x in (q, k, v, dout))
+    ref, _ = wo.forward_backward(q, k, v, dout, 3, 1)
+    # (Weights of three keys are a third each, more or less: a score's gradient, that of dout . v's distance from their mean.)
+    dp = torch.stack([(dout[0, 0, i].double() * v[0, 0, i - 2:i + 1].double()).sum(-1) for i in range(100, 200)])
+    assert ((dp - dp.mean(1, keepdim=True)).abs() / 3 > 65504).sum() > 20
+    assert all(x.abs().max() < 65504 for x in ref.values())
+    got = run(q, k, v, dout, 3, 1)
+    for n in ("dq", "dk", "dv"):
+        assert far_off(got[n], ref[n]) <= torch.finfo(F16).eps / 2, n
+        for rows in (slice(2, 90), slice(220, 400)):  # rows of small gradients on their own
+            a, b = got[n][:, :, rows], ref[n][:, :, rows]
+            assert far_off(a, b) <= torch.finfo(F16).eps / 2 + 2.0 ** -25 * b.numel() ** 0.5 / b.norm(), (n, rows)
