@@ -1082,11 +1082,25 @@ size_t lay_out(Sample* p, int B, char* at) {
   return used;
 }
 
+// Rows of a launch: a grid has less than 2^32 lanes.
+constexpr int kRows = 1 << 21;
+
 template <int DT>
 void launch(const Sample& p, int B, hipStream_t st) {
   const dim3 block(kThreads);
   if (p.S == 1) {
-    hipLaunchKernelGGL(sample_kernel<DT>, dim3((unsigned)B), block, 0, st, p);
+    for (long long b = 0; b < B; b += kRows) {
+      Sample q = p;
+      q.x += b * p.xs;
+      q.u = static_cast<const char*>(p.u) + b * (p.u64bits ? 8 : 4);
+      q.out += b;
+      if (q.logp) q.logp += b;
+      if (q.temperatures) q.temperatures += b;
+      if (q.top_ks) q.top_ks += b;
+      if (q.top_ps) q.top_ps += b;
+      if (q.min_ps) q.min_ps += b;
+      hipLaunchKernelGGL(sample_kernel<DT>, dim3((unsigned)std::min<long long>(B - b, kRows)), block, 0, st, q);
+    }
     return;
   }
   const dim3 grid((unsigned)(B * p.S));
