@@ -847,7 +847,8 @@ int check_tree(const dsqg_paged_tree_args* a, PagedTree* p, long long* parts) {
   if (c.Hkv > 0 ? a->H == 0 || a->H % c.Hkv != 0 : a->H != 0) return DSQG_EINVAL;
   if (a->T > DSQG_MAX_TREE) return DSQG_EUNSUPPORTED;
   if ((long long)c.B * a->H == 0) return DSQG_OK;
-  if ((long long)c.B * a->H * a->T >= (1ll << 30)) return DSQG_EUNSUPPORTED;  // the join's grid
+  // (The grid has less than 2^32 lanes in x.  The join's does: parts are for less than 256 groups of columns in all.)
+  if ((long long)c.B * a->H * a->T >= (1ll << 30) || (long long)c.B * c.Hkv >= (1ll << 24) - 8) return DSQG_EUNSUPPORTED;
   // Offsets inside a page, and from page to page, are 32 bits.
   if (p->c.kn * c.page >= (1ll << 31) || p->c.vn * c.page >= (1ll << 31) || p->c.kp >= (1ll << 31) || p->c.vp >= (1ll << 31))
     return DSQG_EUNSUPPORTED;
@@ -857,6 +858,8 @@ int check_tree(const dsqg_paged_tree_args* a, PagedTree* p, long long* parts) {
   // (No place is 2^30 positions from another, as none is that far from the first.)
   p->window = std::min(a->window, 1 << 30);
   p->sinks = p->window ? std::min(a->sinks, 1 << 30) : 0;
+  const int wide = 16 * group_tiles(p->T * p->G, c.dtype, c.cache_dtype, c.D);
+  if ((p->T * p->G + wide - 1) / wide > 65535) return DSQG_EUNSUPPORTED;  // (the grid in y, with a part for each)
   *parts = plan(*p, c.dtype, c.cache_dtype, c.D);
   return *parts < (1ll << 31) ? DSQG_OK : DSQG_EUNSUPPORTED;
 }

@@ -59,7 +59,7 @@ using namespace dsqg;
 
 extern "C" int dsqg_tree_accept(const dsqg_tree_accept_args* a, dsqg_stream_t stream) {
   if (!a || a->B < 0 || a->T < 1) return DSQG_EINVAL;
-  if (a->T > DSQG_MAX_TREE) return DSQG_EUNSUPPORTED;
+  if (a->T > DSQG_MAX_TREE || a->B >= 1 << 26) return DSQG_EUNSUPPORTED;  // (a grid has less than 2^32 lanes)
   if (a->B == 0) return DSQG_OK;
   if (!a->tokens || !a->parents || !a->picks || !a->path || !a->n || !a->next) return DSQG_EINVAL;
   for (long long s : {a->tokens_stride, a->parents_stride, a->picks_stride})

@@ -703,15 +703,18 @@ hipError_t launch_window_bwd(const WindowParams& p, int dtype, hipStream_t st) {
 
 namespace {
 
-// The checks that all entry points share.
-int check_window(const dsqg_window_shape& s, WindowParams* p) {
+// The checks that all entry points share, and the split.
+int check_window(const dsqg_window_shape& s, WindowParams* p, bool backward) {
   if (s.dtype != DSQG_F32 && s.dtype != DSQG_BF16 && s.dtype != DSQG_F16) return DSQG_EINVAL;
   if (s.B < 0 || s.H < 0 || s.Hkv < 0 || s.N < 0 || s.D <= 0 || s.window < 1 || s.sinks < 0) return DSQG_EINVAL;
   if (s.Hkv > 0 ? s.H == 0 || s.H % s.Hkv != 0 : s.H != 0) return DSQG_EINVAL;
   if (!head_dim_supported(s.D)) return DSQG_EUNSUPPORTED;
   *p = WindowParams{};
   p->B = s.B; p->Hkv = s.Hkv; p->N = s.N; p->D = s.D;
-  if ((long long)s.B * s.H * s.N == 0) return DSQG_OK;
+  if (s.B == 0 || s.H == 0 || s.N == 0) return DSQG_OK;
+  // Positions plus a window are 32 bits, grids less than 2^32 lanes.
+  constexpr long long lanes = 1ll << 32;
+  if (s.N > (1 << 30) || (long long)s.B * s.H >= lanes / 256) return DSQG_EUNSUPPORTED;
   p->G = s.H / s.Hkv;
   p->window = std::min(s.window, 1 << 30);
   p->sinks = std::min(s.sinks, 1 << 30);
@@ -722,8 +725,7 @@ int check_window(const dsqg_window_shape& s, WindowParams* p) {
   // Eight waves of 32 queries share a tile where that leaves two workgroups for each CU, else four (may_be_wide).
   p->waves = may_be_wide(s.dtype, s.D) && (long long)s.B * s.H * ((s.N + 255ll) / 256) >= 512 ? 8 : 4;
   p->blocks = (s.N + 32 * p->waves - 1) / (32 * p->waves);
-  // The grids, and positions plus a window in 32 bits.
-  if (s.N > (1 << 30) || (long long)s.B * s.H * (s.N / 64ll + 64) >= (1ll << 31)) return DSQG_EUNSUPPORTED;
+  if ((long long)s.B * s.H * p->blocks * (64 * p->waves) >= lanes) return DSQG_EUNSUPPORTED;
   // The sinks' far queries: shares of a quarter of the queries that other blocks see, which fill the places that those leave
   // free at the end; 64 of them at most.
   const int kc = p->kcols = 32 * key_pairs(s.dtype, s.D);
@@ -733,6 +735,11 @@ int check_window(const dsqg_window_shape& s, WindowParams* p) {
     p->split = (std::min(p->sinks, s.N) + kc - 1) / kc;
     const long long share = std::max(64, (p->window + kc) / 4);
     p->far = (int)std::min((beyond + share - 1) / share, std::max(1ll, 64ll / p->split));
+  }
+  if (backward) {
+    const long long heads = (long long)s.B * s.Hkv, threads = s.D > kSingle ? 4 * kc : kBlock;
+    if (heads * (p->kblocks + (long long)p->split * p->far) * threads >= lanes || heads * p->split * (kc / 8) * kBlock >= lanes)
+      return DSQG_EUNSUPPORTED;
   }
   return DSQG_OK;
 }
@@ -763,8 +770,8 @@ extern "C" int dsqg_window_fwd(const dsqg_window_fwd_args* a, dsqg_stream_t stre
   if (!a) return DSQG_EINVAL;
   WindowParams p;
   const dsqg_window_shape& s = a->shape;
-  if (const int st = check_window(s, &p)) return st;
-  if ((long long)s.B * s.H * s.N == 0) return DSQG_OK;
+  if (const int st = check_window(s, &p, false)) return st;
+  if (s.B == 0 || s.H == 0 || s.N == 0) return DSQG_OK;
   auto rows = [&](const void* ptr, const int64_t st[3], WindowRows* r) { return rows_of(ptr, st, s.dtype, s.D, s.N, r); };
   if (!rows(a->q, a->q_stride, &p.q) || !rows(a->k, a->k_stride, &p.k) || !rows(a->v, a->v_stride, &p.v) ||
       !rows(a->out, a->out_stride, &p.out) || (reinterpret_cast<uintptr_t>(a->stats) & 7u) != 0)
@@ -777,8 +784,8 @@ extern "C" int dsqg_window_fwd(const dsqg_window_fwd_args* a, dsqg_stream_t stre
 extern "C" int dsqg_window_bwd_workspace_size(const dsqg_window_shape* s, size_t* bytes) {
   WindowParams p;
   if (!s || !bytes) return DSQG_EINVAL;
-  if (const int st = check_window(*s, &p)) return st;
-  *bytes = (long long)s->B * s->H * s->N == 0 ? 0 : delta_bytes(*s) + part_bytes(p);
+  if (const int st = check_window(*s, &p, true)) return st;
+  *bytes = s->B == 0 || s->H == 0 || s->N == 0 ? 0 : delta_bytes(*s) + part_bytes(p);
   return DSQG_OK;
 }
 
@@ -786,8 +793,8 @@ extern "C" int dsqg_window_bwd(const dsqg_window_bwd_args* a, dsqg_stream_t stre
   if (!a) return DSQG_EINVAL;
   WindowParams p;
   const dsqg_window_shape& s = a->shape;
-  if (const int st = check_window(s, &p)) return st;
-  if ((long long)s.B * s.H * s.N == 0) return DSQG_OK;
+  if (const int st = check_window(s, &p, true)) return st;
+  if (s.B == 0 || s.H == 0 || s.N == 0) return DSQG_OK;
   auto rows = [&](const void* ptr, const int64_t st[3], WindowRows* r) { return rows_of(ptr, st, s.dtype, s.D, s.N, r); };
   if (!rows(a->q, a->q_stride, &p.q) || !rows(a->k, a->k_stride, &p.k) || !rows(a->v, a->v_stride, &p.v) ||
       !rows(a->out, a->out_stride, &p.out) || !rows(a->dout, a->dout_stride, &p.dout) || !rows(a->dq, a->dq_stride, &p.dq) ||

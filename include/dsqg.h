@@ -423,8 +423,9 @@ int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
  *
  * q, out and their gradients are [B,H,N,D], k, v and theirs [B,Hkv,N,D], H a multiple of Hkv.  With lengths given, rows
  * i >= lengths[b] are not there: nothing sees them, and their outputs and gradients are zeros.  D is one of
- * dsqg_supported_head_dims (EUNSUPPORTED otherwise), window at least 1, sinks at least 0, N at most 2^30 and B * H * (N / 64 +
- * 64) less than 2^31 (EUNSUPPORTED).  Every tensor has unit inner stride, strides {b, h, n} and a base that keep rows
+ * dsqg_supported_head_dims (EUNSUPPORTED otherwise), window at least 1, sinks at least 0, N at most 2^30, and grids have less
+ * than 2^32 lanes: B * H * ceil(N / 128) less than 2^24 and, in the backward, B * Hkv * (N / 64 + 33) less than 2^21 always do,
+ * larger ones may not (EUNSUPPORTED).  Every tensor has unit inner stride, strides {b, h, n} and a base that keep rows
  * 16-byte aligned, and a row stride of at least D elements and less than 2^24 bytes.
  *
  * stats [B,H,N,2] (float, contiguous, 8-byte aligned; the forward's may be NULL) holds, for the backward, each query's
@@ -485,7 +486,7 @@ int dsqg_window_bwd(const dsqg_window_bwd_args* args, dsqg_stream_t stream);
  *     path[b,0..n[b]-1]: the nodes on the way, -1 behind them;  next[b]: the last one's pick
  *
  * A sequence without nodes has n = 0 and next = -1.  tokens and picks have unit inner stride, path [B,T], n [B] and
- * next [B] are contiguous; T is at most DSQG_MAX_TREE (EUNSUPPORTED otherwise). */
+ * next [B] are contiguous; T is at most DSQG_MAX_TREE and B less than 2^26 (EUNSUPPORTED otherwise). */
 #define DSQG_MAX_TREE 64
 
 typedef struct {
@@ -519,8 +520,8 @@ int dsqg_tree_accept(const dsqg_tree_accept_args* args, dsqg_stream_t stream);
  * pos[b] < 0 is not in use: zeros, and nothing is written.  A node that sees a position without a page gets NaN.  A row
  * that a node does not see does not reach it, whatever it holds.  The range of values is dsqg_paged_decode's; its rules
  * for strides, q_stride {b, h, t} and so on, and workspace hold; out is contiguous [B,T,H,D].  Weights enter the sum as
- * two 16-bit terms where T * H / Hkv is at most 16, else as one (16-bit queries).  T is at most DSQG_MAX_TREE and B * H * T
- * less than 2^30 (EUNSUPPORTED otherwise).  No two sequences may have the same page at positions that a step writes. */
+ * two 16-bit terms where T * H / Hkv is at most 16, else as one (16-bit queries).  T is at most DSQG_MAX_TREE, B * H * T
+ * less than 2^30, B * Hkv less than 2^24 - 8 and T * H / Hkv at most 2^21 - 32 (EUNSUPPORTED otherwise).  No two sequences may have the same page at positions that a step writes. */
 typedef struct {
     dsqg_paged_cache cache;
     int32_t H, T;
