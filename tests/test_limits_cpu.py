@@ -48,6 +48,22 @@ def test_window_backwards_past_the_grid():
                     assert size(dtype=dtype, D=D, B=most, H=1, Hkv=1, N=N, window=1, sinks=sinks) == _lib.DSQG_OK
 
 
+def test_what_rounding_took_off():
+    """The 16-bit rest of the output: rows like any other's, and none for float32."""
+    lib = _lib.load()
+    f, b = _lib.WindowFwdArgs(), _lib.WindowBwdArgs()
+    _fill(f, ("q", "k", "v", "out", "low"))
+    _fill(b, ("q", "k", "v", "out", "dout", "low", "dq", "dk", "dv"))
+    b.stats, b.workspace, b.workspace_bytes = 0x10000, 0x10000, 1 << 60
+    for a, call in ((f, lib.dsqg_window_fwd), (b, lib.dsqg_window_bwd)):
+        a.shape = _shape(dtype=_lib.DSQG_F32)
+        assert call(ctypes.byref(a), None) == _lib.DSQG_EINVAL
+        a.shape, a.low = _shape(), 0x10008
+        assert call(ctypes.byref(a), None) == _lib.DSQG_EINVAL
+        a.low, a.low_stride[2] = 0x10000, 32
+        assert call(ctypes.byref(a), None) == _lib.DSQG_EINVAL
+
+
 def test_trees_past_the_grid():
     lib, n = _lib.load(), ctypes.c_size_t(0)
 

@@ -1,4 +1,5 @@
-"""Drafted-token steps on the GPU at the ends of their range: huge scores, NaN codes of 8-bit pages, parents past 32 bits."""
+"""Drafted-token steps on the GPU at the ends of their range: huge scores, NaN codes of 8-bit pages, parents past 32
+bits, pools beyond the caches."""
 
 import pytest
 import torch
@@ -114,3 +115,33 @@ def test_parents_past_32_bits(gpu_device, shared):
         path, n, _ = draft_tree_accept(tokens, p, tokens)
         assert path[:, :4].tolist() == [[0, 1, 2, 4]] * 2 and n.tolist() == [4, 4]
         assert (paged_tree_step(q, k, v, c.k, c.v, c.table, pos, p) == 0).all()
+
+
+@pytest.mark.parametrize("dtype,kv", [(BF, BF), (F16, E4), (F32, F32)])
+@pytest.mark.parametrize("T", [1, 13])
+def test_pools_beyond_the_caches(gpu_device, dtype, kv, T):
+    """Rows of pools above 85 MiB are read past the caches' retention: the same bits as from a small pool."""
+    D, page, pos = 64, 64, [500, 77, 260]
+    c = Cache(gpu_device, 3, 2, D, page, 10, dtype, kv, [p + T for p in pos])
+    P = (86 << 20) // (2 * 2 * page * D * kv.itemsize) + 1  # (two pools of two heads)
+    at = torch.randperm(P, generator=torch.Generator().manual_seed(3))[:c.P].to(gpu_device)
+    big = {}
+    for n in ("k", "v", "k_scale", "v_scale"):
+        x = getattr(c, n)
+        if x is not None:
+            as_bytes = (lambda t: t.view(torch.uint8)) if x.element_size() == 1 else (lambda t: t)
+            big[n] = torch.zeros(P, *x.shape[1:], dtype=as_bytes(x).dtype, device=gpu_device)
+            big[n][at] = as_bytes(x)
+            big[n] = big[n].view(x.dtype)
+    inside = (c.table >= 0) & (c.table < c.P)
+    table = torch.where(inside, at[c.table.clamp(0, c.P - 1).long()].int(), -1)
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(3, h, T, D, generator=g).to(dtype).to(gpu_device) for h in (4, 2, 2))
+    p, pt = torch.tensor(pos, device=gpu_device), torch.tensor([tree(T, b) for b in range(3)], device=gpu_device)
+    for kw in ({}, dict(window=100, sinks=3)):
+        want = paged_tree_step(q, k, v, c.k, c.v, c.table, p, pt, **kw, **c.state)
+        got = paged_tree_step(q, k, v, big["k"], big["v"], table, p, pt, **kw, k_scale=big.get("k_scale"), v_scale=big.get("v_scale"))
+        assert torch.equal(got, want) and torch.isfinite(got).all()
+        for n in big:
+            a, b = (t.view(torch.uint8) if t.element_size() == 1 else t for t in (big[n], getattr(c, n)))
+            assert torch.equal(a[at], b)

@@ -1,4 +1,5 @@
-"""Attention within a window on the GPU at the ends of its range: huge scores, the largest values."""
+"""Attention within a window on the GPU at the ends of its range: huge scores, the largest values, few keys, float16's
+small and large gradients, and batches whose workgroups have eight waves."""
 
 import pytest
 import torch
@@ -95,3 +96,29 @@ def test_float16_gradients_past_the_largest_on_the_way(gpu_device, D):
         for rows in (slice(2, 90), slice(220, 400)):  # rows of small gradients on their own
             a, b = got[n][:, :, rows], ref[n][:, :, rows]
             assert far_off(a, b) <= torch.finfo(F16).eps / 2 + 2.0 ** -25 * b.numel() ** 0.5 / b.norm(), (n, rows)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("D", [80, 96, 128])
+@pytest.mark.parametrize("window,sinks", [(40, 3), (7, 0), (300, 0)])
+def test_many_short_heads(gpu_device, dtype, D, window, sinks):
+    """Rows above 64 elements of 16 bits in 512 and more blocks of 256 queries: workgroups of eight waves, in the forward and for dq."""
+    B, H, N = 32, 16, 130
+    assert B * H * -(-N // 256) >= 512
+    lengths = [N - 4 * b if b % 3 else N for b in range(B)]
+    check(*inputs(B, H, 4, N, D, dtype), window, sinks, lengths)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (F16, 80)])
+def test_long_rows_of_eight_waves(gpu_device, dtype, D):
+    """... whose queries are several blocks, with tiles in front of the window and sinks beyond it; a few heads of them."""
+    B, H, N, window, sinks = 8, 16, 1100, 150, 70
+    assert B * H * -(-N // 256) >= 512
+    q, k, v, dout = inputs(B, H, 4, N, D, dtype)
+    got = run(q, k, v, dout, window, sinks)
+    for b, hk in ((0, 0), (5, 3)):
+        ref, tol = wo.forward_backward(q[b:b + 1, 4 * hk:4 * hk + 4], k[b:b + 1, hk:hk + 1], v[b:b + 1, hk:hk + 1],
+                                       dout[b:b + 1, 4 * hk:4 * hk + 4], window, sinks)
+        for n, x in got.items():
+            x = x[b:b + 1, 4 * hk:4 * hk + 4] if n in ("out", "dq") else x[b:b + 1, hk:hk + 1]
+            assert ((x.double().cpu() - ref[n]).abs() <= tol[n]).all(), (n, b, hk)
