@@ -54,7 +54,8 @@ __device__ __forceinline__ bool window_fwd_pass(const WindowParams& p, int workg
     }
   }
   if (thread < 2) odd[thread] = 0;
-  if (thread == 0) over = 0;
+  // (A second pass leaves it: slower waves may still be about to read it.)
+  if (thread == 0 && !small) over = 0;
 
   Stage<T, D, RT, 64 * NW> sk, sv;
   auto load = [&](int t) {

@@ -4,6 +4,7 @@ small and large gradients, and batches whose workgroups have eight waves."""
 import pytest
 import torch
 
+from dwarf_amd import window_attention
 from oracle import window_oracle as wo
 from tests.test_window_gpu import BF, F16, F32, check, inputs, run
 
@@ -122,3 +123,19 @@ def test_long_rows_of_eight_waves(gpu_device, dtype, D):
         for n, x in got.items():
             x = x[b:b + 1, 4 * hk:4 * hk + 4] if n in ("out", "dq") else x[b:b + 1, hk:hk + 1]
             assert ((x.double().cpu() - ref[n]).abs() <= tol[n]).all(), (n, b, hk)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_largest_values_in_many_workgroups(gpu_device, dtype):
+    """Every workgroup, or every other one, goes over its tiles twice: causal means of values near the largest, of equal scores."""
+    B, H, N, D = 2, 12, 4100, 64
+    g = torch.Generator().manual_seed(7)
+    v = ((1.0 + 0.9 * torch.rand(B, H, N, D, generator=g)) * 2.0 ** 127).to(dtype)
+    v[:, ::3] *= 2.0 ** -40
+    z = torch.zeros(B, H, N, D, dtype=dtype, device=gpu_device)
+    for _ in range(5):
+        out = window_attention(z, z, v.to(gpu_device), N)
+        assert torch.isfinite(out).all()
+    want = v.double().cumsum(2) / torch.arange(1, N + 1, dtype=torch.float64)[:, None]
+    # Weights are 1; 2 N u of the sums, and the result's half step.
+    assert ((out.double().cpu() - want).abs() <= want * (2 * N * 2.0 ** -24 + torch.finfo(dtype).eps / 2 * 1.01)).all()
