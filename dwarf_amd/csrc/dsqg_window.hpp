@@ -269,6 +269,23 @@ __device__ __forceinline__ f32x16_t scores(const char* rows, int l, const u32x4_
   return s;
 }
 
+// The same of rows as they are in memory, of which `have` exist: those of a tile that Stage::clean took something out of.
+template <int T, int D>
+__device__ __forceinline__ f32x16_t scores_as_stored(const char* rows, long long stride, int have, int l, const u32x4_t (&b)[Tile<T, D>::KS]) {
+  using X = Tile<T, D>;
+  asm volatile("");  // (a branch)
+  const int row = operand_row<T>(l);
+  f32x16_t s = zero_tile();
+#pragma unroll
+  for (int e = 0; e < X::KS; ++e) {
+    u32x4_t a = {0u, 0u, 0u, 0u};
+    if (row < have) a = *reinterpret_cast<const u32x4_t*>(rows + row * stride + (2 * e + (l >> 5)) * 16);
+    s = mma<T>(a, b[e], s);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return s;
+}
+
 // Adds what Stage::clean left out of 32 rows, where the lane's column sees it: the rows as they are in memory, of which
 // `have` exist.  A weight above zero times an infinity is that infinity, whatever the weight; where weights have signs, or
 // the value is NaN, the sum is no number either way.  sees(row).

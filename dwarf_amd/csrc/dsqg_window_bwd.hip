@@ -181,7 +181,10 @@ __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 2) void window_dq_kernel(Win
       if (none) continue;
       const char* const kt = lds[t & 1][0] + 32 * kb * X::RB;
       const char* const vt = lds[t & 1][1] + 32 * kb * X::RB;
-      const f32x16_t s = scores<T, D>(kt, l, q), dp = scores<T, D>(vt, l, dout);
+      f32x16_t s = scores<T, D>(kt, l, q);
+      // (A key's infinity may be a score of -infinity: without it that would be another weight.)
+      if (__builtin_expect(odd[t & 1] == t + 1, 0)) s = scores_as_stored<T, D>(kh + k0 * p.k.n, p.k.n, length - k0, l, q);
+      const f32x16_t dp = scores<T, D>(vt, l, dout);
       const Seen seen = {i - p.window + 1 - k0, i - k0, p.sinks - k0};
       float w[16];
 #pragma unroll

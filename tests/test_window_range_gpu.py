@@ -139,3 +139,28 @@ def test_largest_values_in_many_workgroups(gpu_device, dtype):
     want = v.double().cumsum(2) / torch.arange(1, N + 1, dtype=torch.float64)[:, None]
     # Weights are 1; 2 N u of the sums, and the result's half step.
     assert ((out.double().cpu() - want).abs() <= want * (2 * N * 2.0 ** -24 + torch.finfo(dtype).eps / 2 * 1.01)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("N,window,sinks,at", [(230, 45, 2, 100), (230, 45, 5, 3), (700, 600, 0, 40), (300, 300, 0, 299)])
+def test_scores_of_minus_infinity(gpu_device, dtype, N, window, sinks, at):
+    """A key with an infinity, against queries whose score it makes -infinity: they give it no weight, and their gradients are those
+    of the other keys (but for the infinity's own element, 0 times it)."""
+    D = 64
+    q, k, v, dout = inputs(1, 1, 1, N, D, dtype)
+    q[..., 7] = -q[..., 7].abs() - 0.5
+    k[0, 0, at, 7] = torch.inf
+    got = run(q, k, v, dout, window, sinks)
+    seen = wo.sees(N, window, sinks)
+    seen[:, at] = False
+    some = seen.any(-1)  # (query 0 or `at` itself may see nothing else)
+    x, kk, vv = (t[0, 0].double() for t in (q, k, v))
+    kk[at] = 0.0
+    x.requires_grad_()
+    p = torch.softmax((x @ kk.T * D ** -0.5).masked_fill(~seen, -torch.inf)[some], -1)
+    (dq,) = torch.autograd.grad(p @ vv, x, dout[0, 0].double()[some])
+    rest = torch.arange(D) != 7
+    # As in test_gradients_of_few_keys; float32, which rounds no operand, has its sums' roundings, D for a score.
+    bound = torch.finfo(dtype).eps / 2 if dtype != F32 else 2.0 ** -24 * (D * window) ** 0.5
+    assert far_off(got["dq"][0, 0][some][:, rest], dq[some][:, rest]) <= bound
+    assert far_off(got["out"][0, 0][some], (p @ vv).detach()) <= bound
