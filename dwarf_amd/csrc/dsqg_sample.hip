@@ -938,7 +938,7 @@ __global__ __launch_bounds__(kThreads) void sample_maxima_kernel(Sample p) {
 
 // With top-k the list, else the bins' masses.
 template <int DT>
-__global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(Sample p) {
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(Sample p) {
   __shared__ Shared s;
   const int t = threadIdx.x;
   const long long b = blockIdx.x / p.S;
@@ -1057,7 +1057,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(Sample p) {
   finish<DT>(s, p, b, r, w, limits, by_mass ? found[1] : 0, by_mass ? found[2] : 0);
 }
 
-// Workgroups of a row: as many as leave two to a CU, up to kSplit, of 1024 pieces at least.
+// Workgroups of a row: as many as give each CU one, up to kSplit, of 1024 pieces at least.
 int split_of(int B, int V) {
   const long long pieces = V / kVec;
   return (int)std::max(1ll, std::min({(long long)kSplit, 256ll / B, pieces / kThreads}));
