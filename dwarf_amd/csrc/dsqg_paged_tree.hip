@@ -21,7 +21,7 @@
 // weight, of the size of the output's own.  (float16 queries over 8-bit rows, whose operands are bfloat16: two again, for
 // 2^-8 is more than their output's rounding.)  Scores, statistics and sums are fp32.
 //
-// Measured: 16 sequences of up to 8192, 8 key/value heads of 4, 64 nodes, D = 128 over e4m3, 326 us, 266 TFLOP/s: vector
+// Measured: 16 sequences of up to 8192, 8 key/value heads of 4, 64 nodes, D = 128 over e4m3, 309 us, 281 TFLOP/s: vector
 // instructions (a weight's and the codes', of which 32 columns share each) and the latency of two waves a SIMD bound it.
 // 32 sequences of up to 2048, 12 heads, 26 nodes, D = 64 in bfloat16, 42 us, 3.2 TB/s; one node within a window of 1024 of
 // 8191, 25 us, 3.9 TB/s: reads of pages, each wave a tile ahead.  One sequence of 77 in float32, 8 us: a launch's latency.
@@ -374,58 +374,63 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
   };
 
   // Whether a row is seen by any node, and by one that sees `mask` of the draft and stored rows from `from` on.
-  auto seen_by = [&](int t, u64 mask, int from) {
+  auto seen_by = [&](int t, u64 mask, int from) __attribute__((always_inline)) {
     const int j = t - pos;
     return j < 0 ? t >= from || t < p.sinks : j < 64 && ((mask >> j) & 1);
   };
 
-  // e4m3: zeros in the place of the NaN among the tile's value rows, and marks for the sums that see them.
-  auto take_nan = [&](int tile) {
-    asm volatile("");  // (a branch)
-    uint32_t odd = 0;
+  // e4m3: marks for the sums that see a NaN among the tile's staged rows, and zeros in its place.  (Inlined by force, as what it is
+  // called from: out of line, the arrays that these refer to are memory, and the whole kernel takes twice its time.)
+  auto nan_at = [&](int row, int d) __attribute__((always_inline)) {  // of elements 16 d + 4 g on, which this lane sums
+    const val_t* const x = sVw + row * RV + 16 * d + 4 * g;
+    uint32_t in = 0;
 #pragma unroll
-    for (int u = 0; u < V::passes; ++u)
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (FP32) in |= (x[e] != x[e] ? 1u : 0u) << e;
+      else in |= ((x[e] & 0x7fff) > 0x7f80 ? 1u : 0u) << e;
+    }
+    return in;
+  };
+  auto take_nan = [&](int tile) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int w = 0; w < V::per_lane; ++w) odd |= nan_codes(vr[u][w].x) | nan_codes(vr[u][w].y) | nan_codes(vr[u][w].z) | nan_codes(vr[u][w].w);
-    if (!__any(odd != 0)) return;
-#pragma unroll
-    for (int u = 0; u < V::passes; ++u) {
-#pragma unroll
-      for (int w = 0; w < V::per_lane; ++w) {
-        const int row = u * V::rows + l / V::lanes, piece = l % V::lanes + V::lanes * w;
-        uint32_t x[4] = {vr[u][w].x, vr[u][w].y, vr[u][w].z, vr[u][w].w}, gone = 0;  // a bit for each of the piece's codes
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t at = nan_codes(x[q]) >> 7;
-          x[q] &= ~(at * 255u);
-          gone |= ((at & 1u) | (at >> 7 & 2u) | (at >> 14 & 4u) | (at >> 21 & 8u)) << (4 * q);
-        }
-        vr[u][w] = make_uint4(x[0], x[1], x[2], x[3]);
-        if (piece >= V::pieces) gone = 0;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
+    for (int n = 0; n < NQ; ++n) {
+      const u64 mask = sees[n];
+      const int from = lo[n];
+      uint32_t in = sees_nan[wave][n][l];
 #pragma unroll 1
-          for (int c = 0; c < 16; ++c) {
-            const u64 mask = __shfl(sees[n], c, 64);
-            const int from = __shfl(lo[n], c, 64);
-            // Element 16 d + 4 g + e of column c is the sum o[n][d][e] of lane 16 g + c.
-            if (seen_by(tile + row, mask, from))
-              for (uint32_t rest = gone; rest; rest &= rest - 1) {
-                const int b = __builtin_ctz(rest);
-                atomicOr(&sees_nan[wave][n][16 * (b >> 2) + c], 1u << (4 * piece + (b & 3)));
-              }
-          }
-        }
-      }
+      for (int at = 0; at < kTile * DB; ++at)
+        if (seen_by(tile + at / DB, mask, from)) in |= nan_at(at / DB, at % DB) << (4 * (at % DB));
+      sees_nan[wave][n][l] = in;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int at = 0; at < kTile * DB; ++at) {
+      const uint32_t in = nan_at(at / DB, at % DB);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((in >> e) & 1) sVw[at / DB * RV + 16 * (at % DB) + 4 * g + e] = 0;  // (the lanes of a group write the same)
     }
   };
 
   // The tile's value rows to LDS as operand values, zeros in the place of those that nobody sees; says whether an
   // infinity or NaN is among the others of a tile with masks.
-  auto stage = [&](int tile, bool masks) {
+  auto stage = [&](int tile, bool masks) __attribute__((always_inline)) {
     bool odd = false;
-    if constexpr (CT == DSQG_E4M3)
-      if (masks) take_nan(tile);
+    if constexpr (CT == DSQG_E4M3) {
+      if (masks) {
+        asm volatile("");  // (a branch)
+        uint32_t any_nan = 0;
+#pragma unroll
+        for (int u = 0; u < V::passes; ++u)
+#pragma unroll
+          for (int w = 0; w < V::per_lane; ++w)
+            any_nan |= nan_codes(vr[u][w].x) | nan_codes(vr[u][w].y) | nan_codes(vr[u][w].z) | nan_codes(vr[u][w].w);
+        odd = any_nan != 0;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < V::passes; ++u) {
       const int row = u * V::rows + l / V::lanes;
@@ -458,7 +463,10 @@ __global__ __launch_bounds__(kBlock, QT == DSQG_F32 ? 1 : 2) void paged_tree_ker
         }
       }
     }
-    return masks && __any(odd);
+    odd = masks && __any(odd);
+    if constexpr (CT == DSQG_E4M3)
+      if (__builtin_expect(odd, 0)) take_nan(tile);
+    return odd;
   };
 
   float m[NQ], lsum[NQ];  // the weights' reference exponent, the sum over this lane's rows
@@ -769,7 +777,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PagedTree p) {
 // Columns of a workgroup: 16 for each tile of the products.  Larger groups read the cache less often, and take more
 // registers: four tiles where a wave's rows on their way and its sums leave room, those of 8-bit caches of up to 96 elements,
 // else two, and two where queries have two terms or are float32.  (16 sequences of up to 8192, 8 key/value heads, 256 columns,
-// e4m3: four 193 us and two 206 at D = 64, 221 and 269 at 96, 364 and 331 at 128; bfloat16 at 64 either 120.)
+// e4m3: four 183 us and two 194 at D = 64, 214 and 265 at 80, 214 and 260 at 96, 364 and 331 at 128; bfloat16 at 64 either 120.)
 constexpr bool four_tiles(int dtype, int cache_dtype, int D) { return dtype == DSQG_BF16 && narrow(cache_dtype) && D <= 96; }
 
 int group_tiles(int M, int dtype, int cache_dtype, int D) {
