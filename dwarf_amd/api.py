@@ -212,8 +212,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int = 
     are zeros.  softmax_scale defaults to D ** -0.5.  float32, bfloat16 and float16, head dims 32, 64, 80, 96 and 128;
     sums and softmax statistics are fp32 and deterministic, and weights (in the backward their gradients too) are
     rounded once to a 16-bit type before they multiply rows.  What a query does not see does not reach it, whatever
-    it holds.  Outputs are finite where the values are, up to 2^-7 below the type's largest.  There is no second
-    derivative.  ``paged_tree_step`` with the same window and sinks continues over a cache.
+    it holds.  Outputs are finite where the values are, up to 2^-7 below the type's largest.  A training pass in 16 bits keeps,
+    beside out, as much again for what its rounding took off, which the gradients need.  There is no second derivative.
+    ``paged_tree_step`` with the same window and sinks continues over a cache.
     """
     if ops.traced(q, k, v):
         return ops.window_fwd(q, k, v, lengths, window, sinks, softmax_scale)[0]

@@ -20,8 +20,8 @@
 // A row takes one workgroup where there are rows for all CUs; fewer rows are split, each over up to eight, and four launches
 // take the place of the barriers between the steps.  (256 rows of 32000 bfloat16 in two parts each: 65 us, in one 39.)
 //
-// Measured: 1 row of 32000 float32, top-p, 26 us in its four launches (one workgroup: 72); 256 rows of 32000 bfloat16 with top-k,
-// top-p and temperatures of their own, 39 us; 64 rows of 151001 float32, top-p and min-p, 69 us, of which the masses take 40: two
+// Measured: 1 row of 32000 float32, top-p, 25 us in its four launches (one workgroup: 72); 256 rows of 32000 bfloat16 with top-k,
+// top-p and temperatures of their own, 39 us; 64 rows of 151001 float32, top-p and min-p, 62 us, of which the masses take 43: two
 // passes of some 40 vector instructions an element, half of them in 64 bits.  Memory would take 3 and 8 us; a
 // single row's launches wait for memory and for each other.
 #include <algorithm>

@@ -20,9 +20,11 @@
 // p and dS enter the products rounded to the 16-bit type (2^-8 of each in bfloat16, 2^-11 in float16, where factors keep them in
 // its range); float32 operands are not rounded.  Everything else is fp32.
 //
-// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, dq 365 us, dk/dv 485 us, 565 TFLOP/s of the seven products; B8 H8
-// Hkv1 N2048 D32 window 256 with 4 sinks, dq 30 us, dk/dv 43 us, their parts' sum 4.6 us.  Vector instructions bound both: a
-// pair's exponent, weight, dS and masks cost as much at D = 32 as at D = 128.
+// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, dq 383 us, dk/dv 476 us, 560 TFLOP/s of the seven products; B8 H8
+// Hkv8 N2048 D32 window 256 with 4 sinks, dq 32 us, dk/dv 43 us, their parts' sum 4.9 us.  Latency bounds both: vector instructions
+// issue in 28 and 25 % of the cycles at D = 128, matrix instructions in 23 and 25 %, and a tile's scores, weights and products
+// follow each other; at D = 32 vector instructions issue in 25 and 33 %.  float16, with its factors: 1140 us the whole step for
+// bfloat16's 1050.
 #include <algorithm>
 
 #include "dsqg_window.hpp"
@@ -254,7 +256,8 @@ struct KeyBlock {
   }
 };
 
-// Up to `kSingle` elements a wave has the scores, weights and sums of its 32 keys to itself.
+// Up to `kSingle` elements a wave has the scores, weights and sums of its 32 keys to itself.  (Above, pairs: the whole backward at
+// B2 H16 Hkv4 N4096 window 512, bfloat16, D = 80 236 us and 96 248, by single waves 376 and 403; D = 128 see the pairs' kernel.)
 constexpr int kSingle = 64;
 
 template <int T, int D>

@@ -11,9 +11,9 @@
 // operands are not rounded.  Scores, the maximum, the sum and the output's sums are fp32.  For the backward a query's
 // reference exponent m and 1 / sum are kept apart, for m may be too large to hold the sum's logarithm.
 //
-// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, 262 us, 525 TFLOP/s of the two products; B8 H8 Hkv1 N2048 D32 window
-// 256 with 4 sinks, 24 us, 190 TFLOP/s.  Vector instructions and latency bound it: at D = 128 half of the cycles issue
-// vector work and a fifth matrix work, at D = 32 a score costs as many vector instructions for a quarter of the products.
+// Measured (bfloat16): B1 H16 Hkv4 N16384 D128 window 1024, 240 us, 570 TFLOP/s of the two products; B8 H8 Hkv8 N2048 D32 window
+// 256 with 4 sinks, 24 us, 190 TFLOP/s.  Vector instructions and latency bound it: at D = 128 46 % of the cycles issue
+// vector work and 21 % matrix work, at D = 32 a score costs as many vector instructions for a quarter of the products.
 #include "dsqg_window.hpp"
 
 namespace dsqg {

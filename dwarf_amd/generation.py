@@ -40,8 +40,9 @@ class FullCausalAttention(nn.Module):
     """train/train_2048_condU.py:210-245: softmax attention over all earlier tokens, with the
     DSQG layers' output gate.  ``prefill`` / ``step`` keep its K/V rows in a preallocated
     cache for generation.  With a ``window`` (no counterpart in the reference) a token sees the last
-    ``window`` tokens and the first ``sinks``, on the HIP kernels (``window_attention``: head dims 32, 64, 80, 96
-    and 128), and dropout is on the layer's output alone, as in the DSQG layers."""
+    ``window`` tokens and the first ``sinks``: in the forward and the prefill on the HIP kernels (``window_attention``: head
+    dims 32, 64, 80, 96 and 128), in a step over a paged cache too; over a flat one the step attends the whole cache in
+    torch, under a mask.  Dropout is on the layer's output alone, as in the DSQG layers."""
 
     def __init__(self, embedding_dim: int, num_heads: int, dropout: float = 0.1,
                  window: Optional[int] = None, sinks: int = 0):

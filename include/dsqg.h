@@ -431,8 +431,8 @@ int dsqg_paged_decode(const dsqg_paged_decode_args* args, dsqg_stream_t stream);
  * stats [B,H,N,2] (float, contiguous, 8-byte aligned; the forward's may be NULL) holds, for the backward, each query's
  * reference exponent and the inverse of its weights' sum, and low [B,H,N,D], of the inputs' 16-bit dtype, what out's rounding
  * took off (float16: times 2^11).  The backward takes dout . out from both; where low is NULL, from out alone, whose rounding
- * then shows in dq and dk: 3.5 times the error where a query sees few keys.  Scores and sums are fp32, in an order that does not change
- * between calls; the weights and, in the backward, their gradients are rounded once to a 16-bit dtype before they multiply
+ * then shows in dq and dk: 3.5 times the error where a query sees few keys.  Scores and sums are fp32, in an order that does
+ * not change between calls; the weights and, in the backward, their gradients are rounded once to a 16-bit dtype before they multiply
  * rows.  A row that a query does not see does not reach its output, whatever it holds, nor a row of a query that does not
  * see a key that key's gradients.
  *
