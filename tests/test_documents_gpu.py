@@ -21,24 +21,30 @@ def layouts(line):
     return res
 
 
-@pytest.mark.parametrize("document", ["README.md", "INTEGRATION.md"])
+CALL = "cache.tree_step(q, k, v, parents)"
+DOCUMENTS = [p for p in sorted(ROOT.glob("*.md")) if CALL in p.read_text()]
+
+
+def test_documents_are_found():
+    assert len(DOCUMENTS) >= 2
+
+
+@pytest.mark.parametrize("document", DOCUMENTS, ids=lambda p: p.stem)
 def test_drafted_tokens(gpu_device, document):
-    text = (ROOT / document).read_text()
-    line = next(x for x in text.splitlines() if "cache.tree_step(q, k, v, parents)" in x)
+    text = document.read_text()
+    line = next(x for x in text.splitlines() if CALL in x)
+    block = next((b for b in re.findall(r"```python\n(.*?)```", text, re.S) if line in b), None)
     shapes = layouts(line.split("#", 1)[1])
-    sizes = dict(B=2, H=4, H_kv=2, T=5, D=32)  # (all of them different)
+    sizes = dict(B=3, H=4, H_kv=2, T=5, D=32)  # (all of them different)
     g = torch.Generator().manual_seed(0)
     q, k, v = (torch.randn([sizes[x] for x in shapes[n]], generator=g).to(torch.bfloat16).to(gpu_device) for n in "qkv")
-    space = dict(sizes, q=q, k=k, v=v, parents=torch.tensor([[-1, 0, 0, 1, 3]] * 2, device=gpu_device), u=torch.rand(2, 5, generator=g).to(gpu_device),
-                 drafted=torch.randint(0, 9, (2, 5), generator=g).to(gpu_device), logits=lambda x: x.float() @ weights,
+    space = dict(sizes, q=q, k=k, v=v, parents=torch.tensor([[-1, 0, 0, 1, 3]] * 3, device=gpu_device), u=torch.rand(3, 5, generator=g).to(gpu_device),
+                 drafted=torch.randint(0, 9, (3, 5), generator=g).to(gpu_device), logits=lambda x: x.float() @ weights,
                  sample_tokens=dwarf_amd.sample_tokens, draft_tree_accept=dwarf_amd.draft_tree_accept,
-                 cache=dwarf_amd.PagedKVCache(2, 2, 32, 64, torch.bfloat16, gpu_device))
+                 cache=dwarf_amd.PagedKVCache(3, 2, 32, 64, torch.bfloat16, gpu_device))
     weights = torch.randn(4 * 32, 9, generator=g).to(gpu_device)
-    if document == "README.md":
-        exec(line.strip(), space)
-    else:
-        block = next(b for b in re.findall(r"```python\n(.*?)```", text, re.S) if line in b)
-        exec(block, space)
-        assert space["picks"].shape == (2, 5)
+    exec(line.strip() if block is None else block, space)
+    if block is not None:
+        assert space["picks"].shape == (3, 5)
         assert (space["cache"].pos == space["n"]).all() and (space["n"] >= 1).all()
     assert space["out"].shape == tuple(sizes[x] for x in shapes["out"])
