@@ -1079,6 +1079,15 @@ std::tuple<Tensor, Tensor, Tensor> run_window_bwd(const Tensor& q0, const Tensor
                                                   int64_t window, int64_t sinks, std::optional<double> scale) {
   dsqg_window_bwd_args a = {};
   a.shape = window_shape(q0, k0, v0, lengths0, window, sinks, scale);
+  const auto rows = q0.sizes();
+  for (const Tensor* t : {&out0, &low0})
+    require(!t->defined() || (t->sizes() == rows && t->scalar_type() == q0.scalar_type()), "out and low must be ", q0.scalar_type(), " ",
+            shape_str(rows), ", got ", t->scalar_type(), " ", shape_str(t->sizes()));
+  require(!low0.defined() || a.shape.dtype != DSQG_F32, "low is for 16-bit types");
+  require(dout0.sizes() == rows, "dout must be ", shape_str(rows), ", got ", shape_str(dout0.sizes()));
+  require(stats.scalar_type() == at::kFloat && stats.sizes() == c10::IntArrayRef({rows[0], rows[1], rows[2], 2}) && stats.is_contiguous(),
+          "stats must be contiguous float32 ", shape_str({rows[0], rows[1], rows[2], 2}), ", got ", stats.scalar_type(), " ",
+          shape_str(stats.sizes()));
   const c10::Device dev = require_gpu({&q0, &k0, &v0, &lengths0, &out0, &stats, &low0, &dout0});
   const c10::OptionalDeviceGuard guard(dev);
   const Tensor q = window_rows(q0), k = window_rows(k0), v = window_rows(v0), out = window_rows(out0);

@@ -521,7 +521,8 @@ int dsqg_tree_accept(const dsqg_tree_accept_args* args, dsqg_stream_t stream);
  * that a node does not see does not reach it, whatever it holds.  The range of values is dsqg_paged_decode's; its rules
  * for strides, q_stride {b, h, t} and so on, and workspace hold; out is contiguous [B,T,H,D].  Weights enter the sum as
  * two 16-bit terms where T * H / Hkv is at most 16, else as one (16-bit queries).  T is at most DSQG_MAX_TREE, B * H * T
- * less than 2^30, B * Hkv less than 2^24 - 8 and T * H / Hkv at most 2^21 - 32 (EUNSUPPORTED otherwise).  No two sequences may have the same page at positions that a step writes. */
+ * less than 2^30, B * Hkv less than 2^24 - 8 and T * H / Hkv at most 2^21 - 32 (EUNSUPPORTED otherwise).  No two sequences
+ * may have the same page at positions that a step writes. */
 typedef struct {
     dsqg_paged_cache cache;
     int32_t H, T;

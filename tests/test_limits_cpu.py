@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from dwarf_amd import _lib
+from dwarf_amd import _lib, ops
 from tests.test_paged_tree_cpu import _abi
 from tests.test_window_cpu import _fill, _shape
 
@@ -83,3 +84,21 @@ def test_walks_past_the_grid():
     a.B, a.T = 1 << 26, 1
     a.tokens = a.parents = a.picks = a.path = a.n = a.next = 0x10000
     assert _lib.load().dsqg_tree_accept(ctypes.byref(a), None) == _lib.DSQG_EUNSUPPORTED
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=torch.zeros(2, 4, 8, 32).bfloat16()), dict(out=torch.zeros(2, 4, 9, 32)), dict(dout=torch.zeros(2, 2, 9, 32).bfloat16()),
+    dict(stats=torch.zeros(2, 4, 9)), dict(stats=torch.zeros(2, 4, 9, 2).bfloat16()), dict(stats=torch.zeros(2, 4, 2, 9).transpose(2, 3)),
+    dict(low=torch.zeros(2, 2, 9, 32).bfloat16()), dict(low=torch.zeros(2, 4, 9, 32)),
+])
+def test_window_backward_operands(change):
+    """The backward's operator by itself: shapes and types are checked, and then only the GPU is missing."""
+    def t(heads):
+        return torch.zeros(2, heads, 9, 32).bfloat16()
+
+    a = dict(q=t(4), k=t(2), v=t(2), lengths=None, out=t(4), stats=torch.zeros(2, 4, 9, 2), dout=t(4), window=4, sinks=1, softmax_scale=None,
+             low=t(4))
+    with pytest.raises(RuntimeError, match="GPU"):
+        ops.window_bwd(**a)
+    with pytest.raises(AssertionError):
+        ops.window_bwd(**{**a, **change})
